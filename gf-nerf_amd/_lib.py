@@ -25,7 +25,7 @@ class LaunchOpts(C.Structure):
 MERGE_OFF, MERGE_ON, MERGE_DEVICE = 0, 1, 2  # GFN_MERGE_*
 _opts = C.POINTER(LaunchOpts)
 
-ABI_VERSION = 108  # = GFN_ABI_VERSION of the include/gfnerf_amd.h the SIGNATURES below were written for; lib() refuses any other library
+ABI_VERSION = 109  # = GFN_ABI_VERSION of the include/gfnerf_amd.h the SIGNATURES below were written for; lib() refuses any other library
 
 # name -> (restype, argtypes); must list every function include/gfnerf_amd.h declares
 SIGNATURES = {
@@ -108,6 +108,15 @@ SIGNATURES = {
     "gfn_copy_list": (_i32, [_vp, _vp, _vp, _i32, _vp]),
     "gfn_fill_zero": (_i32, [_vp, _i64, _vp]),
     "gfn_reduce_shards": (_i32, [_vp, _i32, _i64, _i32, _f32, _vp, _vp]),
+    "gfn_gated_fwd": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "gfn_gated_bwd_workspace": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "gfn_gated_bwd": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "gfn_ray_scan_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp, _vp, _i32, _vp]),
+    "gfn_ray_scan_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp,
+                                _i32, _vp]),
+    "gfn_ray_scan_step": (_i32, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
+    "gfn_dropout": (_i32, [_vp, _i64, _i64, _i32, _i32, _f32, _u64, _vp, _vp, _i64, _vp]),
+    "gfn_dropout_call": (_i32, [_vp, _vp, _vp]),
     "gfn_octree_build_host": (_i32, [_vp, _vp, _vp, _i64, _i32, _f32, _f32, _u64, _i32, C.POINTER(_vp),
                                      C.POINTER(_i64), C.POINTER(_vp), C.POINTER(_i64)]),
     "gfn_free_host": (None, [_vp]),

@@ -24,7 +24,8 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libgfnerf_amd.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
-HIP_SOURCES = ["runtime.hip", "hash3d.hip", "lm_lookup.hip", "sampler.hip", "mlp.hip", "field.hip", "field_x3.hip", "fused_fwd.hip", "wgrad_x3.hip", "render.hip", "batch.hip", "grad_part.hip", "octree_proc.hip"]
+HIP_SOURCES = ["runtime.hip", "hash3d.hip", "lm_lookup.hip", "sampler.hip", "mlp.hip", "field.hip", "field_x3.hip", "fused_fwd.hip", "wgrad_x3.hip", "render.hip", "batch.hip", "grad_part.hip", "octree_proc.hip",
+               "gated.hip", "ray_scan.hip", "dropout.hip"]
 CXX_SOURCES = ["octree_build.cpp", "octree_proc.cpp"]
 HIPCC_FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-ffp-contract=off", "-Wall",
                "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", INCLUDE]
@@ -81,7 +82,7 @@ def build_extension(force=False, verbose=False):
 
 def _build_locked(force, verbose):
     os.makedirs(OBJ, exist_ok=True)
-    headers = [os.path.join(CSRC, h) for h in ("gfn_common.h", "x3_device.h", "hash_device.h")]
+    headers = [os.path.join(CSRC, h) for h in ("gfn_common.h", "x3_device.h", "hash_device.h", "gated_device.h")]
     headers += [os.path.join(INCLUDE, "gfnerf_amd.h")]
     hipcc = _hipcc()
     jobs, objs, keys = [], [], []

@@ -1,0 +1,576 @@
+// gated.hip -- the gated feed-forward layer  h = act(x Wg^T + bg) * (x Wu^T + bu)  and its backward pass.
+//
+// Forward.  Weights are the MFMA's A operand (rows = hidden features), samples its columns, so a lane owns ONE sample and, with
+// the feature rows of two 16-row tiles dealt out as 32 p + 8 (i >> 2) + 4 t + (i & 3), eight CONSECUTIVE features of it for both
+// projections: activation and product happen in its registers and leave as one 16-byte store (four lanes write 64 bytes of a row).
+// The weights of a block of features sit in LDS for the life of the workgroup; a wave keeps the inputs of 16 G samples in
+// registers and passes over the features once.  Nothing but x, the weights and h touches memory.
+//
+// Backward.  g and u are formed again (they are cheaper than the two N x H arrays a saved forward would read back), then
+//   dg = dh u act'(g), du = dh act(g)          in registers, eight consecutive features of a sample in each lane -- which is the
+//   dx = dg Wg + du Wu                         B operand of this product as it stands (contraction over the features; the A operand
+//                                              is W transposed, read from the same LDS image with transposing reads);
+//   [dWg; dWu] = [dg; du]^T x                  contracts over the samples: the wave's dz goes to LDS and every wave accumulates its own
+//                                              rows of dW over all samples of the tile, in registers until the workgroup's last tile.
+// One pass: x and dh are read once, dx is written once; each workgroup's partial dW goes to a workspace and a second launch adds the
+// partials in a fixed order (no atomics: the same bits every run).  The biases' gradients are one more column of dW: x gets a column
+// of ones behind its last (and W the bias there, so the recomputed g and u have it too).
+// dz is rounded to the operands' type for the two products -- 2^-9 (bf16) / 2^-12 (f16) per term, below the rounding of the results
+// themselves; f32 stays f32.  f16 has the precision but not the range: see tile_scale.
+#include "gated_device.h"
+
+namespace {
+
+constexpr int kWaves = 4;
+
+// row i of tile t <-> hidden feature 32 p + 8 (i >> 2) + 4 t + (i & 3); the LDS image keeps rows in tile order
+__device__ __forceinline__ int image_feature(int row) { return (row & ~31) + 8 * ((row & 15) >> 2) + 4 * ((row >> 4) & 1) + (row & 3); }
+
+// [2 matrices][HC rows][KS units + one piece]: the odd number of pieces a row keeps 16 rows' equal pieces on different banks.
+template <typename T, int KS>
+__device__ __forceinline__ void stage_weights(char* lds, const T* wg, const T* wu, const T* bg, const T* bu, int k, int h, int h0, int hc) {
+  constexpr int PIECES = 4 * KS, ROW = PIECES * 16 + 16, E = Piece<T>::E;
+  for (int e = threadIdx.x; e < 2 * hc * PIECES; e += blockDim.x) {
+    const int row = e / PIECES, c = e - row * PIECES, m = row >= hc;
+    const int f = h0 + image_feature(row - m * hc);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (f < h) {
+      v = row_piece(((m ? wu : wg) + (int64_t)f * k), c, k);
+      if (bg && k / E == c) {  // the bias, behind the last weight
+        T t[E];
+        __builtin_memcpy(t, &v, 16);
+#pragma unroll
+        for (int i = 0; i < E; i++)
+          if (i == k % E) t[i] = (m ? bu : bg)[f];
+        __builtin_memcpy(&v, t, 16);
+      }
+    }
+    *reinterpret_cast<u32x4*>(lds + row * ROW + c * 16) = v;
+  }
+}
+
+template <typename T, int KS, int G>
+__global__ __launch_bounds__(64 * kWaves) void gated_fwd_kernel(int64_t n_max, const int32_t* __restrict__ n_dev, const T* __restrict__ x, int64_t ldx,
+                                                               const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg,
+                                                               const T* __restrict__ bu, int k, int h, int hc, int act, T* __restrict__ out, int64_t ldo) {
+  constexpr int ROW = KS * 64 + 16;
+  constexpr bool EXACT = sizeof(T) == 4;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  float* bias = reinterpret_cast<float*>(lds + 2 * hc * ROW);  // [2][hc] in tile order
+  const int h0 = blockIdx.y * hc;
+  stage_weights<T, KS>(lds, wg, wu, (const T*)nullptr, (const T*)nullptr, k, h, h0, hc);
+  for (int e = threadIdx.x; e < 2 * hc; e += blockDim.x) {
+    const int m = e >= hc, f = h0 + image_feature(e - m * hc);
+    bias[e] = bg && f < h ? (float)(m ? bu : bg)[f] : 0.f;
+  }
+  __syncthreads();
+  const int64_t n = gfn_live_n(n_max, n_dev);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, kg = lane >> 4;
+  const int pairs = ((h - h0 < hc ? h - h0 : hc) + 31) / 32;
+  const char* wrow = lds + j * ROW + kg * 16;
+  for (int64_t s0 = ((int64_t)blockIdx.x * kWaves + wave) * 16 * G; s0 < n; s0 += (int64_t)gridDim.x * kWaves * 16 * G) {
+    u32x4 xr[G][KS];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int64_t s = s0 + 16 * g + j;
+#pragma unroll
+      for (int u = 0; u < KS; u++) xr[g][u] = s < n ? row_piece(x + s * ldx, 4 * u + kg, k) : u32x4{0u, 0u, 0u, 0u};
+    }
+    for (int p = 0; p < pairs; p++) {
+      f32x4 acc[2][2][G];  // [matrix][tile]
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          const f32x4 b = *reinterpret_cast<const f32x4*>(bias + m * hc + 32 * p + 16 * t + 4 * kg);
+#pragma unroll
+          for (int g = 0; g < G; g++) acc[m][t][g] = b;
+        }
+#pragma unroll
+      for (int u = 0; u < KS; u++)
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(wrow + (m * hc + 32 * p + 16 * t) * ROW + u * 64);
+#pragma unroll
+            for (int g = 0; g < G; g++) acc[m][t][g] = mma(w, xr[g][u], acc[m][t][g], (T*)nullptr);
+          }
+      const int f = h0 + 32 * p + 8 * kg;
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const int64_t s = s0 + 16 * g + j;
+        float v[8];
+        gated8<EXACT>(act, [&](int i) { return acc[0][i >> 2][g][i & 3]; }, [&](int i) { return acc[1][i >> 2][g][i & 3]; }, v);
+        if (s < n) store_row<T, 8>(out + s * ldo + f, h - f, v);
+      }
+    }
+  }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------------------
+// dz in f16: dh may be anywhere in f16's range, so the tile's dz are formed under a power of two that brings its largest |dh| into
+// [2^-5, 1) -- |u act'(g)| and |act(g)| up to 65504 still fit, and what is 2^-20 of the tile's largest is still exact to 2^-4.  dx is
+// scaled back per tile; dW's accumulators follow the running scale (rescaled when a tile's differs: the power moves in steps of 2^4, so
+// hardly ever).
+__device__ __forceinline__ int tile_scale_exponent(float largest, int before) {
+  const int e = (int)((__builtin_bit_cast(uint32_t, largest) >> 23) & 0xffu) - 127;
+  if (e < -60 || e > 60) return before;  // zero, or not finite: nothing to preserve
+  return (-(e + 1) >> 2) * 4;
+}
+__device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23); }
+
+// four rows r0 .. r0 + 3 (one for each lane quarter of a 16-lane group) x 16 columns come back column-major: lane i gets column
+// (i & 3) of the 8-byte piece lane 4 q + (i >> 2) points at, rows q = 0 .. 3.
+__device__ __forceinline__ u32x2 tr4(const char* a) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a));
+}
+
+struct GatedBwd {
+  int64_t n_max;
+  const int32_t* n_dev;
+  const void *x, *wg, *wu, *bg, *bu, *dh;
+  int64_t ldx, lddh, lddx;
+  int k, h, h0, act;
+  void* dx;           // T, or null
+  float* dx_sum;      // f32 [n_max][k] between the launches of several feature blocks, or null
+  int dx_first, dx_last;
+  float* part;        // [workgroup][64 NP][KP] f32, or null
+};
+
+template <typename T, int KS, int NP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
+  constexpr int E = Piece<T>::E, TPU = sizeof(T) == 4 ? 1 : 2;  // 16-column tiles a unit
+  constexpr int KP = KS * 4 * E, KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP;
+  constexpr int SAMPLES = 16 * WAVES, ZROW = 64 * (int)sizeof(T) + 16;
+  constexpr int FT_WAVES = WAVES / 4, KT_WAVE = (KT + FT_WAVES - 1) / FT_WAVES;  // waves that share a row tile of dW, its column tiles a wave
+  constexpr bool EXACT = sizeof(T) == 4, SCALED = sizeof(T) == 2 && !__is_same(T, __bf16);
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  char* xs = lds + 2 * HB * ROW;        // [SAMPLES][ROW]
+  char* zs = xs + SAMPLES * ROW;        // [SAMPLES][dg 32 | du 32]
+  float* top = reinterpret_cast<float*>(zs + SAMPLES * ZROW);  // [WAVES]
+  const T *x = static_cast<const T*>(a.x), *dh = static_cast<const T*>(a.dh);
+  const bool ones = a.bg != nullptr;
+  const int k = a.k, h = a.h, h0 = a.h0, act = a.act;
+  stage_weights<T, KS>(lds, static_cast<const T*>(a.wg), static_cast<const T*>(a.wu), static_cast<const T*>(a.bg), static_cast<const T*>(a.bu), k, h, h0, HB);
+  const int64_t n = gfn_live_n(a.n_max, a.n_dev);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, kg = lane >> 4;
+  const int ft = wave & 3, kt0 = (wave >> 2) * KT_WAVE;
+  f32x4 dw[NP][KT_WAVE];
+#pragma unroll
+  for (int p = 0; p < NP; p++)
+#pragma unroll
+    for (int t = 0; t < KT_WAVE; t++) dw[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int run_e = 0;  // dw holds the sums times 2^run_e
+  const char* wrow = lds + j * ROW + kg * 16;
+  const int64_t tiles = (n + SAMPLES - 1) / SAMPLES;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t s = tile * SAMPLES + wave * 16 + j;
+    u32x4 xr[KS];
+#pragma unroll
+    for (int u = 0; u < KS; u++) {
+      const int c = 4 * u + kg;
+      xr[u] = s < n ? row_piece(x + s * a.ldx, c, k) : u32x4{0u, 0u, 0u, 0u};
+      if (ones && s < n && k / E == c) {
+        T t[E];
+        __builtin_memcpy(t, &xr[u], 16);
+#pragma unroll
+        for (int i = 0; i < E; i++)
+          if (i == k % E) t[i] = (T)1.f;
+        __builtin_memcpy(&xr[u], t, 16);
+      }
+    }
+    float d[NP][8];
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      const int f = h0 + 32 * p + 8 * kg;
+      if (s < n) {
+        load_row8(dh + s * a.lddh + f, h - f, d[p]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) d[p][i] = 0.f;
+      }
+    }
+    __syncthreads();  // the weights are staged (first tile); the tile before has been read from xs, zs and top
+#pragma unroll
+    for (int u = 0; u < KS; u++) *reinterpret_cast<u32x4*>(xs + (wave * 16 + j) * ROW + u * 64 + kg * 16) = xr[u];
+    float back = 1.f;
+    if constexpr (SCALED) {
+      float m = 0.f;
+#pragma unroll
+      for (int p = 0; p < NP; p++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, __builtin_fabsf(d[p][i]));
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+      if (lane == 0) top[wave] = m;
+      __syncthreads();
+      m = top[0];
+#pragma unroll
+      for (int w = 1; w < WAVES; w++) m = fmaxf(m, top[w]);
+      const int e = __builtin_amdgcn_readfirstlane(tile_scale_exponent(m, run_e));
+      const float to = pow2(e);
+      back = pow2(-e);
+#pragma unroll
+      for (int p = 0; p < NP; p++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) d[p][i] *= to;
+      if (e != run_e) {
+        const float by = pow2(e - run_e);
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+#pragma unroll
+          for (int t = 0; t < KT_WAVE; t++) dw[p][t] *= by;
+        run_e = e;
+      }
+    }
+    f32x4 dx[KT];
+#pragma unroll
+    for (int t = 0; t < KT; t++) dx[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      f32x4 acc[2][2];
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int t = 0; t < 2; t++) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < KS; u++)
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+            acc[m][t] = mma(*reinterpret_cast<const u32x4*>(wrow + (m * HB + 32 * p + 16 * t) * ROW + u * 64), xr[u], acc[m][t], (T*)nullptr);
+      T z[2][8];
+      gated8_grad<EXACT>(act, [&](int i) { return acc[0][i >> 2][i & 3]; }, [&](int i) { return acc[1][i >> 2][i & 3]; }, d[p], z[0], z[1]);
+      if (a.dx || a.dx_sum) {  // dx[k] += sum over these 32 features
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int m = 0; m < 2; m++) {
+            const u32x4 b = __builtin_bit_cast(u32x4, z[m]);
+            // features 8 kg .. + 3 are image rows 4 kg .. + 3 of tile 0, the next four those of tile 1
+            const char* r = lds + (m * HB + 32 * p + 4 * kg + (j >> 2)) * ROW;
+#pragma unroll
+            for (int t = 0; t < KT; t++) {
+              const char* q = r + (32 * (t >> 1) + 8 * (j & 3) + 4 * (t & 1)) * 2;
+              const u32x2 lo = tr4(q), hi = tr4(q + 16 * ROW);
+              dx[t] = mma(u32x4{lo[0], lo[1], hi[0], hi[1]}, b, dx[t], (T*)nullptr);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const char* r = lds + (m * HB + 32 * p + 4 * kg + 16 * (i >> 2) + (i & 3)) * ROW;
+#pragma unroll
+              for (int t = 0; t < KT; t++)
+                dx[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(*reinterpret_cast<const float*>(r + (16 * t + j) * 4), (float)z[m][i], dx[t], 0, 0, 0);
+            }
+        }
+      }
+      if (a.part) {
+        if (p) __syncthreads();  // the features before have been read
+        char* zr = zs + (wave * 16 + j) * ZROW + 8 * kg * sizeof(T);
+        __builtin_memcpy(__builtin_assume_aligned(zr, 16), z[0], sizeof(z[0]));
+        __builtin_memcpy(__builtin_assume_aligned(zr + 32 * sizeof(T), 16), z[1], sizeof(z[1]));
+        __syncthreads();
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int c = 0; c < SAMPLES; c += 32) {  // rows 8 kg .. 8 kg + 7 of these 32 samples
+            const char* r = zs + (c + 8 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
+            const u32x2 l = tr4(r), u = tr4(r + 4 * ZROW);
+            const u32x4 av = {l[0], l[1], u[0], u[1]};
+            const char* q = xs + (c + 8 * kg + (j >> 2)) * ROW + 4 * (j & 3) * 2;
+#pragma unroll
+            for (int t = 0; t < KT_WAVE; t++)
+              if (KT % FT_WAVES == 0 || kt0 + t < KT) {
+                const u32x2 lo = tr4(q + 32 * (kt0 + t)), hi = tr4(q + 32 * (kt0 + t) + 4 * ROW);
+                dw[p][t] = mma(av, u32x4{lo[0], lo[1], hi[0], hi[1]}, dw[p][t], (T*)nullptr);
+              }
+          }
+        } else {
+#pragma unroll 4
+          for (int c = 0; c < SAMPLES; c += 4) {
+            const float av = *reinterpret_cast<const float*>(zs + (c + kg) * ZROW + (16 * ft + j) * 4);
+            const char* q = xs + (c + kg) * ROW + j * 4;
+#pragma unroll
+            for (int t = 0; t < KT_WAVE; t++)
+              if (KT % FT_WAVES == 0 || kt0 + t < KT)
+                dw[p][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av, *reinterpret_cast<const float*>(q + 64 * (kt0 + t)), dw[p][t], 0, 0, 0);
+          }
+        }
+      }
+    }
+    if ((a.dx || a.dx_sum) && s < n) {  // lane (j, kg) holds columns 16 t' + 4 kg + r of sample j; two 16-bit tiles a unit: 32 u + 8 kg + 4 t + r
+#pragma unroll
+      for (int u = 0; u < KS; u++) {
+        constexpr int W = 4 * TPU;
+        const int col = KP / KS * u + W * kg;
+        float v[W];
+#pragma unroll
+        for (int i = 0; i < W; i++) v[i] = dx[TPU * u + (i >> 2)][i & 3] * back;
+        if (col < k) {
+          if (!a.dx_first) {
+#pragma unroll
+            for (int i = 0; i < W; i++)
+              if (col + i < k) v[i] += a.dx_sum[s * k + col + i];
+          }
+          if (a.dx_last) {
+            store_row<T, W>(static_cast<T*>(a.dx) + s * a.lddx + col, k - col, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; i++)
+              if (col + i < k) a.dx_sum[s * k + col + i] = v[i];
+          }
+        }
+      }
+    }
+  }
+  if (a.part) {
+    const float back = pow2(-run_e);
+    float* o = a.part + (int64_t)blockIdx.x * (64 * NP * KP);
+#pragma unroll
+    for (int p = 0; p < NP; p++)
+#pragma unroll
+      for (int t = 0; t < KT_WAVE; t++)
+        if (KT % FT_WAVES == 0 || kt0 + t < KT)
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[(64 * p + 16 * ft + 4 * kg + r) * KP + 16 * (kt0 + t) + j] = dw[p][t][r] * back;
+  }
+}
+
+// dW[f][c] = sum over the workgroups of part[f's row][c], in their order: 32 columns x 8 runs of workgroups a block
+template <typename T>
+__global__ __launch_bounds__(256) void gated_reduce_kernel(const float* __restrict__ part, int parts, int rows, int kp, int k, int h, int h0, int cols,
+                                                           T* __restrict__ dwg, T* __restrict__ dwu, T* __restrict__ dbg, T* __restrict__ dbu) {
+  __shared__ float sums[8][32];
+  const int col = threadIdx.x & 31, run = threadIdx.x >> 5, row = blockIdx.y;
+  const int c = blockIdx.x * 32 + col, f = h0 + (row >> 6) * 32 + (row & 31);
+  const int per = (parts + 7) / 8;
+  float s = 0.f;
+  if (c < cols && f < h)
+    for (int b = run * per; b < parts && b < (run + 1) * per; b++) s += part[((int64_t)b * rows + row) * kp + c];
+  sums[run][col] = s;
+  __syncthreads();
+  if (run || c >= cols || f >= h) return;
+#pragma unroll
+  for (int r = 1; r < 8; r++) s += sums[r][col];
+  const bool up = (row >> 5) & 1;
+  if (c < k) (up ? dwu : dwg)[(int64_t)f * k + c] = (T)s;
+  else (up ? dbu : dbg)[f] = (T)s;
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------
+constexpr int kMaxIn = 128, kMaxHidden = 1024;
+
+int check_common(const char* who, int64_t n_max, int k, int h, int dtype, int act) {
+  GFN_CHECK_ARG(n_max >= 0 && n_max < (1ll << 31), "%s: n_max=%lld", who, (long long)n_max);
+  GFN_CHECK_ARG(k >= 1 && k <= kMaxIn && h >= 1 && h <= kMaxHidden, "%s: dims %dx%d unsupported (in 1..%d, hidden 1..%d)", who, k, h, kMaxIn, kMaxHidden);
+  GFN_CHECK_ARG(dtype >= GFN_F32 && dtype <= GFN_F16, "%s: dtype %d", who, dtype);
+  GFN_CHECK_ARG(act >= 0 && act <= 3, "%s: act %d", who, act);
+  return GFN_OK;
+}
+
+template <typename K>
+int allow_lds(K kernel, size_t bytes) {  // above the 64 KB a kernel may use without asking
+  GFN_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return GFN_OK;
+}
+
+struct GatedFwd {
+  const void *x, *wg, *wu, *bg, *bu;
+  int64_t ldx, ldo, n_max;
+  const int32_t* n_dev;
+  int k, h, act;
+  void* out;
+};
+
+template <typename T, int KS, int G>
+int launch_fwd(const GatedFwd& a, hipStream_t st) {
+  constexpr int ROW = KS * 64 + 16;
+  const int hp = (a.h + 31) & ~31;
+  const int64_t tiles = (a.n_max + 16 * G * kWaves - 1) / (16 * G * kWaves);
+  // features a workgroup: all of them (x is read once) while there are samples enough for every CU, else blocks of 32
+  int hc = hp < 128 ? hp : 128;
+  if ((size_t)2 * hc * ROW > 80 * 1024) hc = 64;
+  if (tiles < 256) hc = 32;
+  const size_t bytes = (size_t)2 * hc * (ROW + 4);
+  static unsigned long long seen = 0;
+  if (gfn_first_call_on_device(seen))
+    if (int rc = allow_lds(gated_fwd_kernel<T, KS, G>, 160 * 1024)) return rc;
+  const int64_t at_once = 256 * (int64_t)(160 * 1024 / (bytes + 512) < 4 ? 160 * 1024 / (bytes + 512) : 4);
+  const int64_t blocks = tiles < at_once ? tiles : at_once;
+  const dim3 grid((unsigned)blocks, (unsigned)((hp + hc - 1) / hc));
+  gated_fwd_kernel<T, KS, G><<<grid, 64 * kWaves, bytes, st>>>(a.n_max, a.n_dev, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.wg),
+                                                              static_cast<const T*>(a.wu), static_cast<const T*>(a.bg), static_cast<const T*>(a.bu), a.k, a.h,
+                                                              hc, a.act, static_cast<T*>(a.out), a.ldo);
+  GFN_CHECK_LAUNCH();
+  return GFN_OK;
+}
+
+template <typename T>
+int dispatch_fwd(const GatedFwd& a, hipStream_t st) {
+  const int units = (a.k + 4 * Piece<T>::E - 1) / (4 * Piece<T>::E);
+  const bool few = a.n_max < 16384;  // a sample group a wave: more workgroups
+#define GFN_GATED(KS, G)                                                             \
+  if (units <= KS) return few ? launch_fwd<T, KS, 1>(a, st) : launch_fwd<T, KS, G>(a, st)
+  GFN_GATED(1, 4);
+  GFN_GATED(2, 4);
+  if constexpr (sizeof(T) == 4) {
+    GFN_GATED(4, 4);
+    GFN_GATED(8, 2);
+  } else {
+    GFN_GATED(3, 4);
+    GFN_GATED(4, 4);
+  }
+#undef GFN_GATED
+  return GFN_ERR_ARG;
+}
+
+// The backward's plan for (n, k + bias, h, type): units a row, feature blocks of 32 NP, waves and workgroups.
+struct BwdPlan {
+  int ks, np, waves, blocks, launches;
+  size_t lds, part_floats;
+  bool dx_sum;
+};
+
+BwdPlan plan_bwd(int64_t n, int k, int h, int dtype, bool bias) {
+  BwdPlan p;
+  const int e = dtype == GFN_F32 ? 4 : 8, size = dtype == GFN_F32 ? 4 : 2;
+  const int units = (k + (bias ? 1 : 0) + 4 * e - 1) / (4 * e);
+  p.ks = units;
+  if (dtype == GFN_F32 && units > 5) p.ks = 9;
+  p.waves = dtype != GFN_F32 && units >= 4 ? 8 : 4;
+  const int most = dtype == GFN_F32 ? (p.ks > 5 ? 2 : 4) : (p.ks > 4 ? 2 : 4);  // 32-feature pairs a launch: the weights and dW's accumulators fit
+  const int pairs = (h + 31) / 32;
+  p.np = pairs >= 3 && most == 4 ? 4 : pairs >= 2 ? 2 : 1;
+  p.launches = (pairs + p.np - 1) / p.np;
+  const int row = p.ks * 64 + 16, samples = 16 * p.waves;
+  p.lds = (size_t)64 * p.np * row + (size_t)samples * row + (size_t)samples * (64 * size + 16) + 64;
+  const int64_t tiles = (n + samples - 1) / samples;
+  const int at_once = 256 * (p.lds <= 80 * 1024 ? 2 : 1);
+  p.blocks = (int)(tiles < at_once ? tiles : at_once);
+  if (p.blocks < 1) p.blocks = 1;
+  p.part_floats = (size_t)p.blocks * 64 * p.np * (p.ks * 4 * e);
+  p.dx_sum = p.launches > 1;
+  return p;
+}
+
+template <typename T, int KS, int NP, int WAVES>
+int launch_bwd(const GatedBwd& a, const BwdPlan& p, hipStream_t st) {
+  static unsigned long long seen = 0;
+  if (gfn_first_call_on_device(seen))
+    if (int rc = allow_lds(gated_bwd_kernel<T, KS, NP, WAVES>, 160 * 1024)) return rc;
+  gated_bwd_kernel<T, KS, NP, WAVES><<<p.blocks, 64 * WAVES, p.lds, st>>>(a);
+  GFN_CHECK_LAUNCH();
+  return GFN_OK;
+}
+
+template <typename T>
+int dispatch_bwd(const GatedBwd& a, const BwdPlan& p, hipStream_t st) {
+#define GFN_GATED_NP(KS, NP, WAVES) \
+  if (p.ks == KS && p.np == NP) return launch_bwd<T, KS, NP, WAVES>(a, p, st)
+#define GFN_GATED(KS, WAVES)   \
+  GFN_GATED_NP(KS, 1, WAVES);  \
+  GFN_GATED_NP(KS, 2, WAVES);  \
+  GFN_GATED_NP(KS, 4, WAVES)
+  if constexpr (sizeof(T) == 4) {
+    GFN_GATED(1, 4);
+    GFN_GATED(2, 4);
+    GFN_GATED(3, 4);
+    GFN_GATED(4, 4);
+    GFN_GATED(5, 4);
+    GFN_GATED_NP(9, 1, 4);
+    GFN_GATED_NP(9, 2, 4);
+  } else {
+    GFN_GATED(1, 4);
+    GFN_GATED(2, 4);
+    GFN_GATED(3, 4);
+    GFN_GATED(4, 8);
+    GFN_GATED_NP(5, 1, 8);
+    GFN_GATED_NP(5, 2, 8);
+  }
+#undef GFN_GATED
+#undef GFN_GATED_NP
+  gfn_set_error("gfn_gated_bwd: no kernel for %d units x %d", p.ks, p.np);
+  return GFN_ERR_ARG;
+}
+
+template <typename T>
+int gated_bwd_typed(GatedBwd a, const BwdPlan& p, int kp, void* dwg, void* dwu, void* dbg, void* dbu, hipStream_t st) {
+  const int cols = a.k + (a.bg ? 1 : 0);
+  for (int l = 0; l < p.launches; l++) {
+    a.h0 = l * 32 * p.np;
+    a.dx_first = l == 0;
+    a.dx_last = l == p.launches - 1;
+    if (int rc = dispatch_bwd<T>(a, p, st)) return rc;
+    if (a.part) {
+      gated_reduce_kernel<T><<<dim3((unsigned)((cols + 31) / 32), (unsigned)(64 * p.np)), 256, 0, st>>>(
+          a.part, p.blocks, 64 * p.np, kp, a.k, a.h, a.h0, cols, static_cast<T*>(dwg), static_cast<T*>(dwu), static_cast<T*>(dbg), static_cast<T*>(dbu));
+      GFN_CHECK_LAUNCH();
+    }
+  }
+  return GFN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gfn_gated_fwd(const void* x, int64_t ldx, const void* wg, const void* wu, const void* bg, const void* bu, int64_t n_max, const int32_t* n_dev,
+                  int in_dim, int hidden, int dtype, int act, void* out, int64_t ldo, void* stream) {
+  if (int rc = check_common("gfn_gated_fwd", n_max, in_dim, hidden, dtype, act)) return rc;
+  if (n_max == 0) return GFN_OK;
+  GFN_CHECK_ARG(x && wg && wu && out, "gfn_gated_fwd: null pointer");
+  GFN_CHECK_ARG(!bg == !bu, "gfn_gated_fwd: one bias without the other");
+  GFN_CHECK_ARG(ldx >= in_dim && ldo >= hidden, "gfn_gated_fwd: row strides %lld / %lld below %d / %d", (long long)ldx, (long long)ldo, in_dim, hidden);
+  const GatedFwd a{x, wg, wu, bg, bu, ldx, ldo, n_max, n_dev, in_dim, hidden, act, out};
+  hipStream_t st = gfn_stream(stream);
+  if (dtype == GFN_F32) return dispatch_fwd<float>(a, st);
+  if (dtype == GFN_BF16) return dispatch_fwd<__bf16>(a, st);
+  return dispatch_fwd<_Float16>(a, st);
+}
+
+int64_t gfn_gated_bwd_workspace(int64_t n_max, int in_dim, int hidden, int dtype, int bias, int need_dx, int need_dw) {
+  if (check_common("gfn_gated_bwd_workspace", n_max, in_dim, hidden, dtype, 0)) return GFN_ERR_ARG;
+  const BwdPlan p = plan_bwd(n_max, in_dim, hidden, dtype, bias != 0);
+  int64_t bytes = need_dw ? (int64_t)p.part_floats * 4 : 0;
+  if (need_dx && p.dx_sum) bytes += n_max * (int64_t)in_dim * 4;
+  return bytes;
+}
+
+int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, const void* bg, const void* bu, const void* dh, int64_t lddh, int64_t n_max,
+                  const int32_t* n_dev, int in_dim, int hidden, int dtype, int act, void* dx, int64_t lddx, void* dwg, void* dwu, void* dbg, void* dbu,
+                  void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = check_common("gfn_gated_bwd", n_max, in_dim, hidden, dtype, act)) return rc;
+  GFN_CHECK_ARG(wg && wu && (n_max == 0 || (x && dh)), "gfn_gated_bwd: null pointer");
+  GFN_CHECK_ARG(!bg == !bu, "gfn_gated_bwd: one bias without the other");
+  GFN_CHECK_ARG(!dwg == !dwu, "gfn_gated_bwd: one weight gradient without the other");
+  GFN_CHECK_ARG((dbg != nullptr) == (dbu != nullptr) && (dbg != nullptr) == (dwg != nullptr && bg != nullptr), "gfn_gated_bwd: the biases' gradients go with the biases and the weights' gradients");
+  GFN_CHECK_ARG(ldx >= in_dim && lddh >= hidden && (!dx || lddx >= in_dim), "gfn_gated_bwd: a row stride is below the row's width");
+  if (!dx && !dwg) return GFN_OK;
+  const int64_t need = gfn_gated_bwd_workspace(n_max, in_dim, hidden, dtype, bg != nullptr, dx != nullptr, dwg != nullptr);
+  GFN_CHECK_ARG(workspace_bytes >= need && (need == 0 || workspace), "gfn_gated_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  if (n_max == 0 && !dwg) return GFN_OK;
+  const BwdPlan p = plan_bwd(n_max, in_dim, hidden, dtype, bg != nullptr);
+  GatedBwd a{};
+  a.n_max = n_max; a.n_dev = n_dev;
+  a.x = x; a.wg = wg; a.wu = wu; a.bg = bg; a.bu = bu; a.dh = dh;
+  a.ldx = ldx; a.lddh = lddh; a.lddx = lddx;
+  a.k = in_dim; a.h = hidden; a.act = act;
+  a.dx = dx;
+  float* ws = static_cast<float*>(workspace);
+  if (dwg) {
+    a.part = ws;
+    ws += p.part_floats;
+  }
+  if (dx && p.dx_sum) a.dx_sum = ws;
+  hipStream_t st = gfn_stream(stream);
+  const int kp = p.ks * 4 * (dtype == GFN_F32 ? 4 : 8);
+  if (dtype == GFN_F32) return gated_bwd_typed<float>(a, p, kp, dwg, dwu, dbg, dbu, st);
+  if (dtype == GFN_BF16) return gated_bwd_typed<__bf16>(a, p, kp, dwg, dwu, dbg, dbu, st);
+  return gated_bwd_typed<_Float16>(a, p, kp, dwg, dwu, dbg, dbu, st);
+}
+
+}  // extern "C"

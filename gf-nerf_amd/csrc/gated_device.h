@@ -1,0 +1,198 @@
+// gated_device.h -- operand types and 16-byte pieces of the gated feed-forward kernels (gated.hip).
+//
+// Everything moves in 16-byte pieces of a row: E = 8 f16 / bf16 or 4 f32 elements.  A UNIT is 64 bytes of a row = four pieces,
+// one for each 16-lane quarter kg of a wave: lane (j = lane & 15, kg = lane >> 4) holds piece kg of its row's unit.  That is the
+// operand layout of v_mfma_f32_16x16x32_{f16,bf16} (one instruction a unit) and, with the contraction index taken as
+// k = 16 u + 4 kg + m, of four v_mfma_f32_16x16x4_f32: both operands use the same order, so the sum does not see it.
+// Accumulators: lane (j, kg), register r = row 4 kg + r, column j.
+#pragma once
+#include "gfn_common.h"
+
+namespace {
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+
+enum { GATED_SILU = 0, GATED_GELU = 1, GATED_RELU = 2, GATED_SIGMOID = 3 };
+
+template <typename T>
+struct Piece {
+  static constexpr int E = 16 / (int)sizeof(T);
+};
+
+__device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, f32x4 c, __bf16*) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, f32x4 c, _Float16*) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, f32x4 c, float*) {
+#pragma unroll
+  for (int m = 0; m < 4; m++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, a)[m], __builtin_bit_cast(f32x4, b)[m], c, 0, 0, 0);
+  return c;
+}
+
+__device__ __forceinline__ u32x4 load16(const void* p) {  // rows of odd width start at any element: no alignment is assumed
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// Piece c (elements c E .. c E + E - 1) of a row of `k` elements, zeros behind its end; nothing outside the row is read.  The piece
+// that the row's end cuts is read as the row's last 16 bytes and shifted down (`k` is the same for every lane: a scalar shift).
+template <typename T>
+__device__ __forceinline__ u32x4 row_piece(const T* row, int c, int k) {
+  constexpr int E = Piece<T>::E;
+  const int left = k - c * E;
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (left >= E) return load16(row + c * E);
+  if (left <= 0) return v;
+  if (k >= E) {
+    const u32x4 w = load16(row + k - E);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 3; i++)  // element i of the piece = element i + E - left of the row's last E
+        v[i] = i < left ? (left == 3 ? w[i + 1] : left == 2 ? w[(i + 2) & 3] : w[3]) : 0u;
+    } else {
+      typedef unsigned __int128 u128;
+      const u128 s = __builtin_bit_cast(u128, w) >> (16 * (E - left));
+      v = __builtin_bit_cast(u32x4, s);
+    }
+    return v;
+  }
+  T e[E];
+#pragma unroll
+  for (int i = 0; i < E; i++) e[i] = i < left ? row[c * E + i] : (T)0.f;
+  __builtin_memcpy(&v, e, 16);
+  return v;
+}
+
+// eight consecutive values of a row -> f32, zeros from `left` on
+template <typename T>
+__device__ __forceinline__ void load_row8(const T* p, int left, float (&v)[8]) {
+  if (left >= 8) {
+    T e[8];
+    __builtin_memcpy(e, p, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = (float)e[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = i < left ? (float)p[i] : 0.f;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* p, int left, const float (&v)[N]) {
+  using Row = __attribute__((ext_vector_type(N))) T;
+  Row e;
+#pragma unroll
+  for (int i = 0; i < N; i++) e[i] = (T)v[i];
+  if (left >= N) {
+#pragma unroll
+    for (int c = 0; c < (int)sizeof(Row) / 16; c++) {
+      using Rows = __attribute__((ext_vector_type(sizeof(Row) / 4))) uint32_t;
+      const Rows r = __builtin_bit_cast(Rows, e);
+      const u32x4 q = {r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]};
+      __builtin_memcpy(reinterpret_cast<char*>(p) + 16 * c, &q, 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (i < left) p[i] = e[i];
+  }
+}
+
+// 1 / (1 + exp(-z)) and the same of -z, each to the last bits of f32 (EXACT) or of the hardware's exp and reciprocal (2^-22: far
+// below the rounding of a 16-bit result).
+template <bool EXACT>
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (EXACT) return 1.f / (1.f + expf(-z));
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
+}
+
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2.  EXACT: erfcf, which keeps the relative accuracy of the tail of z -> -inf.  Else the rational
+// approximation of Abramowitz & Stegun 7.1.26 of erfc(|z| / sqrt 2) = poly(t) exp(-z^2 / 2), |error| <= 1.5e-7 before the exponential;
+// `gauss` = exp(-z^2 / 2) comes with it (the derivative needs it as well).
+template <bool EXACT>
+__device__ __forceinline__ float normal_cdf(float z, float& gauss) {
+  const float h = -0.72134752044448170368f * z * z;  // -z^2 / 2 / ln 2
+  if constexpr (EXACT) {
+    gauss = expf(-0.5f * z * z);
+    return 0.5f * erfcf(z * -0.70710678118654752440f);
+  }
+  gauss = __builtin_amdgcn_exp2f(h);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752440f, __builtin_fabsf(z), 1.f));
+  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  p = __builtin_fmaf(p, t, 1.421413741f);
+  p = __builtin_fmaf(p, t, -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.254829592f);
+  const float tail = 0.5f * p * t * gauss;
+  return z < 0.f ? tail : 1.f - tail;
+}
+
+// v[i] = act(g[i]) u[i] for eight values: the choice of act is the same for every lane, taken once.  A NaN stays one.
+template <bool EXACT, typename F, typename U>
+__device__ __forceinline__ void gated8(int act, F g, U u, float (&v)[8]) {
+  switch (act) {
+    case GATED_SILU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = g(i) * sigmoid<EXACT>(g(i)) * u(i);
+      break;
+    case GATED_GELU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float gauss;
+        v[i] = g(i) * normal_cdf<EXACT>(g(i), gauss) * u(i);
+      }
+      break;
+    case GATED_RELU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = (g(i) < 0.f ? 0.f : g(i)) * u(i);
+      break;
+    default:
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = sigmoid<EXACT>(g(i)) * u(i);
+  }
+}
+// dg[i] = d[i] u[i] act'(g[i]), du[i] = d[i] act(g[i])
+template <bool EXACT, typename F, typename U, typename T>
+__device__ __forceinline__ void gated8_grad(int act, F g, U u, const float (&d)[8], T (&dg)[8], T (&du)[8]) {
+  switch (act) {
+    case GATED_SILU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float s = sigmoid<EXACT>(g(i)), a = g(i) * s;
+        dg[i] = (T)(d[i] * u(i) * __builtin_fmaf(a, 1.f - s, s));
+        du[i] = (T)(d[i] * a);
+      }
+      break;
+    case GATED_GELU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float gauss;
+        const float cdf = normal_cdf<EXACT>(g(i), gauss);
+        dg[i] = (T)(d[i] * u(i) * __builtin_fmaf(g(i) * 0.39894228040143267794f, gauss, cdf));
+        du[i] = (T)(d[i] * (g(i) * cdf));
+      }
+      break;
+    case GATED_RELU:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        dg[i] = (T)(g(i) > 0.f ? d[i] * u(i) : 0.f);
+        du[i] = (T)(d[i] * (g(i) < 0.f ? 0.f : g(i)));
+      }
+      break;
+    default:
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float s = sigmoid<EXACT>(g(i));
+        dg[i] = (T)(d[i] * u(i) * (s * (1.f - s)));
+        du[i] = (T)(d[i] * s);
+      }
+  }
+}
+
+}  // namespace

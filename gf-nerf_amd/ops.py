@@ -1388,6 +1388,200 @@ def adam_step_table(p, g, m, v, step, lr=1e-2, beta1=0.9, beta2=0.999, eps=1e-15
                                            _ptr(hyper), _stream()), "gfn_adam_step_ex")
 
 
+# ------------------------------------------------------------------------------ sequence-head operators
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GFN_F32 / GFN_BF16 / GFN_F16
+GATED_ACT = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+SCAN_GATE = {"linear": 0, "sigmoid": 1, "decay": 2}
+SCAN_BLOCK = 16  # GFN_SCAN_BLOCK: rows a saved state covers
+
+
+def _place(tensors):
+    """Every tensor on the current device (the launch goes to the current stream of the current device)."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise _lib.GfnError(f"a tensor on {t.device} in a call on device {here}: make it current (torch.cuda.device) first")
+
+
+def _rows(t, name, dtype=None, width=None, n=None):
+    """A 2-D tensor whose rows are contiguous, any row stride that keeps them apart -> its row stride in elements."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise _lib.GfnError(f"{name}: expected a CUDA(HIP) tensor")
+    if t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype):
+        raise _lib.GfnError(f"{name}: expected dtype {'float32, bfloat16 or float16' if dtype is None else dtype}, got {t.dtype}")
+    if t.dim() != 2 or (width is not None and t.shape[1] != width) or (n is not None and t.shape[0] != n):
+        raise _lib.GfnError(f"{name}: expected shape [{'n' if n is None else n}, {'columns' if width is None else width}], got {tuple(t.shape)}")
+    if t.shape[0] > 1 and (t.stride(0) < t.shape[1]) or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise _lib.GfnError(f"{name}: rows must be contiguous and apart, got strides {t.stride()} for shape {tuple(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _flat(t, dtype, name, shape):
+    """A contiguous tensor (or None) of exactly this dtype and shape."""
+    _chk(t, dtype, name)
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise _lib.GfnError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _apart(out, *inputs):
+    """The output is not one of the inputs (rows are read by other workgroups while it is written)."""
+    for t in inputs:
+        if t is not None and out.numel() and t.data_ptr() == out.data_ptr():
+            raise _lib.GfnError("out is one of the inputs")
+
+
+def _gated_args(x, Wg, Wu, bg, bu, act, n_dev, what):
+    ldx = _rows(x, "x")
+    if act not in GATED_ACT:
+        raise _lib.GfnError(f"{what}: act {act!r} is none of {sorted(GATED_ACT)}")
+    if not isinstance(Wg, torch.Tensor) or Wg.dim() != 2 or Wg.shape[1] != x.shape[1]:
+        raise _lib.GfnError(f"{what}: Wg must be [hidden, {x.shape[1]}], got {tuple(getattr(Wg, 'shape', ()))}")
+    h, k = Wg.shape
+    _flat(Wg, x.dtype, "Wg", (h, k)); _flat(Wu, x.dtype, "Wu", (h, k)); _flat(bg, x.dtype, "bg", (h,)); _flat(bu, x.dtype, "bu", (h,))
+    if Wu is None or (bg is None) != (bu is None):
+        raise _lib.GfnError(f"{what}: Wg needs Wu, and bg needs bu")
+    _flat(n_dev, torch.int32, "n_dev", (1,))
+    _place((x, Wg, Wu, bg, bu, n_dev))
+    return x.shape[0], k, h, ldx
+
+
+def gated_fwd(x, Wg, Wu, bg=None, bu=None, act="silu", out=None, n_dev=None):
+    """h = act(x Wg^T + bg) * (x Wu^T + bu): both projections, the activation and the product in one launch.  x [n, in] (rows at any
+    stride), Wg / Wu [hidden, in], bg / bu [hidden] or both None; f32, bf16 or f16 throughout, sums in f32; act "silu", "gelu" (erf),
+    "relu" or "sigmoid"; in 1..128, hidden 1..1024.  n_dev i32 [1]: live rows (those behind are left alone)."""
+    n, k, h, ldx = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_fwd")
+    if out is None:
+        out = torch.empty((n, h), dtype=x.dtype, device=x.device)
+    ldo = _rows(out, "out", x.dtype, h, n)
+    _place((out,)); _apart(out, x, Wg, Wu, bg, bu)
+    rc = _lib.lib().gfn_gated_fwd(_ptr(x), ldx, _ptr(Wg), _ptr(Wu), _ptr(bg), _ptr(bu), n, _ptr(n_dev), k, h, DTYPES[x.dtype], GATED_ACT[act], _ptr(out), ldo,
+                                  _stream())
+    _lib.check(rc, "gfn_gated_fwd")
+    return out
+
+
+def gated_bwd(x, Wg, Wu, dh, bg=None, bu=None, act="silu", need_dx=True, need_dw=True, n_dev=None):
+    """Gradients of gated_fwd for dh -> (dx, dWg, dWu, dbg, dbu); None for what is not wanted or not there.  The projections are formed
+    again from x (the forward saves nothing); the weights' gradients are sums in a fixed order, rounded once to x's dtype."""
+    n, k, h, ldx = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_bwd")
+    lddh = _rows(dh, "dh", x.dtype, h, n)
+    _place((dh,))
+    new = lambda *shape: torch.empty(shape, dtype=x.dtype, device=x.device)  # noqa: E731
+    dx = new(n, k) if need_dx else None
+    dWg, dWu = (new(h, k), new(h, k)) if need_dw else (None, None)
+    dbg, dbu = (new(h), new(h)) if need_dw and bg is not None else (None, None)
+    lib = _lib.lib()
+    size = lib.gfn_gated_bwd_workspace(n, k, h, DTYPES[x.dtype], bg is not None, need_dx, need_dw)
+    _lib.check(min(size, 0), "gfn_gated_bwd_workspace")
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    rc = lib.gfn_gated_bwd(_ptr(x), ldx, _ptr(Wg), _ptr(Wu), _ptr(bg), _ptr(bu), _ptr(dh), lddh, n, _ptr(n_dev), k, h, DTYPES[x.dtype], GATED_ACT[act], _ptr(dx), k,
+                           _ptr(dWg), _ptr(dWu), _ptr(dbg), _ptr(dbu), _ptr(ws), size, _stream())
+    _lib.check(rc, "gfn_gated_bwd")
+    return dx, dWg, dWu, dbg, dbu
+
+
+def _scan_args(f, c, gate, what, n=None):
+    ldf, ldc = _rows(f, "f", None, None, n), _rows(c, "c", getattr(f, "dtype", None), None, f.shape[0])
+    if gate not in SCAN_GATE:
+        raise _lib.GfnError(f"{what}: gate {gate!r} is none of {sorted(SCAN_GATE)}")
+    if f.shape[1] == 0 or c.shape[1] % f.shape[1]:
+        raise _lib.GfnError(f"{what}: {f.shape[1]} gates for {c.shape[1]} channels")
+    return ldf, ldc
+
+
+def _scan_rays(pts_offsets, what):
+    _chk(pts_offsets, torch.int32, "pts_offsets")
+    if pts_offsets is None or pts_offsets.dim() != 1 or pts_offsets.numel() < 1:
+        raise _lib.GfnError(f"{what}: pts_offsets must be i32 [rays + 1]")
+    return pts_offsets.numel() - 1
+
+
+def ray_scan_fwd(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, out=None, save=False):
+    """The gated linear recurrence h_t = a_t h_{t-1} + b_t along each ray's packed samples (front to back; reverse: back to front).
+    f [n, gates], c [n, channels] (f32, bf16 or f16; rows at any stride; gate d // (channels // gates) is channel d's):
+      gate "linear": a = f, b = c;  "sigmoid": a = sigmoid(f), b = (1 - a) c;  "decay": a = exp(-f), b = (1 - a) c -- with f = sigma dt and
+      reverse, the first sample's h is the composite of `channels` feature channels.
+    h0 f32 [rays, channels] or None (0).  -> dict(h [n, channels], state f32 [rays, channels] (every ray's last state), saved (save=True:
+    what ray_scan_bwd needs)).  Rows behind the last ray's: 0 in an h allocated here, left alone in `out`."""
+    R = _scan_rays(pts_offsets, "ray_scan_fwd")
+    ldf, ldc = _scan_args(f, c, gate, "ray_scan_fwd")
+    (n, d), g, dev = c.shape, f.shape[1], c.device
+    _flat(h0, torch.float32, "h0", (R, d))
+    h = torch.empty((n, d), dtype=c.dtype, device=dev) if out is None else out
+    ldh = _rows(h, "out", c.dtype, d, n)
+    _place((pts_offsets, f, c, h0, h)); _apart(h, f, c, h0)
+    state = torch.empty((R, d), dtype=torch.float32, device=dev)
+    saved = torch.empty(((n + SCAN_BLOCK - 1) // SCAN_BLOCK, d), dtype=torch.float32, device=dev) if save else None
+    rc = _lib.lib().gfn_ray_scan_fwd(_ptr(pts_offsets), R, _ptr(f), ldf, _ptr(c), ldc, n, d, g, DTYPES[c.dtype], SCAN_GATE[gate], int(reverse), _ptr(h0), _ptr(h), ldh,
+                                     _ptr(state), _ptr(saved), out is None, _stream())
+    _lib.check(rc, "gfn_ray_scan_fwd")
+    return dict(h=h, state=state, saved=saved)
+
+
+def ray_scan_bwd(pts_offsets, f, c, dh, saved, gate="sigmoid", reverse=False, h0=None, d_state=None):
+    """Gradients of ray_scan_fwd (same f, c, h0, flags; `saved` from its save=True) for dh [n, channels] and d_state f32 [rays, channels] or
+    None (0) -> dict(df [n, gates], dc [n, channels], dh0 f32 [rays, channels]).  Rows behind the last ray's are 0."""
+    R = _scan_rays(pts_offsets, "ray_scan_bwd")
+    ldf, ldc = _scan_args(f, c, gate, "ray_scan_bwd")
+    (n, d), g, dev = c.shape, f.shape[1], c.device
+    lddh = _rows(dh, "dh", c.dtype, d, n)
+    _flat(h0, torch.float32, "h0", (R, d)); _flat(d_state, torch.float32, "d_state", (R, d))
+    if saved is None:
+        raise _lib.GfnError("ray_scan_bwd: saved is missing (ray_scan_fwd with save=True)")
+    _flat(saved, torch.float32, "saved", ((n + SCAN_BLOCK - 1) // SCAN_BLOCK, d))
+    _place((pts_offsets, f, c, dh, saved, h0, d_state))
+    df, dc = torch.empty((n, g), dtype=c.dtype, device=dev), torch.empty((n, d), dtype=c.dtype, device=dev)
+    dh0 = torch.empty((R, d), dtype=torch.float32, device=dev)
+    rc = _lib.lib().gfn_ray_scan_bwd(_ptr(pts_offsets), R, _ptr(f), ldf, _ptr(c), ldc, _ptr(dh), lddh, n, d, g, DTYPES[c.dtype], SCAN_GATE[gate], int(reverse), _ptr(h0),
+                                     _ptr(d_state), _ptr(saved), _ptr(df), g, _ptr(dc), d, _ptr(dh0), 1, _stream())
+    _lib.check(rc, "gfn_ray_scan_bwd")
+    return dict(df=df, dc=dc, dh0=dh0)
+
+
+def ray_scan_step(f, c, state, gate="sigmoid", out=None):
+    """One more sample of every ray: state [rays, channels] f32 <- a state + b, in place; -> h [rays, channels] in c's dtype.  f [rays, gates],
+    c [rays, channels] as in ray_scan_fwd."""
+    ldf, ldc = _scan_args(f, c, gate, "ray_scan_step")
+    n, d = c.shape
+    if state is None:
+        raise _lib.GfnError("ray_scan_step: state is missing")
+    _flat(state, torch.float32, "state", (n, d))
+    h = torch.empty((n, d), dtype=c.dtype, device=c.device) if out is None else out
+    ldh = _rows(h, "out", c.dtype, d, n)
+    _place((f, c, state, h)); _apart(h, f, state)
+    rc = _lib.lib().gfn_ray_scan_step(_ptr(f), ldf, _ptr(c), ldc, n, d, f.shape[1], DTYPES[c.dtype], SCAN_GATE[gate], _ptr(state), _ptr(h), ldh, _stream())
+    _lib.check(rc, "gfn_ray_scan_step")
+    return h
+
+
+def dropout_call(counter):
+    """The number of this forward pass for `dropout`, i64 [1]: counter's value (i64 [1] on the device), which moves on by one.  Taken on the
+    device, so a replayed hipGraph gets a new number each time."""
+    _flat(counter, torch.int64, "counter", (1,))
+    if counter is None:
+        raise _lib.GfnError("dropout_call: counter is missing")
+    _place((counter,))
+    call = torch.empty(1, dtype=torch.int64, device=counter.device)
+    _lib.check(_lib.lib().gfn_dropout_call(_ptr(counter), _ptr(call), _stream()), "gfn_dropout_call")
+    return call
+
+
+def dropout(x, p, seed, call, out=None):
+    """y = x where the element is kept, times 65536 / (65536 - t), t = round(65536 p); 0 where it is dropped.  Which elements are kept is a
+    function of (seed, call, row, column) -- Philox4x32-10, 16 bits an element -- and never stored: the gradient is the same call on dy.
+    x [n, columns] (f32, bf16 or f16, rows at any stride), call i64 [1] (dropout_call); out may be x."""
+    ldx = _rows(x, "x")
+    if call is None:
+        raise _lib.GfnError("dropout: call is missing")
+    _flat(call, torch.int64, "call", (1,))
+    y = torch.empty((x.shape[0], x.shape[1]), dtype=x.dtype, device=x.device) if out is None else out
+    ldy = _rows(y, "out", x.dtype, x.shape[1], x.shape[0])
+    _place((x, call, y))
+    rc = _lib.lib().gfn_dropout(_ptr(x), ldx, x.shape[0], x.shape[1], DTYPES[x.dtype], float(p), int(seed) & 0xFFFFFFFFFFFFFFFF, _ptr(call), _ptr(y), ldy, _stream())
+    _lib.check(rc, "gfn_dropout")
+    return y
+
+
 def copy_list(pairs):
     """[(dst, src)]: up to 8 small same-dtype, same-size contiguous device tensors copied in ONE launch (gfn_copy_list)."""
     import ctypes as C

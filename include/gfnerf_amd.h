@@ -59,8 +59,9 @@ typedef enum {
  *   gfn_field_bwd_x3, gfn_field_bwd_scatter_x3, gfn_fused_forward, gfn_fused_render, gfn_fused_render_rec); the two-phase inference
  *   march is gone too (gfn_sample_rays_continue and those arguments: a 6 % gain on a random-init scene, a 3x loss on a trained one);
  *   gfn_train_losses, gfn_loss_grad_combine added; gfn_fused_render(_rec) gained cam_uniform.
- *   108: round 6 -- gfn_launch_opts.reserved became colour_x2 (same size and offsets: a 107 caller's zeroed word is the default). */
-#define GFN_ABI_VERSION 108
+ *   108: round 6 -- gfn_launch_opts.reserved became colour_x2 (same size and offsets: a 107 caller's zeroed word is the default).
+ *   109: gfn_gated_*, gfn_ray_scan_*, gfn_dropout* added. */
+#define GFN_ABI_VERSION 109
 
 const char* gfn_last_error(void);
 int gfn_version(void);
@@ -746,6 +747,66 @@ int gfn_octree_construct_trans_host(const float* c2w_visible, const float* intri
                                     int64_t first_cam, const float* pts, int64_t n_pts, uint64_t seed, void* trans_out,
                                     int64_t* good_cams_out);
 int gfn_octree_fit_weight_host(const float* w2xz, const float* pts, int64_t n_pts, float* weight_out);
+
+/* ====================================================================== *
+ * Sequence-head operators: a gated feed-forward layer on every sample, dropout, and a
+ * gated linear recurrence along each ray's packed samples.  No reference
+ * counterpart: they stand beside gfn_linear_*, gfn_step_draws and gfn_composite_*.
+ * Element types of their tensors: */
+typedef enum { GFN_F32 = 0, GFN_BF16 = 1, GFN_F16 = 2 } gfn_dtype;
+
+/* h = act(x wg^T + bg) * (x wu^T + bu), act 0 silu (z sigmoid(z)), 1 gelu (z Phi(z), erf form), 2 relu, 3 sigmoid.
+ * x [n, in_dim] with row stride ldx, wg / wu [hidden, in_dim] (nn.Linear's layout, contiguous), bg / bu [hidden] or both NULL,
+ * out [n, hidden] with row stride ldo (strides in elements; no alignment beyond the element's); all of type dtype, sums in f32.
+ * in_dim 1..128, hidden 1..1024.  Rows behind *n_dev (NULL: n_max) are not read and not written. */
+int gfn_gated_fwd(const void* x, int64_t ldx, const void* wg, const void* wu, const void* bg, const void* bu,
+                  int64_t n_max, const int32_t* n_dev, int in_dim, int hidden, int dtype, int act, void* out,
+                  int64_t ldo, void* stream);
+/* Gradients of gfn_gated_fwd for dh = d loss / d out.  dx may be NULL (not wanted), and so may dwg and dwu together; dbg / dbu are
+ * given exactly when the biases and dwg are.  All gradients are WRITTEN (not added to) in type dtype, each rounded once from an f32
+ * sum taken in a fixed order: a call repeats its bits.  The intermediate gradients of the two projections are rounded to dtype (f16:
+ * under a power-of-two scale that follows |dh|).  workspace: gfn_gated_bwd_workspace bytes of device memory, 16-byte aligned, owned by
+ * the call until its work is done (two calls in flight need two). */
+int64_t gfn_gated_bwd_workspace(int64_t n_max, int in_dim, int hidden, int dtype, int bias, int need_dx, int need_dw);
+int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, const void* bg, const void* bu,
+                  const void* dh, int64_t lddh, int64_t n_max, const int32_t* n_dev, int in_dim, int hidden, int dtype,
+                  int act, void* dx, int64_t lddx, void* dwg, void* dwu, void* dbg, void* dbu, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
+/* The gated linear recurrence along each ray's packed samples: h_t = a_t h_{t-1} + b_t from h_{-1} = h0, front to back, or (reverse
+ * != 0) back to front.  f [n, gates] and c [n, channels] of type dtype (row strides ldf / ldc in elements); gates divides channels
+ * (at most 4096) and gate d / (channels / gates) belongs to channel d; a gate is shared by at most 64 channels (256 where rows are
+ * aligned to 4 elements), or every channel has its own.
+ *   gate 0 (linear)   a = f,            b = c
+ *   gate 1 (sigmoid)  a = sigmoid(f),   b = (1 - a) c
+ *   gate 2 (decay)    a = exp(-f),      b = (1 - a) c     (f = sigma dt: reverse, this composites `channels` feature channels)
+ * h0 f32 [n_rays, channels] (NULL: 0); h [n, channels] of type dtype: every row's state, rounded once; state f32 [n_rays, channels]
+ * (may be NULL): each ray's last state (an empty ray's is its h0).  saved f32 [(n_max + 15) / 16, channels] (may be NULL): what
+ * gfn_ray_scan_bwd needs from the forward.  pts_offsets i32 [n_rays + 1] ascending from 0; rows behind the last ray's are not read, and
+ * their rows of h are left as they are, or cleared (clear_tail != 0). */
+#define GFN_SCAN_BLOCK 16
+#define GFN_SCAN_MAX_CHANNELS 4096
+int gfn_ray_scan_fwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, int64_t ldf, const void* c, int64_t ldc,
+                     int64_t n_max, int channels, int gates, int dtype, int gate, int reverse, const float* h0, void* h,
+                     int64_t ldh, float* state, float* saved, int clear_tail, void* stream);
+/* Its gradients for dh = d loss / d h (type dtype) and d_state = d loss / d state (f32, NULL: 0): df, dc of type dtype, dh0 f32
+ * [n_rays, channels] (may be NULL), all written.  f, c, h0, pts_offsets and the flags as in the forward call that wrote `saved`. */
+int gfn_ray_scan_bwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, int64_t ldf, const void* c, int64_t ldc,
+                     const void* dh, int64_t lddh, int64_t n_max, int channels, int gates, int dtype, int gate, int reverse,
+                     const float* h0, const float* d_state, const float* saved, void* df, int64_t lddf, void* dc, int64_t lddc,
+                     float* dh0, int clear_tail, void* stream);
+/* One more sample of every ray: state[r] = a state[r] + b in place, h [n_rays, channels] = state rounded to dtype. */
+int gfn_ray_scan_step(const void* f, int64_t ldf, const void* c, int64_t ldc, int64_t n_rays, int channels, int gates,
+                      int dtype, int gate, float* state, void* h, int64_t ldh, void* stream);
+
+/* Dropout with a mask that is a function of (seed, *call, row, column) and is never stored: y = keep ? x * 65536 / (65536 - t) : 0,
+ * t = round(65536 p), keep = the element's 16 random bits >= t -- element (row, col) takes bits 16 (col % 2) .. of word (col % 8) / 2 of
+ * Philox4x32-10 with counter (col / 8, row, *call low, *call high) and key `seed`.  A dropped element is 0 whatever x holds (p = 1:
+ * all of them).  The gradient is the same call on dy.  x, y [rows, cols] of type dtype, row strides ldx / ldy; y may be x. */
+int gfn_dropout(const void* x, int64_t ldx, int64_t rows, int cols, int dtype, float p, uint64_t seed, const uint64_t* call,
+                void* y, int64_t ldy, void* stream);
+/* The number of this forward pass: *call = *counter, *counter += 1, on the device -- a replayed hipGraph draws a fresh mask each time. */
+int gfn_dropout_call(uint64_t* counter, uint64_t* call, void* stream);
 
 #ifdef __cplusplus
 }
