@@ -111,9 +111,10 @@ SIGNATURES = {
     "gfn_gated_fwd": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
     "gfn_gated_bwd_workspace": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
     "gfn_gated_bwd": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
-    "gfn_ray_scan_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp, _vp, _i32, _vp]),
+    "gfn_ray_scan_workspace": (_i64, [_i64, _i64, _i32, _i32]),
+    "gfn_ray_scan_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i64, _vp]),
     "gfn_ray_scan_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp,
-                                _i32, _vp]),
+                                _i32, _vp, _i64, _vp]),
     "gfn_ray_scan_step": (_i32, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
     "gfn_dropout": (_i32, [_vp, _i64, _i64, _i32, _i32, _f32, _u64, _vp, _vp, _i64, _vp]),
     "gfn_dropout_call": (_i32, [_vp, _vp, _vp]),

@@ -7,11 +7,15 @@
 //     decay    a = exp(-f)        b = (1 - a) c        (f = optical thickness: back to front this is alpha compositing of D channels)
 // Backward:  l_t = dh_t + a_{t+1} l_{t+1} (the last row's: + d_state);  dc = l (1 - a) (linear: l);  df = l (h_{t-1} - c) da/df (linear:
 // l h_{t-1}), summed over the channels of a gate;  dh0 = a_first l_first.  h_{t-1} is not read back: the forward leaves the f32 state it
-// had on entering every aligned block of 16 rows (1/8 of the bytes of a 16-bit h, and nothing is rounded), and the backward walks each
+// had on entering every aligned block of 8 rows (1/4 of the bytes of a 16-bit h, and nothing is rounded), and the backward walks each
 // block forward from there in registers before it walks it backward.
 //
-// A lane owns VEC channels of one ray and walks the ray's rows; the 16 rows of a block are requested together, so the recurrence's
-// chain of multiply-adds runs on data that has arrived.  State and adjoint are f32.
+// A lane owns VEC channels and walks rows: of one ray where there are rays enough to fill the chip, else of one RUN of rows (several to a
+// ray, or several rays to one).  Rows are taken in aligned blocks of 8, the next block requested before this one is worked on, so the
+// recurrence's chain of multiply-adds runs on data that has arrived.  A run's walk starts from a state that the rows in front of it
+// decide: a first reading (AGG) reduces every run to one step state -> A state + S, with A = 0 as soon as a ray begins in it,
+// run_prefix_kernel composes the steps in order, and the second reading writes the results.  Every sum has a fixed order: the same bits
+// every run.  State and adjoint are f32.
 #include "gfn_common.h"
 
 namespace {
@@ -32,10 +36,9 @@ __device__ __forceinline__ void gate_of(float f, float& a, float& rest) {
     a = f;
     rest = 1.f;
   } else if constexpr (GATE == GATE_SIGMOID) {
-    const float e = exp_of<EXACT>(-__builtin_fabsf(f));
-    const float r = EXACT ? 1.f / (1.f + e) : __builtin_amdgcn_rcpf(1.f + e);
-    a = f >= 0.f ? r : e * r;
-    rest = f >= 0.f ? e * r : r;
+    const float e = exp_of<EXACT>(-f);  // infinite from f < -88 on: a = 0, 1 - a = 1
+    a = EXACT ? 1.f / (1.f + e) : __builtin_amdgcn_rcpf(1.f + e);
+    rest = e > 1.f ? 1.f - a : e * a;
   } else {
     a = exp_of<EXACT>(-f);
     if constexpr (EXACT) {
@@ -66,171 +69,447 @@ struct ScanArgs {
   void *h, *df, *dc;
   float *state, *saved, *dh0;
   const float* saved_in;
-  int slot;      // lanes a (ray, gate) takes when gates are shared: a power of two >= the lanes it needs
   int per_gate;  // channels of a gate
+  int clear;     // rows of no ray: write zeros
+  // how lanes are dealt out: `lanes` to a walk, in slots of `slot` (a power of two) to a shared gate, `parts` slots of 64 where one is
+  // not enough (df's sums over each go to `partial` [parts][n_max][g] then)
+  int lanes, slot, parts;
+  float* partial;
+  int64_t run_rows, runs;  // 0: a walk is a ray; else rows of a run (a multiple of kBlock) and their number
+  float2* agg;             // [runs][d]: AGG writes (A, S); then .y is the state in front of the run
 };
 
-// this thread's ray and first channel; false: nothing to do (the lanes of a slot that no channel fills stay for the reductions)
+// a state that meets a ray's beginning (a = 0) stays out of it, infinite or not
+__device__ __forceinline__ float compose(float a, float b, float s) { return a == 0.f || s == 0.f ? b : __builtin_fmaf(a, s, b); }
+
+struct Place {
+  int64_t walk;  // the ray or run
+  int ch, gate, part;
+  bool active;   // a lane of a slot that no channel fills stays for the slot's reductions, reading channel 0 of its gate
+};
+
 template <int VEC, bool SHARED>
-__device__ __forceinline__ bool scan_place(const ScanArgs& a, int64_t& ray, int& ch, int& gate, bool& active) {
+__device__ __forceinline__ bool scan_place(const ScanArgs& a, Place& p) {
   const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  p.walk = id / a.lanes;
+  const int at = (int)(id - p.walk * a.lanes);
+  p.part = 0;
   if constexpr (SHARED) {
-    const int64_t s = id / a.slot;
-    ray = s / a.g;
-    gate = (int)(s - ray * a.g);
-    const int at = (int)(id & (a.slot - 1)) * VEC;
-    ch = gate * a.per_gate + at;
-    active = at < a.per_gate;
+    const int span = a.slot * a.parts, in = at % span;
+    p.gate = at / span;
+    p.part = in / a.slot;
+    p.active = in * VEC < a.per_gate;
+    p.ch = p.gate * a.per_gate + (p.active ? in * VEC : 0);
   } else {
-    const int lanes = a.d / VEC;
-    ray = id / lanes;
-    ch = (int)(id - ray * lanes) * VEC;
-    gate = ch;
-    active = true;
+    p.ch = p.gate = at * VEC;
+    p.active = true;
   }
-  return ray < a.rays;
+  return p.walk < (a.run_rows ? a.runs : a.rays);
 }
 
-__device__ __forceinline__ void ray_rows(const ScanArgs& a, int64_t ray, int64_t& start, int64_t& end) {  // inside the arrays, whatever the offsets say
-  start = a.offsets[ray];
-  end = a.offsets[ray + 1];
-  start = start < 0 ? 0 : (start > a.n_max ? a.n_max : start);
-  end = end < start ? start : (end > a.n_max ? a.n_max : end);
-}
+__device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-template <typename T, int GATE, int VEC, bool SHARED>
-__global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
-  constexpr bool EXACT = sizeof(T) == 4;
-  using V = Vec<T, VEC>;
-  int64_t ray, start, end;
-  int ch, gate;
-  bool active;
-  if (!scan_place<VEC, SHARED>(a, ray, ch, gate, active) || !active) return;
-  ray_rows(a, ray, start, end);
-  const T *f = static_cast<const T*>(a.f) + gate, *c = static_cast<const T*>(a.c) + ch;
-  T* h = static_cast<T*>(a.h) + ch;
-  float s[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; v++) s[v] = a.h0 ? a.h0[ray * a.d + ch + v] : 0.f;
-  const int64_t b0 = start / kBlock, blocks = end > start ? (end - 1) / kBlock - b0 + 1 : 0;
-  for (int64_t i = 0; i < blocks; i++) {
-    const int64_t base = (a.reverse ? b0 + blocks - 1 - i : b0 + i) * kBlock;
-    const int64_t lo = base > start ? base : start, hi = base + kBlock < end ? base + kBlock : end;
-    if (a.saved && i)
-#pragma unroll
-      for (int v = 0; v < VEC; v++) a.saved[base / kBlock * a.d + ch + v] = s[v];
-    V fr[kBlock], cr[kBlock];
-#pragma unroll
-    for (int r = 0; r < kBlock; r++) {
-      int64_t row = base + (a.reverse ? kBlock - 1 - r : r);
-      row = row < lo ? lo : (row >= hi ? hi - 1 : row);
-      if constexpr (SHARED) fr[r].v[0] = f[row * a.ldf];
-      else fr[r] = *reinterpret_cast<const V*>(f + row * a.ldf);
-      cr[r] = *reinterpret_cast<const V*>(c + row * a.ldc);
+// The pieces of a walk: one ray, or a run's share of each ray it meets, in the order `asc` says.  Offsets are kept inside the arrays,
+// whatever they hold.
+struct Pieces {
+  const ScanArgs& a;
+  bool asc;
+  int64_t lo, hi, ray;  // the run's rows (a ray: all); the ray of the next piece
+  __device__ Pieces(const ScanArgs& args, int64_t walk, bool up) : a(args), asc(up) {
+    if (!a.run_rows) {
+      lo = 0;
+      hi = a.n_max;
+      ray = walk;
+      return;
     }
-#pragma unroll
-    for (int r = 0; r < kBlock; r++) {
-      const int64_t row = base + (a.reverse ? kBlock - 1 - r : r);
-      if (row >= lo && row < hi) {
-        V out;
-        float ga, rest;
-#pragma unroll
-        for (int v = 0; v < VEC; v++) {
-          if (!SHARED || v == 0) gate_of<GATE, EXACT>((float)fr[r].v[v], ga, rest);
-          s[v] = __builtin_fmaf(ga, s[v], rest * (float)cr[r].v[v]);
-          out.v[v] = (T)s[v];
-        }
-        *reinterpret_cast<V*>(h + row * a.ldh) = out;
+    const int64_t r = asc ? walk : a.runs - 1 - walk;  // runs are numbered in the walk's order
+    lo = r * a.run_rows;
+    hi = lo + a.run_rows < a.n_max ? lo + a.run_rows : a.n_max;
+    int64_t x = 0, y = a.rays;  // up: the first ray that ends behind the first row; down: the last that begins in front of the last
+    while (x < y) {
+      const int64_t m = (x + y) >> 1;
+      if (asc ? a.offsets[m + 1] > lo : a.offsets[m] >= hi) y = m;
+      else x = m + 1;
+    }
+    ray = asc ? x : x - 1;
+  }
+  // rows [s, e) of the next piece and whether its ray begins / ends (in the walk's order) there; false: no more
+  __device__ bool next(int64_t& of, int64_t& s, int64_t& e, bool& begins, bool& ends) {
+    for (;;) {
+      if (ray < 0 || ray >= a.rays) return false;
+      const int64_t rs = clamp_row(a.offsets[ray], 0, a.n_max), re = clamp_row(a.offsets[ray + 1], rs, a.n_max);
+      if (a.run_rows && (asc ? rs >= hi : re <= lo)) {
+        if (rs < re || (asc ? rs > hi : re < lo)) return false;  // an empty ray on the border says nothing about the next one
       }
+      of = ray;
+      s = rs > lo ? rs : lo;
+      e = re < hi ? re : hi;
+      begins = asc ? s == rs : e == re;
+      ends = asc ? e == re : s == rs;
+      if (!a.run_rows) {
+        ray = a.rays;
+        return true;
+      }
+      ray += asc ? 1 : -1;
+      if (s < e) return true;
     }
   }
-  if (a.state)
-#pragma unroll
-    for (int v = 0; v < VEC; v++) a.state[ray * a.d + ch + v] = s[v];
+};
+
+// rows of no ray (behind the last ray's): -> 0
+template <typename T>
+__device__ __forceinline__ void clear_rows(const ScanArgs& a, T* p, int64_t ld, int width) {
+  const int64_t begin = clamp_row(a.offsets[a.rays], 0, a.n_max);
+  for (int64_t e = begin * width + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < a.n_max * width; e += (int64_t)gridDim.x * blockDim.x)
+    p[e / width * ld + e % width] = (T)0.f;
 }
 
-template <typename T, int GATE, int VEC, bool SHARED>
-__global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs a) {
-  constexpr bool EXACT = sizeof(T) == 4;
-  using V = Vec<T, VEC>;
-  int64_t ray, start = 0, end = 0;
-  int ch, gate;
-  bool active;
-  const bool here = scan_place<VEC, SHARED>(a, ray, ch, gate, active);
-  if (!SHARED && !here) return;
-  if (here) ray_rows(a, ray, start, end);
-  active = active && here;
-  if (!here) gate = ch = 0;
-  const int cl = active ? ch : 0;  // a lane without a channel reads channel 0 and counts for nothing
-  const T *f = static_cast<const T*>(a.f) + gate, *c = static_cast<const T*>(a.c) + cl, *dh = static_cast<const T*>(a.dh) + cl;
-  T *df = static_cast<T*>(a.df) + gate, *dc = static_cast<T*>(a.dc) + ch;
-  float l[VEC], first[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; v++) {
-    l[v] = active && a.d_state ? a.d_state[ray * a.d + ch + v] : 0.f;
-    first[v] = active && a.h0 ? a.h0[ray * a.d + ch + v] : 0.f;
+template <int BYTES>
+struct BitsOf { using type = uint32_t; };
+template <>
+struct BitsOf<2> { using type = uint16_t; };
+
+// One block of a piece: its rows in the walk's order are row0, row0 + dir, ...; those in [s, e) count.
+template <typename T, int VEC, bool SHARED, bool BWD, bool AGG>
+struct Rows {
+  using F = typename BitsOf<sizeof(T) * (SHARED ? 1 : VEC)>::type;
+  using C = typename BitsOf<sizeof(T) * VEC>::type;
+  F f[kBlock];
+  C c[kBlock], dh[BWD ? kBlock : 1];
+  T fd;  // shared gates dealt out over 8 lanes or more: this lane's row's
+  __device__ __forceinline__ float gate(int r, int v) const {
+    if constexpr (SHARED) return (float)__builtin_bit_cast(T, f[r]);
+    else return (float)__builtin_bit_cast(Vec<T, VEC>, f[r]).v[v];
   }
-  const int64_t b0 = start / kBlock, blocks = end > start ? (end - 1) / kBlock - b0 + 1 : 0;
-  for (int64_t i = blocks - 1; i >= 0; i--) {  // the recurrence's last block first
-    const int64_t base = (a.reverse ? b0 + blocks - 1 - i : b0 + i) * kBlock;
-    const int64_t lo = base > start ? base : start, hi = base + kBlock < end ? base + kBlock : end;
-    V fr[kBlock], cr[kBlock], dr[kBlock];
+  __device__ __forceinline__ float in(int r, int v) const { return (float)__builtin_bit_cast(Vec<T, VEC>, c[r]).v[v]; }
+  __device__ __forceinline__ float grad(int r, int v) const { return (float)__builtin_bit_cast(Vec<T, VEC>, dh[BWD ? r : 0]).v[v]; }
+  template <typename R>
+  static __device__ __forceinline__ void column(R (&to)[kBlock], const T* from, int64_t ld, int64_t row0, bool asc, bool whole, int64_t s, int64_t e) {
+    if (whole) {
+      const T* q = from + row0 * ld;
+      const int64_t step = asc ? ld : -ld;
 #pragma unroll
-    for (int r = 0; r < kBlock; r++) {
-      int64_t row = base + (a.reverse ? kBlock - 1 - r : r);
-      row = row < lo ? lo : (row >= hi ? hi - 1 : row);
-      if constexpr (SHARED) fr[r].v[0] = f[row * a.ldf];
-      else fr[r] = *reinterpret_cast<const V*>(f + row * a.ldf);
-      cr[r] = *reinterpret_cast<const V*>(c + row * a.ldc);
-      dr[r] = *reinterpret_cast<const V*>(dh + row * a.lddh);
+      for (int r = 0; r < kBlock; r++) to[r] = *reinterpret_cast<const R*>(q + r * step);
+    } else {  // another kind of load, or the compiler joins the two ways' loads and keeps sixteen addresses for them
+#pragma unroll
+      for (int r = 0; r < kBlock; r++) to[r] = __builtin_nontemporal_load(reinterpret_cast<const R*>(from + clamp_row(asc ? row0 + r : row0 - r, s, e - 1) * ld));
     }
-    float before[kBlock][VEC], s[VEC];  // the state in front of each row
+  }
+  __device__ __forceinline__ void load(const ScanArgs& a, const T* pf, const T* pc, const T* pd, int64_t base, bool asc, int64_t s, int64_t e, int deal) {
+    const int64_t row0 = base + (asc ? 0 : kBlock - 1);
+    const bool whole = __all(base >= s && base + kBlock <= e);
+    if (SHARED && deal >= 0) fd = pf[clamp_row(asc ? row0 + deal : row0 - deal, s, e - 1) * a.ldf];
+    else column(f, pf, a.ldf, row0, asc, whole, s, e);
+    if constexpr (!(BWD && AGG)) column(c, pc, a.ldc, row0, asc, whole, s, e);
+    if constexpr (BWD) column(dh, pd, a.lddh, row0, asc, whole, s, e);
+  }
+};
+
+constexpr int kScanThreads = 256;
+
+// The gates of a block: each lane its own, or -- shared by 8 lanes or more -- one evaluation a lane, dealt through LDS.
+template <typename T, int GATE, int VEC, bool SHARED>
+struct Gates {
+  float2* pool;  // kBlock entries of the slot's, or null
+  int deal;
+  __device__ __forceinline__ void begin(const T& fd) {
+    if (SHARED && pool) {
+      float x, y;
+      gate_of<GATE, sizeof(T) == 4>((float)fd, x, y);
+      __builtin_amdgcn_wave_barrier();
+      pool[deal] = make_float2(x, y);  // lanes with the same row write the same value
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  template <typename R>
+  __device__ __forceinline__ void get(int r, const R& rows, float (&x)[VEC], float (&y)[VEC]) const {
+    if (SHARED && pool) {
+      const float2 q = pool[r];
 #pragma unroll
-    for (int v = 0; v < VEC; v++) s[v] = i ? a.saved_in[base / kBlock * a.d + cl + v] : first[v];
-#pragma unroll
-    for (int r = 0; r < kBlock; r++) {
-      const int64_t row = base + (a.reverse ? kBlock - 1 - r : r);
-      float ga, rest;
+      for (int v = 0; v < VEC; v++) { x[v] = q.x; y[v] = q.y; }
+    } else {
 #pragma unroll
       for (int v = 0; v < VEC; v++) {
-        before[r][v] = s[v];
-        if (!SHARED || v == 0) gate_of<GATE, EXACT>((float)fr[r].v[v], ga, rest);
-        if (row >= lo && row < hi) s[v] = __builtin_fmaf(ga, s[v], rest * (float)cr[r].v[v]);
-      }
-    }
-#pragma unroll
-    for (int r = kBlock - 1; r >= 0; r--) {
-      const int64_t row = base + (a.reverse ? kBlock - 1 - r : r);
-      if (row >= lo && row < hi) {
-        V oc, of;
-        float ga, rest, sum = 0.f;
-#pragma unroll
-        for (int v = 0; v < VEC; v++) {
-          if (!SHARED || v == 0) gate_of<GATE, EXACT>((float)fr[r].v[v], ga, rest);
-          const float lt = l[v] + (float)dr[r].v[v], cv = (float)cr[r].v[v];
-          float d;
-          if constexpr (GATE == GATE_LINEAR) d = lt * before[r][v];
-          else if constexpr (GATE == GATE_SIGMOID) d = lt * (before[r][v] - cv) * (ga * rest);
-          else d = lt * (cv - before[r][v]) * ga;
-          oc.v[v] = (T)(lt * rest);
-          if constexpr (SHARED) sum += d;
-          else of.v[v] = (T)d;
-          l[v] = ga * lt;
-        }
-        if (active) *reinterpret_cast<V*>(dc + row * a.lddc) = oc;
-        if constexpr (SHARED) {
-          if (!active) sum = 0.f;
-          for (int o = a.slot >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-          if ((threadIdx.x & (a.slot - 1)) == 0) df[row * a.lddf] = (T)sum;
-        } else {
-          *reinterpret_cast<V*>(df + row * a.lddf) = of;
-        }
+        if (!SHARED || v == 0) gate_of<GATE, sizeof(T) == 4>(rows.gate(r, v), x[v], y[v]);
+        else { x[v] = x[0]; y[v] = y[0]; }
       }
     }
   }
-  if (a.dh0 && active)
+};
+
+template <typename T, int GATE, int VEC, bool SHARED, bool AGG>
+__global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
+  using V = Vec<T, VEC>;
+  __shared__ float2 pool[SHARED ? kScanThreads : 1];
+  if (!AGG && a.clear) clear_rows(a, static_cast<T*>(a.h), a.ldh, a.d);
+  Place at;
+  if (!scan_place<VEC, SHARED>(a, at)) return;
+  const bool asc = !a.reverse, dealt = SHARED && a.slot >= kBlock;
+  const int deal = dealt ? threadIdx.x & (kBlock - 1) : -1;
+  Gates<T, GATE, VEC, SHARED> gates{dealt ? pool + (threadIdx.x & ~(a.slot - 1)) : nullptr, deal};
+  const T *f = static_cast<const T*>(a.f) + at.gate, *c = static_cast<const T*>(a.c) + at.ch;
+  T* h = static_cast<T*>(a.h) + at.ch;
+  float s[VEC], A[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; v++) a.dh0[ray * a.d + ch + v] = l[v];
+  for (int v = 0; v < VEC; v++) {
+    s[v] = !AGG && a.run_rows ? a.agg[at.walk * a.d + at.ch + v].y : 0.f;
+    A[v] = 1.f;
+  }
+  Pieces pieces(a, at.walk, asc);
+  int64_t ray, lo, hi;
+  bool begins, ends;
+  while (pieces.next(ray, lo, hi, begins, ends)) {
+    if (begins)
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        s[v] = a.h0 ? a.h0[ray * a.d + at.ch + v] : 0.f;
+        A[v] = 0.f;
+      }
+    const int64_t b0 = lo / kBlock, blocks = hi > lo ? (hi - 1) / kBlock - b0 + 1 : 0;
+    Rows<T, VEC, SHARED, false, AGG> now, next;
+    auto base_of = [&](int64_t i) { return (asc ? b0 + i : b0 + blocks - 1 - i) * kBlock; };
+    if (blocks) now.load(a, f, c, nullptr, base_of(0), asc, lo, hi, deal);
+    for (int64_t i = 0; i < blocks; i++) {
+      const int64_t base = base_of(i), row0 = base + (asc ? 0 : kBlock - 1);
+      if (i + 1 < blocks) next.load(a, f, c, nullptr, base_of(i + 1), asc, lo, hi, deal);
+      if (!AGG && a.saved && at.active && row0 >= lo && row0 < hi)
+#pragma unroll
+        for (int v = 0; v < VEC; v++) a.saved[base / kBlock * a.d + at.ch + v] = s[v];
+      gates.begin(now.fd);
+      const bool whole = __all(base >= lo && base + kBlock <= hi && at.active);
+      T* out = h + row0 * a.ldh;
+      const int64_t step = asc ? a.ldh : -a.ldh;
+#pragma unroll
+      for (int r = 0; r < kBlock; r++) {
+        float x[VEC], y[VEC];
+        gates.get(r, now, x, y);
+        V o;
+        const int64_t row = asc ? row0 + r : row0 - r;
+        const bool in = whole || (row >= lo && row < hi);
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+          const float n = __builtin_fmaf(x[v], s[v], y[v] * now.in(r, v));
+          s[v] = in ? n : s[v];
+          if (AGG) A[v] = in ? A[v] * x[v] : A[v];
+          o.v[v] = (T)s[v];
+        }
+        if (!AGG) {
+          if (whole) *reinterpret_cast<V*>(out + r * step) = o;
+          else if (in && at.active) *reinterpret_cast<V*>(out + r * step) = o;
+        }
+      }
+      if (i + 1 < blocks) now = next;
+    }
+    if (!AGG && ends && a.state && at.active)
+#pragma unroll
+      for (int v = 0; v < VEC; v++) a.state[ray * a.d + at.ch + v] = s[v];
+  }
+  if (AGG && at.active)
+#pragma unroll
+    for (int v = 0; v < VEC; v++) a.agg[at.walk * a.d + at.ch + v] = make_float2(A[v], s[v]);
+}
+
+template <typename T, int GATE, int VEC, bool SHARED, bool AGG>
+__global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
+  using V = Vec<T, VEC>;
+  __shared__ float2 pool[SHARED ? kScanThreads : 1];
+  if (!AGG && a.clear) {
+    clear_rows(a, static_cast<T*>(a.df), a.lddf, a.g);
+    clear_rows(a, static_cast<T*>(a.dc), a.lddc, a.d);
+  }
+  Place at;
+  if (!scan_place<VEC, SHARED>(a, at)) return;
+  const bool asc = a.reverse != 0, dealt = SHARED && a.slot >= kBlock;  // against the recurrence
+  const int deal = dealt ? threadIdx.x & (kBlock - 1) : -1;
+  Gates<T, GATE, VEC, SHARED> gates{dealt ? pool + (threadIdx.x & ~(a.slot - 1)) : nullptr, deal};
+  const T *f = static_cast<const T*>(a.f) + at.gate, *c = static_cast<const T*>(a.c) + at.ch, *dh = static_cast<const T*>(a.dh) + at.ch;
+  T *df = static_cast<T*>(a.df) + at.gate, *dc = static_cast<T*>(a.dc) + at.ch;
+  float l[VEC], A[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; v++) {
+    l[v] = !AGG && a.run_rows ? a.agg[at.walk * a.d + at.ch + v].y : 0.f;
+    A[v] = 1.f;
+  }
+  Pieces pieces(a, at.walk, asc);
+  int64_t ray, lo, hi;
+  bool begins, ends;
+  while (pieces.next(ray, lo, hi, begins, ends)) {
+    if (begins)
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        l[v] = a.d_state ? a.d_state[ray * a.d + at.ch + v] : 0.f;
+        A[v] = 0.f;
+      }
+    const int64_t b0 = lo / kBlock, blocks = hi > lo ? (hi - 1) / kBlock - b0 + 1 : 0;
+    Rows<T, VEC, SHARED, true, AGG> now, next;
+    auto base_of = [&](int64_t i) { return (asc ? b0 + i : b0 + blocks - 1 - i) * kBlock; };
+    if (blocks) now.load(a, f, c, dh, base_of(0), asc, lo, hi, deal);
+    for (int64_t i = 0; i < blocks; i++) {
+      const int64_t base = base_of(i), row0 = base + (asc ? 0 : kBlock - 1);
+      const bool ray_starts = ends && i == blocks - 1;  // the recurrence's first row of the ray is in this block
+      float before[AGG ? 1 : kBlock][VEC], st[VEC];
+      if (!AGG) {
+        const int64_t first = asc ? hi - 1 : lo;  // the recurrence's first row of the piece, in its last block
+        const float* from = ray_starts ? a.h0 : a.saved_in;
+        const int64_t of = ray_starts ? ray : (asc ? (base + kBlock - 1 < first ? base + kBlock - 1 : first) : (base > first ? base : first)) / kBlock;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) st[v] = from ? from[of * a.d + at.ch + v] : 0.f;
+      }
+      if (i + 1 < blocks) next.load(a, f, c, dh, base_of(i + 1), asc, lo, hi, deal);
+      gates.begin(now.fd);
+      const bool whole = __all(base >= lo && base + kBlock <= hi && at.active);
+      float x[kBlock][VEC], y[kBlock][VEC];
+#pragma unroll
+      for (int r = kBlock - 1; r >= 0; r--) {  // the recurrence's order
+        gates.get(r, now, x[r], y[r]);
+        if (!AGG) {
+          const int64_t row = asc ? row0 + r : row0 - r;
+          const bool in = whole || (row >= lo && row < hi);
+#pragma unroll
+          for (int v = 0; v < VEC; v++) {
+            before[r][v] = st[v];
+            const float n = __builtin_fmaf(x[r][v], st[v], y[r][v] * now.in(r, v));
+            st[v] = in ? n : st[v];
+          }
+        }
+      }
+      float sums[SHARED && !AGG ? kBlock : 1];
+      T *out_c = dc + row0 * a.lddc, *out_f = df + row0 * a.lddf;
+      const int64_t step_c = asc ? a.lddc : -a.lddc, step_f = asc ? a.lddf : -a.lddf;
+#pragma unroll
+      for (int r = 0; r < kBlock; r++) {
+        const int64_t row = asc ? row0 + r : row0 - r;
+        const bool in = whole || (row >= lo && row < hi);
+        V oc, of;
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+          const float lt = l[v] + now.grad(r, v), xv = x[r][v], yv = y[r][v];
+          if (!AGG) {
+            const float cv = now.in(r, v);
+            float d;
+            if constexpr (GATE == GATE_LINEAR) d = lt * before[r][v];
+            else if constexpr (GATE == GATE_SIGMOID) d = lt * (before[r][v] - cv) * (xv * yv);
+            else d = lt * (cv - before[r][v]) * xv;
+            oc.v[v] = (T)(lt * yv);
+            if constexpr (SHARED) sum += d;
+            else of.v[v] = (T)d;
+          }
+          l[v] = in ? xv * lt : l[v];
+          if (AGG) A[v] = in ? A[v] * xv : A[v];
+        }
+        if (!AGG) {
+          if (whole) {
+            *reinterpret_cast<V*>(out_c + r * step_c) = oc;
+            if constexpr (!SHARED) *reinterpret_cast<V*>(out_f + r * step_f) = of;
+          } else if (in && at.active) {
+            *reinterpret_cast<V*>(out_c + r * step_c) = oc;
+            if constexpr (!SHARED) *reinterpret_cast<V*>(out_f + r * step_f) = of;
+          }
+          if constexpr (SHARED) sums[r] = at.active ? sum : 0.f;
+        }
+      }
+      if constexpr (SHARED && !AGG) {  // a gate's lanes add their channels: halve the rows a lane holds while lanes are left, then add plainly
+        int held = kBlock, first = 0;
+#pragma unroll
+        for (int o = 1; o < kBlock; o <<= 1) {
+          if (o < a.slot) {
+            held >>= 1;
+            const bool up = threadIdx.x & o;
+#pragma unroll
+            for (int k = 0; k < kBlock / 2; k++)
+              if (k < held) {
+                const float send = up ? sums[k] : sums[k + held], keep = up ? sums[k + held] : sums[k];
+                sums[k] = keep + __shfl_xor(send, o, 64);
+              }
+            first += up ? held : 0;
+          }
+        }
+        for (int o = kBlock; o < a.slot; o <<= 1) sums[0] += __shfl_xor(sums[0], o, 64);
+        const bool writer = (int)(threadIdx.x & (a.slot - 1)) < kBlock;
+#pragma unroll
+        for (int k = 0; k < kBlock; k++)
+          if (k < held && writer) {
+            const int64_t row = asc ? row0 + first + k : row0 - first - k;
+            if (row >= lo && row < hi) {
+              if (a.parts > 1) a.partial[((int64_t)at.part * a.n_max + row) * a.g + at.gate] = sums[k];
+              else df[row * a.lddf] = (T)sums[k];
+            }
+          }
+      }
+      if (i + 1 < blocks) now = next;
+    }
+    if (!AGG && ends && a.dh0 && at.active)
+#pragma unroll
+      for (int v = 0; v < VEC; v++) a.dh0[ray * a.d + at.ch + v] = l[v];
+  }
+  if (AGG && at.active)
+#pragma unroll
+    for (int v = 0; v < VEC; v++) a.agg[at.walk * a.d + at.ch + v] = make_float2(A[v], l[v]);
+}
+
+// AGG's steps -> the state in front of every run (in the walk's order).  A workgroup: 4 channels, 256 stretches of runs, each composed in registers
+// (up to kHeld runs of a stretch; more are read twice), joined in order through LDS.
+constexpr int kHeld = 16;
+__global__ __launch_bounds__(1024) void run_prefix_kernel(float2* __restrict__ agg, int64_t runs, int d) {
+  __shared__ float2 part[256][4];
+  const int lane = threadIdx.x & 3, stretch = threadIdx.x >> 2, ch = blockIdx.x * 4 + lane;
+  const int64_t per = (runs + 255) / 256, lo = stretch * per, hi = lo + per < runs ? lo + per : runs;
+  float2 held[kHeld];
+  float a = 1.f, s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) held[i] = ch < d && lo + i < hi ? agg[(lo + i) * d + ch] : make_float2(1.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kHeld; i++)
+    if (lo + i < hi) {
+      s = compose(held[i].x, held[i].y, s);
+      a *= held[i].x;
+    }
+  if (ch < d)
+    for (int64_t i = lo + kHeld; i < hi; i++) {
+      const float2 q = agg[i * d + ch];
+      s = compose(q.x, q.y, s);
+      a *= q.x;
+    }
+  part[stretch][lane] = make_float2(a, s);
+  __syncthreads();
+  if (ch >= d || lo >= hi) return;
+  s = 0.f;
+#pragma unroll 8
+  for (int r = 0; r < stretch; r++) s = compose(part[r][lane].x, part[r][lane].y, s);
+#pragma unroll
+  for (int i = 0; i < kHeld; i++)
+    if (lo + i < hi) {
+      agg[(lo + i) * d + ch].y = s;
+      s = compose(held[i].x, held[i].y, s);
+    }
+  for (int64_t i = lo + kHeld; i < hi; i++) {
+    const float2 q = agg[i * d + ch];
+    agg[i * d + ch].y = s;
+    s = compose(q.x, q.y, s);
+  }
+}
+
+// df of gates whose channels take several slots: the slots' sums in order
+template <typename T>
+__global__ __launch_bounds__(256) void scan_gate_sums_kernel(ScanArgs a, const float* __restrict__ partial, int parts) {
+  const int64_t n = a.n_max * a.g, live_lo = (int64_t)a.offsets[0] * a.g, live_hi = (int64_t)a.offsets[a.rays] * a.g;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
+    const bool live = e >= live_lo && e < live_hi;
+    if (!live && !a.clear) continue;
+    float s = 0.f;
+    if (live)
+      for (int i = 0; i < parts; i++) s += partial[i * n + e];
+    static_cast<T*>(a.df)[e / a.g * a.lddf + e % a.g] = (T)s;
+  }
+}
+
+// rays without samples: their state is what it starts from
+__global__ __launch_bounds__(256) void empty_rays_kernel(const int32_t* __restrict__ offsets, int64_t rays, int d, const float* __restrict__ from, float* __restrict__ to) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t ray = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); ray < rays; ray += (int64_t)gridDim.x * 4)
+    if (offsets[ray + 1] <= offsets[ray])
+      for (int i = lane; i < d; i += 64) to[ray * d + i] = from ? from[ray * d + i] : 0.f;
 }
 
 // one more row of every ray: state[r] = a state[r] + b
@@ -248,96 +527,136 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
   }
 }
 
-// rows behind the last ray's last -> 0
-template <typename T>
-__global__ __launch_bounds__(256) void zero_tail_kernel(const int32_t* __restrict__ offsets, int64_t rays, int64_t n_max, T* __restrict__ p, int64_t ld, int width) {
-  int64_t begin = offsets[rays];
-  begin = begin < 0 ? 0 : begin;
-  for (int64_t e = begin * width + (int64_t)blockIdx.x * 256 + threadIdx.x; e < n_max * width; e += (int64_t)gridDim.x * 256) p[e / width * ld + e % width] = (T)0.f;
-}
-
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
 int check_scan(const char* who, int64_t rays, int64_t n_max, int d, int g, int dtype, int gate, int64_t ldf, int64_t ldc) {
   GFN_CHECK_ARG(rays >= 0 && rays < (1ll << 31) && n_max >= 0 && n_max < (1ll << 31), "%s: %lld rays, n_max %lld", who, (long long)rays, (long long)n_max);
   GFN_CHECK_ARG(d >= 1 && d <= GFN_SCAN_MAX_CHANNELS && g >= 1 && g <= d && d % g == 0, "%s: %d gates for %d channels (1..%d channels, the gates dividing them)", who, g, d,
                 GFN_SCAN_MAX_CHANNELS);
-  GFN_CHECK_ARG(d / g <= 256 || g == d, "%s: %d channels share a gate (at most 256)", who, d / g);
   GFN_CHECK_ARG(dtype >= GFN_F32 && dtype <= GFN_F16, "%s: dtype %d", who, dtype);
   GFN_CHECK_ARG(gate >= 0 && gate <= 2, "%s: gate %d", who, gate);
   GFN_CHECK_ARG(ldf >= g && ldc >= d, "%s: a row stride is below the row's width", who);
   return GFN_OK;
 }
 
-// channels a lane: as wide as every pointer, stride and gate group allows
-int pick_vec(const ScanArgs& a, int size, bool shared, bool bwd) {
-  const int per = shared ? a.per_gate : a.d;
-  for (int vec = shared && per > 128 ? 4 : 2; vec > 1; vec >>= 1) {
-    const int64_t strides = a.ldc | (bwd ? a.lddh | a.lddc : a.ldh) | (shared ? 0 : a.ldf | (bwd ? a.lddf : 0));
-    uintptr_t at = reinterpret_cast<uintptr_t>(a.c) | (bwd ? reinterpret_cast<uintptr_t>(a.dh) | reinterpret_cast<uintptr_t>(a.dc) : reinterpret_cast<uintptr_t>(a.h));
-    if (!shared) at |= reinterpret_cast<uintptr_t>(a.f) | (bwd ? reinterpret_cast<uintptr_t>(a.df) : 0);
-    if (per % vec == 0 && strides % vec == 0 && at % ((uintptr_t)vec * size) == 0) return vec;
+// whether every pointer, stride and gate group leaves pairs of 16-bit channels aligned
+bool two_channels(const ScanArgs& a, bool shared, bool bwd) {
+  const int64_t strides = a.ldc | (bwd ? a.lddh | a.lddc : a.ldh) | (shared ? 0 : a.ldf | (bwd ? a.lddf : 0)) | (shared ? a.per_gate : a.d);
+  uintptr_t at = reinterpret_cast<uintptr_t>(a.c) | (bwd ? reinterpret_cast<uintptr_t>(a.dh) | reinterpret_cast<uintptr_t>(a.dc) : reinterpret_cast<uintptr_t>(a.h));
+  if (!shared) at |= reinterpret_cast<uintptr_t>(a.f) | (bwd ? reinterpret_cast<uintptr_t>(a.df) : 0);
+  return strides % 2 == 0 && at % 4 == 0;
+}
+
+// Rays or runs: a lane a ray as long as that fills the chip with walks that are not too long to wait for.
+bool use_runs(int64_t rays, int64_t n_max, int d) {
+  const int64_t mean = rays > 0 ? n_max / rays : 0;
+  return n_max > 0 && mean > 64 && rays * d < 64 * 1024;
+}
+
+struct ScanPlan {
+  int slot, parts, lanes;
+  int64_t run_rows, runs;
+};
+ScanPlan plan_scan(int64_t rays, int64_t n_max, int d, int g, int vec) {
+  ScanPlan p{1, 1, d / vec, 0, 0};
+  if (g != d) {
+    const int need = (d / g + vec - 1) / vec;
+    while (p.slot < need && p.slot < 64) p.slot <<= 1;
+    p.parts = (need + 63) / 64;
+    p.lanes = g * p.slot * p.parts;
   }
-  return 1;
+  if (use_runs(rays, n_max, d)) {
+    p.run_rows = n_max * p.lanes / (128 * 1024);  // two waves a SIMD
+    p.run_rows = (p.run_rows + kBlock - 1) / kBlock * kBlock;
+    if (p.run_rows < 4 * kBlock) p.run_rows = 4 * kBlock;
+    p.runs = (n_max + p.run_rows - 1) / p.run_rows;
+  }
+  return p;
+}
+// workspace: the runs' steps, df's sums over parts of gates
+int64_t scan_workspace(int64_t rays, int64_t n_max, int d, int g) {
+  int64_t runs = 0, parts = 0;
+  for (int vec = 1; vec <= 2; vec++)
+    if (d / (g == d ? 1 : g) % vec == 0) {
+      const ScanPlan p = plan_scan(rays, n_max, d, g, vec);
+      if (p.runs > runs) runs = p.runs;
+      if (p.parts > parts) parts = p.parts;
+    }
+  return runs * d * 8 + (parts > 1 ? parts * n_max * g * 4 : 0);
 }
 
 template <typename T, int GATE, int VEC, bool SHARED>
-int launch_scan(ScanArgs a, bool bwd, hipStream_t st) {
-  int64_t threads;
-  if (SHARED) {
-    const int need = (a.per_gate + VEC - 1) / VEC;
-    a.slot = 1;
-    while (a.slot < need) a.slot <<= 1;
-    threads = a.rays * a.g * a.slot;
-  } else {
-    threads = a.rays * (a.d / VEC);
-  }
-  const int64_t blocks = (threads + 255) / 256;
+int launch_scan(ScanArgs a, bool bwd, char* ws, hipStream_t st) {
+  const ScanPlan p = plan_scan(a.rays, a.n_max, a.d, a.g, VEC);
+  a.slot = p.slot;
+  a.parts = p.parts;
+  a.lanes = p.lanes;
+  a.run_rows = p.run_rows;
+  a.runs = p.runs;
+  a.agg = reinterpret_cast<float2*>(ws);
+  a.partial = reinterpret_cast<float*>(ws + p.runs * a.d * 8);
+  const int64_t threads = (p.run_rows ? p.runs : a.rays) * p.lanes, blocks = (threads + kScanThreads - 1) / kScanThreads;
   GFN_CHECK_ARG(blocks < (1ll << 31), "gfn_ray_scan: %lld rays of %d channels are too many for one launch", (long long)a.rays, a.d);
-  if (bwd) scan_bwd_kernel<T, GATE, VEC, SHARED><<<(unsigned)blocks, 256, 0, st>>>(a);
-  else scan_fwd_kernel<T, GATE, VEC, SHARED><<<(unsigned)blocks, 256, 0, st>>>(a);
+  const unsigned grid = (unsigned)(blocks < 1 ? 1 : blocks);
+  if (p.run_rows) {
+    if (bwd) scan_bwd_kernel<T, GATE, VEC, SHARED, true><<<grid, kScanThreads, 0, st>>>(a);
+    else scan_fwd_kernel<T, GATE, VEC, SHARED, true><<<grid, kScanThreads, 0, st>>>(a);
+    GFN_CHECK_LAUNCH();
+    run_prefix_kernel<<<(unsigned)((a.d + 3) / 4), 1024, 0, st>>>(a.agg, p.runs, a.d);
+    GFN_CHECK_LAUNCH();
+  }
+  if (bwd) scan_bwd_kernel<T, GATE, VEC, SHARED, false><<<grid, kScanThreads, 0, st>>>(a);
+  else scan_fwd_kernel<T, GATE, VEC, SHARED, false><<<grid, kScanThreads, 0, st>>>(a);
   GFN_CHECK_LAUNCH();
+  if (bwd && p.parts > 1 && a.n_max > 0) {
+    const int64_t groups = (a.n_max * a.g + 255) / 256;
+    scan_gate_sums_kernel<T><<<(unsigned)(groups < 4096 ? groups : 4096), 256, 0, st>>>(a, a.partial, p.parts);
+    GFN_CHECK_LAUNCH();
+  }
+  float* to = bwd ? a.dh0 : a.state;
+  if (p.run_rows && to) {  // a walk along a ray sees to an empty ray itself
+    const int64_t groups = (a.rays + 3) / 4;
+    empty_rays_kernel<<<(unsigned)(groups < 512 ? groups : 512), 256, 0, st>>>(a.offsets, a.rays, a.d, bwd ? a.d_state : a.h0, to);
+    GFN_CHECK_LAUNCH();
+  }
   return GFN_OK;
 }
 
 template <typename T, int GATE>
-int dispatch_vec(const ScanArgs& a, bool bwd, hipStream_t st) {
+int dispatch_vec(const ScanArgs& a, bool bwd, char* ws, hipStream_t st) {
   const bool shared = a.g != a.d;
-  const int vec = pick_vec(a, sizeof(T), shared, bwd);
-  if (!shared) return vec == 2 ? launch_scan<T, GATE, 2, false>(a, bwd, st) : launch_scan<T, GATE, 1, false>(a, bwd, st);
-  GFN_CHECK_ARG((a.per_gate + vec - 1) / vec <= 64, "gfn_ray_scan: %d channels share a gate, but their rows are not aligned to %d elements (at most 64 a gate then)",
-                a.per_gate, a.per_gate > 128 ? 4 : 2);
-  if (vec == 4) return launch_scan<T, GATE, 4, true>(a, bwd, st);
-  return vec == 2 ? launch_scan<T, GATE, 2, true>(a, bwd, st) : launch_scan<T, GATE, 1, true>(a, bwd, st);
+  if constexpr (sizeof(T) == 2) {  // two 16-bit channels a lane; f32: one is 256 bytes a wave already
+    if (two_channels(a, shared, bwd)) return shared ? launch_scan<T, GATE, 2, true>(a, bwd, ws, st) : launch_scan<T, GATE, 2, false>(a, bwd, ws, st);
+  }
+  return shared ? launch_scan<T, GATE, 1, true>(a, bwd, ws, st) : launch_scan<T, GATE, 1, false>(a, bwd, ws, st);
 }
 template <typename T>
-int dispatch_gate(const ScanArgs& a, int gate, bool bwd, hipStream_t st) {
-  if (gate == GATE_LINEAR) return dispatch_vec<T, GATE_LINEAR>(a, bwd, st);
-  if (gate == GATE_SIGMOID) return dispatch_vec<T, GATE_SIGMOID>(a, bwd, st);
-  return dispatch_vec<T, GATE_DECAY>(a, bwd, st);
+int dispatch_gate(const ScanArgs& a, int gate, bool bwd, char* ws, hipStream_t st) {
+  if (gate == GATE_LINEAR) return dispatch_vec<T, GATE_LINEAR>(a, bwd, ws, st);
+  if (gate == GATE_SIGMOID) return dispatch_vec<T, GATE_SIGMOID>(a, bwd, ws, st);
+  return dispatch_vec<T, GATE_DECAY>(a, bwd, ws, st);
 }
-int dispatch_scan(const ScanArgs& a, int dtype, int gate, bool bwd, hipStream_t st) {
-  if (a.rays == 0) return GFN_OK;
-  if (dtype == GFN_F32) return dispatch_gate<float>(a, gate, bwd, st);
-  if (dtype == GFN_BF16) return dispatch_gate<__bf16>(a, gate, bwd, st);
-  return dispatch_gate<_Float16>(a, gate, bwd, st);
-}
-
-int zero_tail(const ScanArgs& a, int dtype, void* p, int64_t ld, int width, hipStream_t st) {
-  if (a.n_max == 0) return GFN_OK;
-  const int64_t blocks = (a.n_max * width + 2047) / 2048;
-  const unsigned grid = (unsigned)(blocks < 1024 ? blocks : 1024);
-  if (dtype == GFN_F32) zero_tail_kernel<float><<<grid, 256, 0, st>>>(a.offsets, a.rays, a.n_max, static_cast<float*>(p), ld, width);
-  else zero_tail_kernel<_Float16><<<grid, 256, 0, st>>>(a.offsets, a.rays, a.n_max, static_cast<_Float16*>(p), ld, width);
-  GFN_CHECK_LAUNCH();
-  return GFN_OK;
+int dispatch_scan(const char* who, const ScanArgs& a, int dtype, int gate, bool bwd, void* workspace, int64_t bytes, hipStream_t st) {
+  const int64_t need = scan_workspace(a.rays, a.n_max, a.d, a.g);
+  GFN_CHECK_ARG(bytes >= need && (need == 0 || workspace), "%s: workspace of %lld bytes, %lld needed", who, (long long)bytes, (long long)need);
+  if (a.rays == 0 && !(a.clear && a.n_max > 0)) return GFN_OK;
+  char* ws = static_cast<char*>(workspace);
+  if (dtype == GFN_F32) return dispatch_gate<float>(a, gate, bwd, ws, st);
+  if (dtype == GFN_BF16) return dispatch_gate<__bf16>(a, gate, bwd, ws, st);
+  return dispatch_gate<_Float16>(a, gate, bwd, ws, st);
 }
 
 }  // namespace
 
 extern "C" {
 
+int64_t gfn_ray_scan_workspace(int64_t n_rays, int64_t n_max, int channels, int gates) {
+  if (check_scan("gfn_ray_scan_workspace", n_rays, n_max, channels, gates, GFN_F32, 0, gates, channels)) return GFN_ERR_ARG;
+  return scan_workspace(n_rays, n_max, channels, gates);
+}
+
 int gfn_ray_scan_fwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, int64_t ldf, const void* c, int64_t ldc, int64_t n_max, int channels,
-                     int gates, int dtype, int gate, int reverse, const float* h0, void* h, int64_t ldh, float* state, float* saved, int clear_tail, void* stream) {
+                     int gates, int dtype, int gate, int reverse, const float* h0, void* h, int64_t ldh, float* state, float* saved, int clear_tail,
+                     void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_scan("gfn_ray_scan_fwd", n_rays, n_max, channels, gates, dtype, gate, ldf, ldc)) return rc;
   GFN_CHECK_ARG(pts_offsets && (n_max == 0 || (f && c && h)), "gfn_ray_scan_fwd: null pointer");
   GFN_CHECK_ARG(ldh >= channels, "gfn_ray_scan_fwd: a row stride is below the row's width");
@@ -346,13 +665,14 @@ int gfn_ray_scan_fwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, 
   a.f = f; a.ldf = ldf; a.c = c; a.ldc = ldc; a.h = h; a.ldh = ldh;
   a.d = channels; a.g = gates; a.per_gate = channels / gates; a.reverse = reverse != 0;
   a.h0 = h0; a.state = state; a.saved = saved;
-  if (int rc = dispatch_scan(a, dtype, gate, false, gfn_stream(stream))) return rc;
-  return clear_tail ? zero_tail(a, dtype, h, ldh, channels, gfn_stream(stream)) : GFN_OK;
+  a.clear = clear_tail != 0;
+  return dispatch_scan("gfn_ray_scan_fwd", a, dtype, gate, false, workspace, workspace_bytes, gfn_stream(stream));
 }
 
 int gfn_ray_scan_bwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, int64_t ldf, const void* c, int64_t ldc, const void* dh, int64_t lddh,
                      int64_t n_max, int channels, int gates, int dtype, int gate, int reverse, const float* h0, const float* d_state, const float* saved,
-                     void* df, int64_t lddf, void* dc, int64_t lddc, float* dh0, int clear_tail, void* stream) {
+                     void* df, int64_t lddf, void* dc, int64_t lddc, float* dh0, int clear_tail, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
   if (int rc = check_scan("gfn_ray_scan_bwd", n_rays, n_max, channels, gates, dtype, gate, ldf, ldc)) return rc;
   GFN_CHECK_ARG(pts_offsets && (n_max == 0 || (f && c && dh && saved && df && dc)), "gfn_ray_scan_bwd: null pointer");
   GFN_CHECK_ARG(lddh >= channels && lddf >= gates && lddc >= channels, "gfn_ray_scan_bwd: a row stride is below the row's width");
@@ -362,10 +682,8 @@ int gfn_ray_scan_bwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, 
   a.d = channels; a.g = gates; a.per_gate = channels / gates; a.reverse = reverse != 0;
   a.h0 = h0; a.d_state = d_state; a.saved_in = saved;
   a.df = df; a.lddf = lddf; a.dc = dc; a.lddc = lddc; a.dh0 = dh0;
-  if (int rc = dispatch_scan(a, dtype, gate, true, gfn_stream(stream))) return rc;
-  if (!clear_tail) return GFN_OK;
-  if (int rc = zero_tail(a, dtype, df, lddf, gates, gfn_stream(stream))) return rc;
-  return zero_tail(a, dtype, dc, lddc, channels, gfn_stream(stream));
+  a.clear = clear_tail != 0;
+  return dispatch_scan("gfn_ray_scan_bwd", a, dtype, gate, true, workspace, workspace_bytes, gfn_stream(stream));
 }
 
 int gfn_ray_scan_step(const void* f, int64_t ldf, const void* c, int64_t ldc, int64_t n_rays, int channels, int gates, int dtype, int gate, float* state,

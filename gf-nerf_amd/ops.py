@@ -1392,7 +1392,7 @@ def adam_step_table(p, g, m, v, step, lr=1e-2, beta1=0.9, beta2=0.999, eps=1e-15
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GFN_F32 / GFN_BF16 / GFN_F16
 GATED_ACT = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 SCAN_GATE = {"linear": 0, "sigmoid": 1, "decay": 2}
-SCAN_BLOCK = 16  # GFN_SCAN_BLOCK: rows a saved state covers
+SCAN_BLOCK = 8  # GFN_SCAN_BLOCK: rows a saved state covers
 
 
 def _place(tensors):
@@ -1496,6 +1496,12 @@ def _scan_rays(pts_offsets, what):
     return pts_offsets.numel() - 1
 
 
+def _scan_workspace(rays, n, d, g, device):
+    size = _lib.lib().gfn_ray_scan_workspace(rays, n, d, g)
+    _lib.check(min(size, 0), "gfn_ray_scan_workspace")
+    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+
+
 def ray_scan_fwd(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, out=None, save=False):
     """The gated linear recurrence h_t = a_t h_{t-1} + b_t along each ray's packed samples (front to back; reverse: back to front).
     f [n, gates], c [n, channels] (f32, bf16 or f16; rows at any stride; gate d // (channels // gates) is channel d's):
@@ -1511,9 +1517,10 @@ def ray_scan_fwd(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, out=
     ldh = _rows(h, "out", c.dtype, d, n)
     _place((pts_offsets, f, c, h0, h)); _apart(h, f, c, h0)
     state = torch.empty((R, d), dtype=torch.float32, device=dev)
+    ws, size = _scan_workspace(R, n, d, g, dev)
     saved = torch.empty(((n + SCAN_BLOCK - 1) // SCAN_BLOCK, d), dtype=torch.float32, device=dev) if save else None
     rc = _lib.lib().gfn_ray_scan_fwd(_ptr(pts_offsets), R, _ptr(f), ldf, _ptr(c), ldc, n, d, g, DTYPES[c.dtype], SCAN_GATE[gate], int(reverse), _ptr(h0), _ptr(h), ldh,
-                                     _ptr(state), _ptr(saved), out is None, _stream())
+                                     _ptr(state), _ptr(saved), out is None, _ptr(ws), size, _stream())
     _lib.check(rc, "gfn_ray_scan_fwd")
     return dict(h=h, state=state, saved=saved)
 
@@ -1532,8 +1539,9 @@ def ray_scan_bwd(pts_offsets, f, c, dh, saved, gate="sigmoid", reverse=False, h0
     _place((pts_offsets, f, c, dh, saved, h0, d_state))
     df, dc = torch.empty((n, g), dtype=c.dtype, device=dev), torch.empty((n, d), dtype=c.dtype, device=dev)
     dh0 = torch.empty((R, d), dtype=torch.float32, device=dev)
+    ws, size = _scan_workspace(R, n, d, g, dev)
     rc = _lib.lib().gfn_ray_scan_bwd(_ptr(pts_offsets), R, _ptr(f), ldf, _ptr(c), ldc, _ptr(dh), lddh, n, d, g, DTYPES[c.dtype], SCAN_GATE[gate], int(reverse), _ptr(h0),
-                                     _ptr(d_state), _ptr(saved), _ptr(df), g, _ptr(dc), d, _ptr(dh0), 1, _stream())
+                                     _ptr(d_state), _ptr(saved), _ptr(df), g, _ptr(dc), d, _ptr(dh0), 1, _ptr(ws), size, _stream())
     _lib.check(rc, "gfn_ray_scan_bwd")
     return dict(df=df, dc=dc, dh0=dh0)
 

@@ -775,26 +775,27 @@ int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, co
 
 /* The gated linear recurrence along each ray's packed samples: h_t = a_t h_{t-1} + b_t from h_{-1} = h0, front to back, or (reverse
  * != 0) back to front.  f [n, gates] and c [n, channels] of type dtype (row strides ldf / ldc in elements); gates divides channels
- * (at most 4096) and gate d / (channels / gates) belongs to channel d; a gate is shared by at most 64 channels (256 where rows are
- * aligned to 4 elements), or every channel has its own.
+ * (at most 4096) and gate d / (channels / gates) belongs to channel d.
  *   gate 0 (linear)   a = f,            b = c
  *   gate 1 (sigmoid)  a = sigmoid(f),   b = (1 - a) c
  *   gate 2 (decay)    a = exp(-f),      b = (1 - a) c     (f = sigma dt: reverse, this composites `channels` feature channels)
  * h0 f32 [n_rays, channels] (NULL: 0); h [n, channels] of type dtype: every row's state, rounded once; state f32 [n_rays, channels]
- * (may be NULL): each ray's last state (an empty ray's is its h0).  saved f32 [(n_max + 15) / 16, channels] (may be NULL): what
+ * (may be NULL): each ray's last state (an empty ray's is its h0).  saved f32 [(n_max + 7) / 8, channels] (may be NULL): what
  * gfn_ray_scan_bwd needs from the forward.  pts_offsets i32 [n_rays + 1] ascending from 0; rows behind the last ray's are not read, and
- * their rows of h are left as they are, or cleared (clear_tail != 0). */
-#define GFN_SCAN_BLOCK 16
+ * their rows of h are left as they are, or cleared (clear_tail != 0).  workspace: gfn_ray_scan_workspace bytes of device memory (0 for
+ * short rays), 16-byte aligned, owned by the call until its work is done (two calls in flight need two). */
+#define GFN_SCAN_BLOCK 8
 #define GFN_SCAN_MAX_CHANNELS 4096
+int64_t gfn_ray_scan_workspace(int64_t n_rays, int64_t n_max, int channels, int gates);
 int gfn_ray_scan_fwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, int64_t ldf, const void* c, int64_t ldc,
                      int64_t n_max, int channels, int gates, int dtype, int gate, int reverse, const float* h0, void* h,
-                     int64_t ldh, float* state, float* saved, int clear_tail, void* stream);
+                     int64_t ldh, float* state, float* saved, int clear_tail, void* workspace, int64_t workspace_bytes, void* stream);
 /* Its gradients for dh = d loss / d h (type dtype) and d_state = d loss / d state (f32, NULL: 0): df, dc of type dtype, dh0 f32
  * [n_rays, channels] (may be NULL), all written.  f, c, h0, pts_offsets and the flags as in the forward call that wrote `saved`. */
 int gfn_ray_scan_bwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, int64_t ldf, const void* c, int64_t ldc,
                      const void* dh, int64_t lddh, int64_t n_max, int channels, int gates, int dtype, int gate, int reverse,
                      const float* h0, const float* d_state, const float* saved, void* df, int64_t lddf, void* dc, int64_t lddc,
-                     float* dh0, int clear_tail, void* stream);
+                     float* dh0, int clear_tail, void* workspace, int64_t workspace_bytes, void* stream);
 /* One more sample of every ray: state[r] = a state[r] + b in place, h [n_rays, channels] = state rounded to dtype. */
 int gfn_ray_scan_step(const void* f, int64_t ldf, const void* c, int64_t ldc, int64_t n_rays, int channels, int gates,
                       int dtype, int gate, float* state, void* h, int64_t ldh, void* stream);

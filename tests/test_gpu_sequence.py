@@ -378,7 +378,7 @@ def test_ray_scan_refusals(T, ops):
                 lambda: ops.ray_scan_fwd(off, f, c, out=c), lambda: ops.ray_scan_fwd(off, f, c, out=c.half()), lambda: ops.ray_scan_bwd(off, f, c, c, None),
                 lambda: ops.ray_scan_bwd(off, f, c, c, s[:0]), lambda: ops.ray_scan_bwd(off, f, c, c[:, :4], s), lambda: ops.ray_scan_bwd(off, f, c, c, s, d_state=z[0]),
                 lambda: ops.ray_scan_step(f, c, z), lambda: ops.ray_scan_step(f[:2], c[:2], z.half()), lambda: ops.ray_scan_step(f[:2], c[:2], None),
-                lambda: ops.ray_scan_fwd(off, f[:, :1].expand(8, 4), c), lambda: ops.ray_scan_fwd(off, T.zeros(8, 1, device="cuda"), T.zeros(8, 300, device="cuda"))):
+                lambda: ops.ray_scan_fwd(off, f[:, :1].expand(8, 4), c)):
         with pytest.raises(_lib.GfnError):
             bad()
     empty = ops.ray_scan_fwd(T.zeros(1, dtype=T.int32, device="cuda"), f[:0], c[:0], save=True)
@@ -588,12 +588,12 @@ def test_offsets_past_32_bits(T, ops):
     f = T.full((n, 20), 0.5, dtype=T.bfloat16, device="cuda")  # 50 channels a gate
     small = ops.ray_scan_fwd(T.tensor([0, 200], dtype=T.int32, device="cuda"), f[-200:], x[-200:], save=True)
     r = ops.ray_scan_fwd(off, f, x, save=True)
-    assert T.equal(r["h"][-200:], small["h"]) and T.equal(r["state"][1:], small["state"])
+    # the rows meet other tiles' borders in the two calls: f32 states a few units apart, of which a few round to the next bf16 number (2^-7 away)
+    near = lambda p, q: float((p.float() - q.float()).norm() / q.float().norm()) <= oseq.HALF["bf16"]  # noqa: E731
+    assert near(r["h"][-200:], small["h"]) and float((r["state"][1:] - small["state"]).norm() / small["state"].norm()) <= 1e-6
     want = ops.ray_scan_bwd(T.tensor([0, 200], dtype=T.int32, device="cuda"), f[-200:], x[-200:], x[-200:], small["saved"])
     b = ops.ray_scan_bwd(off, f, x, x, r["saved"])
-    # the saved states of a block of 16 rows start at other rows in the small call: the same recurrence, restarted elsewhere
-    for k in ("df", "dc"):
-        assert float((b[k][-200:].float() - want[k].float()).norm() / want[k].float().norm()) <= 2 * oseq.HALF["bf16"]
+    assert near(b["df"][-200:], want["df"]) and near(b["dc"][-200:], want["dc"])
     del r, b, x, f
     w = T.randn(1000, 8, device="cuda").bfloat16()
     z = T.randn(n, 8, device="cuda").bfloat16()

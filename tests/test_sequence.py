@@ -64,22 +64,22 @@ def test_gated_workspace_is_a_function_of_the_sizes(lib):
 
 
 def scan_args(**k):
-    a = dict(off=P, rays=10, f=P, ldf=8, c=P, ldc=32, n=100, d=32, g=8, dtype=0, gate=1, rev=0, h0=None, h=P, ldh=32, state=P, saved=None, tail=0, st=None)
+    a = dict(off=P, rays=10, f=P, ldf=8, c=P, ldc=32, n=100, d=32, g=8, dtype=0, gate=1, rev=0, h0=None, h=P, ldh=32, state=P, saved=None, tail=0, ws=None, size=0, st=None)
     return list({**a, **k}.values())
 
 
 @pytest.mark.parametrize("change,match", [
     (dict(d=0), "gates for"), (dict(d=4097, ldc=4097), "gates for"), (dict(g=0), "gates for"), (dict(g=5), "gates for"), (dict(g=64, ldf=64), "gates for"),
-    (dict(d=2048, g=4, ldc=2048, ldh=2048), "share a gate"), (dict(rays=-1), "rays"), (dict(n=1 << 31), "n_max"), (dict(dtype=3), "dtype"), (dict(gate=3), "gate 3"),
+    (dict(rays=-1), "rays"), (dict(n=1 << 31), "n_max"), (dict(dtype=3), "dtype"), (dict(gate=3), "gate 3"),
     (dict(off=None), "null"), (dict(f=None), "null"), (dict(c=None), "null"), (dict(h=None), "null"), (dict(ldf=7), "row stride"), (dict(ldc=31), "row stride"),
-    (dict(ldh=31), "row stride"), (dict(d=260, g=2, ldc=261, ldh=260), "aligned")])
+    (dict(ldh=31), "row stride")])
 def test_ray_scan_fwd_refuses(lib, change, match):
     refused(lib, "gfn_ray_scan_fwd", *scan_args(**change), match=match)
 
 
 def scan_bwd_args(**k):
     a = dict(off=P, rays=10, f=P, ldf=8, c=P, ldc=32, dh=P, lddh=32, n=100, d=32, g=8, dtype=0, gate=1, rev=0, h0=None, ds=None, saved=P, df=P, lddf=8, dc=P, lddc=32, dh0=None,
-             tail=0, st=None)
+             tail=0, ws=None, size=0, st=None)
     return list({**a, **k}.values())
 
 
@@ -87,6 +87,15 @@ def scan_bwd_args(**k):
                                           (dict(lddc=31), "row stride"), (dict(lddh=31), "row stride"), (dict(g=3), "gates for")])
 def test_ray_scan_bwd_refuses(lib, change, match):
     refused(lib, "gfn_ray_scan_bwd", *scan_bwd_args(**change), match=match)
+
+
+def test_ray_scan_workspace(lib):
+    f = lib.lib().gfn_ray_scan_workspace
+    assert f(10, 100, 32, 8) == 0 and f(10, 0, 32, 8) == 0            # short rays need none
+    assert f(10, 100000, 32, 8) > 0 and f(1, 1 << 20, 128, 128) > 0
+    assert f(10, 100, 0, 1) == -1 and f(10, 100, 32, 5) == -1
+    refused(lib, "gfn_ray_scan_fwd", *scan_args(rays=10, n=100000), match="workspace of 0")
+    refused(lib, "gfn_ray_scan_bwd", *scan_bwd_args(rays=10, n=100000, ws=P, size=64), match="workspace of 64")
 
 
 def test_ray_scan_step_and_dropout_refuse(lib):
