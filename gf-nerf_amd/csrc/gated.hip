@@ -68,14 +68,24 @@ __global__ __launch_bounds__(64 * kWaves) void gated_fwd_kernel(int64_t n_max, c
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, kg = lane >> 4;
   const int pairs = ((h - h0 < hc ? h - h0 : hc) + 31) / 32;
   const char* wrow = lds + j * ROW + kg * 16;
-  for (int64_t s0 = ((int64_t)blockIdx.x * kWaves + wave) * 16 * G; s0 < n; s0 += (int64_t)gridDim.x * kWaves * 16 * G) {
-    u32x4 xr[G][KS];
+  const int64_t stride = (int64_t)gridDim.x * kWaves * 16 * G;
+  int64_t s0 = ((int64_t)blockIdx.x * kWaves + wave) * 16 * G;
+  u32x4 xr[G][KS], next[G][KS];
+  auto fetch = [&](u32x4 (&to)[G][KS], int64_t first) {
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      const int64_t s = s0 + 16 * g + j;
+      const int64_t s = first + 16 * g + j;
 #pragma unroll
-      for (int u = 0; u < KS; u++) xr[g][u] = s < n ? row_piece(x + s * ldx, 4 * u + kg, k) : u32x4{0u, 0u, 0u, 0u};
+      for (int u = 0; u < KS; u++) to[g][u] = s < n ? row_piece(x + s * ldx, 4 * u + kg, k) : u32x4{0u, 0u, 0u, 0u};
     }
+  };
+  if (s0 < n) fetch(next, s0);
+  for (; s0 < n; s0 += stride) {
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int u = 0; u < KS; u++) xr[g][u] = next[g][u];
+    if (s0 + stride < n) fetch(next, s0 + stride);  // on its way under this tile's work
     for (int p = 0; p < pairs; p++) {
       f32x4 acc[2][2][G];  // [matrix][tile]
 #pragma unroll
@@ -126,6 +136,9 @@ __device__ __forceinline__ u32x2 tr4(const char* a) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a));
 }
 
+// waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit
+constexpr int bwd_waves(int ks) { return ks >= 3 && ks <= 5 ? 8 : 4; }
+
 struct GatedBwd {
   int64_t n_max;
   const int32_t* n_dev;
@@ -135,11 +148,13 @@ struct GatedBwd {
   void* dx;           // T, or null
   float* dx_sum;      // f32 [n_max][k] between the launches of several feature blocks, or null
   int dx_first, dx_last;
+  int z_buffers;      // 1 or 2 tiles of dz in LDS
   float* part;        // [workgroup][64 NP][KP] f32, or null
 };
 
-template <typename T, int KS, int NP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
+template <typename T, int KS, int NP>
+__global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_kernel(GatedBwd a) {
+  constexpr int WAVES = bwd_waves(KS);
   constexpr int E = Piece<T>::E, TPU = sizeof(T) == 4 ? 1 : 2;  // 16-column tiles a unit
   constexpr int KP = KS * 4 * E, KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP;
   constexpr int SAMPLES = 16 * WAVES, ZROW = 64 * (int)sizeof(T) + 16;
@@ -147,8 +162,8 @@ __global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
   constexpr bool EXACT = sizeof(T) == 4, SCALED = sizeof(T) == 2 && !__is_same(T, __bf16);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* xs = lds + 2 * HB * ROW;        // [SAMPLES][ROW]
-  char* zs = xs + SAMPLES * ROW;        // [SAMPLES][dg 32 | du 32]
-  float* top = reinterpret_cast<float*>(zs + SAMPLES * ZROW);  // [WAVES]
+  char* zs = xs + SAMPLES * ROW;        // [z_buffers][SAMPLES][dg 32 | du 32]
+  float* top = reinterpret_cast<float*>(zs + a.z_buffers * SAMPLES * ZROW);  // [WAVES]
   const T *x = static_cast<const T*>(a.x), *dh = static_cast<const T*>(a.dh);
   const bool ones = a.bg != nullptr;
   const int k = a.k, h = a.h, h0 = a.h0, act = a.act;
@@ -164,43 +179,64 @@ __global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
   int run_e = 0;  // dw holds the sums times 2^run_e
   const char* wrow = lds + j * ROW + kg * 16;
   const int64_t tiles = (n + SAMPLES - 1) / SAMPLES;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+  constexpr int DP = 8 / E;  // pieces of eight features
+  const int width = h - h0 < HB ? h - h0 : HB;
+  constexpr bool AHEAD = KS < 4;  // dh of the next tile is requested with its x where registers are left for it
+  u32x4 xr[KS], xn[KS], dr[NP][DP], dn[AHEAD ? NP : 1][DP];
+  auto fetch_dh = [&](int64_t s, u32x4 (&to)[DP], int p) {
+#pragma unroll
+    for (int q = 0; q < DP; q++) to[q] = s < n ? row_piece(dh + s * a.lddh + h0, (32 * p + 8 * kg) / E + q, width) : u32x4{0u, 0u, 0u, 0u};
+  };
+  auto fetch = [&](int64_t tile) {
     const int64_t s = tile * SAMPLES + wave * 16 + j;
-    u32x4 xr[KS];
 #pragma unroll
     for (int u = 0; u < KS; u++) {
       const int c = 4 * u + kg;
-      xr[u] = s < n ? row_piece(x + s * a.ldx, c, k) : u32x4{0u, 0u, 0u, 0u};
+      xn[u] = s < n ? row_piece(x + s * a.ldx, c, k) : u32x4{0u, 0u, 0u, 0u};
       if (ones && s < n && k / E == c) {
         T t[E];
-        __builtin_memcpy(t, &xr[u], 16);
+        __builtin_memcpy(t, &xn[u], 16);
 #pragma unroll
         for (int i = 0; i < E; i++)
           if (i == k % E) t[i] = (T)1.f;
-        __builtin_memcpy(&xr[u], t, 16);
+        __builtin_memcpy(&xn[u], t, 16);
       }
     }
-    float d[NP][8];
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int p = 0; p < NP; p++) fetch_dh(s, dn[p], p);
+    }
+  };
+  if ((int64_t)blockIdx.x < tiles) fetch(blockIdx.x);
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t s = tile * SAMPLES + wave * 16 + j;
+#pragma unroll
+    for (int u = 0; u < KS; u++) xr[u] = xn[u];
 #pragma unroll
     for (int p = 0; p < NP; p++) {
-      const int f = h0 + 32 * p + 8 * kg;
-      if (s < n) {
-        load_row8(dh + s * a.lddh + f, h - f, d[p]);
-      } else {
+      if constexpr (AHEAD) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) d[p][i] = 0.f;
+        for (int q = 0; q < DP; q++) dr[p][q] = dn[p][q];
+      } else {
+        fetch_dh(s, dr[p], p);
       }
     }
     __syncthreads();  // the weights are staged (first tile); the tile before has been read from xs, zs and top
 #pragma unroll
     for (int u = 0; u < KS; u++) *reinterpret_cast<u32x4*>(xs + (wave * 16 + j) * ROW + u * 64 + kg * 16) = xr[u];
-    float back = 1.f;
+    if (tile + gridDim.x < tiles) fetch(tile + gridDim.x);  // on its way under this tile's work
+    auto grad = [&](int p, int i) {  // dh of feature 32 p + 8 kg + i
+      T t[E];
+      __builtin_memcpy(t, &dr[p][i / E], 16);
+      return (float)t[i % E];
+    };
+    float back = 1.f, to = 1.f;
     if constexpr (SCALED) {
       float m = 0.f;
 #pragma unroll
       for (int p = 0; p < NP; p++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, __builtin_fabsf(d[p][i]));
+        for (int i = 0; i < 8; i++) m = fmaxf(m, __builtin_fabsf(grad(p, i)));
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
       if (lane == 0) top[wave] = m;
@@ -209,12 +245,8 @@ __global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
 #pragma unroll
       for (int w = 1; w < WAVES; w++) m = fmaxf(m, top[w]);
       const int e = __builtin_amdgcn_readfirstlane(tile_scale_exponent(m, run_e));
-      const float to = pow2(e);
+      to = pow2(e);
       back = pow2(-e);
-#pragma unroll
-      for (int p = 0; p < NP; p++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) d[p][i] *= to;
       if (e != run_e) {
         const float by = pow2(e - run_e);
 #pragma unroll
@@ -242,7 +274,10 @@ __global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
           for (int t = 0; t < 2; t++)
             acc[m][t] = mma(*reinterpret_cast<const u32x4*>(wrow + (m * HB + 32 * p + 16 * t) * ROW + u * 64), xr[u], acc[m][t], (T*)nullptr);
       T z[2][8];
-      gated8_grad<EXACT>(act, [&](int i) { return acc[0][i >> 2][i & 3]; }, [&](int i) { return acc[1][i >> 2][i & 3]; }, d[p], z[0], z[1]);
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) d[i] = SCALED ? grad(p, i) * to : grad(p, i);
+      gated8_grad<EXACT>(act, [&](int i) { return acc[0][i >> 2][i & 3]; }, [&](int i) { return acc[1][i >> 2][i & 3]; }, d, z[0], z[1]);
       if (a.dx || a.dx_sum) {  // dx[k] += sum over these 32 features
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -270,15 +305,16 @@ __global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
         }
       }
       if (a.part) {
-        if (p) __syncthreads();  // the features before have been read
-        char* zr = zs + (wave * 16 + j) * ZROW + 8 * kg * sizeof(T);
+        if (p && a.z_buffers == 1) __syncthreads();  // the features before have been read; of two buffers, the one before those
+        char* zb = zs + (p & (a.z_buffers - 1)) * SAMPLES * ZROW;
+        char* zr = zb + (wave * 16 + j) * ZROW + 8 * kg * sizeof(T);
         __builtin_memcpy(__builtin_assume_aligned(zr, 16), z[0], sizeof(z[0]));
         __builtin_memcpy(__builtin_assume_aligned(zr + 32 * sizeof(T), 16), z[1], sizeof(z[1]));
         __syncthreads();
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
           for (int c = 0; c < SAMPLES; c += 32) {  // rows 8 kg .. 8 kg + 7 of these 32 samples
-            const char* r = zs + (c + 8 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
+            const char* r = zb + (c + 8 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
             const u32x2 l = tr4(r), u = tr4(r + 4 * ZROW);
             const u32x4 av = {l[0], l[1], u[0], u[1]};
             const char* q = xs + (c + 8 * kg + (j >> 2)) * ROW + 4 * (j & 3) * 2;
@@ -292,7 +328,7 @@ __global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
         } else {
 #pragma unroll 4
           for (int c = 0; c < SAMPLES; c += 4) {
-            const float av = *reinterpret_cast<const float*>(zs + (c + kg) * ZROW + (16 * ft + j) * 4);
+            const float av = *reinterpret_cast<const float*>(zb + (c + kg) * ZROW + (16 * ft + j) * 4);
             const char* q = xs + (c + kg) * ROW + j * 4;
 #pragma unroll
             for (int t = 0; t < KT_WAVE; t++)
@@ -340,22 +376,25 @@ __global__ __launch_bounds__(64 * WAVES) void gated_bwd_kernel(GatedBwd a) {
   }
 }
 
-// dW[f][c] = sum over the workgroups of part[f's row][c], in their order: 32 columns x 8 runs of workgroups a block
+// dW[f][c] = sum over the workgroups of part[f's row][c], in their order: 32 columns x 32 runs of workgroups a block
 template <typename T>
-__global__ __launch_bounds__(256) void gated_reduce_kernel(const float* __restrict__ part, int parts, int rows, int kp, int k, int h, int h0, int cols,
-                                                           T* __restrict__ dwg, T* __restrict__ dwu, T* __restrict__ dbg, T* __restrict__ dbu) {
-  __shared__ float sums[8][32];
+__global__ __launch_bounds__(1024) void gated_reduce_kernel(const float* __restrict__ part, int parts, int rows, int kp, int k, int h, int h0, int cols,
+                                                            T* __restrict__ dwg, T* __restrict__ dwu, T* __restrict__ dbg, T* __restrict__ dbu) {
+  __shared__ float sums[32][33];
   const int col = threadIdx.x & 31, run = threadIdx.x >> 5, row = blockIdx.y;
   const int c = blockIdx.x * 32 + col, f = h0 + (row >> 6) * 32 + (row & 31);
-  const int per = (parts + 7) / 8;
+  const int per = (parts + 31) / 32, last = parts < (run + 1) * per ? parts : (run + 1) * per;
   float s = 0.f;
-  if (c < cols && f < h)
-    for (int b = run * per; b < parts && b < (run + 1) * per; b++) s += part[((int64_t)b * rows + row) * kp + c];
+  if (c < cols && f < h) {
+    const float* p = part + (int64_t)row * kp + c;
+#pragma unroll 16
+    for (int b = run * per; b < last; b++) s += p[(int64_t)b * rows * kp];
+  }
   sums[run][col] = s;
   __syncthreads();
   if (run || c >= cols || f >= h) return;
 #pragma unroll
-  for (int r = 1; r < 8; r++) s += sums[r][col];
+  for (int r = 1; r < 32; r++) s += sums[r][col];
   const bool up = (row >> 5) & 1;
   if (c < k) (up ? dwu : dwg)[(int64_t)f * k + c] = (T)s;
   else (up ? dbu : dbg)[f] = (T)s;
@@ -415,14 +454,14 @@ int dispatch_fwd(const GatedFwd& a, hipStream_t st) {
   const bool few = a.n_max < 16384;  // a sample group a wave: more workgroups
 #define GFN_GATED(KS, G)                                                             \
   if (units <= KS) return few ? launch_fwd<T, KS, 1>(a, st) : launch_fwd<T, KS, G>(a, st)
-  GFN_GATED(1, 4);
-  GFN_GATED(2, 4);
+  GFN_GATED(1, 2);
+  GFN_GATED(2, 2);
   if constexpr (sizeof(T) == 4) {
-    GFN_GATED(4, 4);
+    GFN_GATED(4, 2);
     GFN_GATED(8, 2);
   } else {
-    GFN_GATED(3, 4);
-    GFN_GATED(4, 4);
+    GFN_GATED(3, 2);
+    GFN_GATED(4, 2);
   }
 #undef GFN_GATED
   return GFN_ERR_ARG;
@@ -430,7 +469,7 @@ int dispatch_fwd(const GatedFwd& a, hipStream_t st) {
 
 // The backward's plan for (n, k + bias, h, type): units a row, feature blocks of 32 NP, waves and workgroups.
 struct BwdPlan {
-  int ks, np, waves, blocks, launches;
+  int ks, np, waves, blocks, launches, z_buffers;
   size_t lds, part_floats;
   bool dx_sum;
 };
@@ -441,13 +480,17 @@ BwdPlan plan_bwd(int64_t n, int k, int h, int dtype, bool bias) {
   const int units = (k + (bias ? 1 : 0) + 4 * e - 1) / (4 * e);
   p.ks = units;
   if (dtype == GFN_F32 && units > 5) p.ks = 9;
-  p.waves = dtype != GFN_F32 && units >= 4 ? 8 : 4;
-  const int most = dtype == GFN_F32 ? (p.ks > 5 ? 2 : 4) : (p.ks > 4 ? 2 : 4);  // 32-feature pairs a launch: the weights and dW's accumulators fit
+  p.waves = bwd_waves(p.ks);
+  const int most = p.ks > 4 ? 2 : 4;  // 32-feature pairs a launch: the weights and dW's accumulators fit
   const int pairs = (h + 31) / 32;
   p.np = pairs >= 3 && most == 4 ? 4 : pairs >= 2 ? 2 : 1;
   p.launches = (pairs + p.np - 1) / p.np;
   const int row = p.ks * 64 + 16, samples = 16 * p.waves;
-  p.lds = (size_t)64 * p.np * row + (size_t)samples * row + (size_t)samples * (64 * size + 16) + 64;
+  const size_t z = (size_t)samples * (64 * size + 16);
+  p.lds = (size_t)64 * p.np * row + (size_t)samples * row + z + 64;
+  // a second buffer for dz (one barrier a pair of tiles instead of two) where it does not cost the CU its second workgroup
+  p.z_buffers = p.np > 1 && (p.lds + z <= 80 * 1024 || (p.lds > 80 * 1024 && p.lds + z <= 160 * 1024)) ? 2 : 1;
+  p.lds += (p.z_buffers - 1) * z;
   const int64_t tiles = (n + samples - 1) / samples;
   const int at_once = 256 * (p.lds <= 80 * 1024 ? 2 : 1);
   p.blocks = (int)(tiles < at_once ? tiles : at_once);
@@ -457,39 +500,33 @@ BwdPlan plan_bwd(int64_t n, int k, int h, int dtype, bool bias) {
   return p;
 }
 
-template <typename T, int KS, int NP, int WAVES>
+template <typename T, int KS, int NP>
 int launch_bwd(const GatedBwd& a, const BwdPlan& p, hipStream_t st) {
   static unsigned long long seen = 0;
   if (gfn_first_call_on_device(seen))
-    if (int rc = allow_lds(gated_bwd_kernel<T, KS, NP, WAVES>, 160 * 1024)) return rc;
-  gated_bwd_kernel<T, KS, NP, WAVES><<<p.blocks, 64 * WAVES, p.lds, st>>>(a);
+    if (int rc = allow_lds(gated_bwd_kernel<T, KS, NP>, 160 * 1024)) return rc;
+  gated_bwd_kernel<T, KS, NP><<<p.blocks, 64 * p.waves, p.lds, st>>>(a);
   GFN_CHECK_LAUNCH();
   return GFN_OK;
 }
 
 template <typename T>
 int dispatch_bwd(const GatedBwd& a, const BwdPlan& p, hipStream_t st) {
-#define GFN_GATED_NP(KS, NP, WAVES) \
-  if (p.ks == KS && p.np == NP) return launch_bwd<T, KS, NP, WAVES>(a, p, st)
-#define GFN_GATED(KS, WAVES)   \
-  GFN_GATED_NP(KS, 1, WAVES);  \
-  GFN_GATED_NP(KS, 2, WAVES);  \
-  GFN_GATED_NP(KS, 4, WAVES)
+#define GFN_GATED_NP(KS, NP) \
+  if (p.ks == KS && p.np == NP) return launch_bwd<T, KS, NP>(a, p, st)
+#define GFN_GATED(KS)   \
+  GFN_GATED_NP(KS, 1);  \
+  GFN_GATED_NP(KS, 2);  \
+  GFN_GATED_NP(KS, 4)
+  GFN_GATED(1);
+  GFN_GATED(2);
+  GFN_GATED(3);
+  GFN_GATED(4);
+  GFN_GATED_NP(5, 1);
+  GFN_GATED_NP(5, 2);
   if constexpr (sizeof(T) == 4) {
-    GFN_GATED(1, 4);
-    GFN_GATED(2, 4);
-    GFN_GATED(3, 4);
-    GFN_GATED(4, 4);
-    GFN_GATED(5, 4);
-    GFN_GATED_NP(9, 1, 4);
-    GFN_GATED_NP(9, 2, 4);
-  } else {
-    GFN_GATED(1, 4);
-    GFN_GATED(2, 4);
-    GFN_GATED(3, 4);
-    GFN_GATED(4, 8);
-    GFN_GATED_NP(5, 1, 8);
-    GFN_GATED_NP(5, 2, 8);
+    GFN_GATED_NP(9, 1);
+    GFN_GATED_NP(9, 2);
   }
 #undef GFN_GATED
 #undef GFN_GATED_NP
@@ -506,7 +543,7 @@ int gated_bwd_typed(GatedBwd a, const BwdPlan& p, int kp, void* dwg, void* dwu, 
     a.dx_last = l == p.launches - 1;
     if (int rc = dispatch_bwd<T>(a, p, st)) return rc;
     if (a.part) {
-      gated_reduce_kernel<T><<<dim3((unsigned)((cols + 31) / 32), (unsigned)(64 * p.np)), 256, 0, st>>>(
+      gated_reduce_kernel<T><<<dim3((unsigned)((cols + 31) / 32), (unsigned)(64 * p.np)), 1024, 0, st>>>(
           a.part, p.blocks, 64 * p.np, kp, a.k, a.h, a.h0, cols, static_cast<T*>(dwg), static_cast<T*>(dwu), static_cast<T*>(dbg), static_cast<T*>(dbu));
       GFN_CHECK_LAUNCH();
     }
@@ -560,6 +597,7 @@ int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, co
   a.ldx = ldx; a.lddh = lddh; a.lddx = lddx;
   a.k = in_dim; a.h = hidden; a.act = act;
   a.dx = dx;
+  a.z_buffers = p.z_buffers;
   float* ws = static_cast<float*>(workspace);
   if (dwg) {
     a.part = ws;

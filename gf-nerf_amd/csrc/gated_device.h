@@ -71,19 +71,6 @@ __device__ __forceinline__ u32x4 row_piece(const T* row, int c, int k) {
   return v;
 }
 
-// eight consecutive values of a row -> f32, zeros from `left` on
-template <typename T>
-__device__ __forceinline__ void load_row8(const T* p, int left, float (&v)[8]) {
-  if (left >= 8) {
-    T e[8];
-    __builtin_memcpy(e, p, sizeof(e));
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (float)e[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = i < left ? (float)p[i] : 0.f;
-  }
-}
 template <typename T, int N>
 __device__ __forceinline__ void store_row(T* p, int left, const float (&v)[N]) {
   using Row = __attribute__((ext_vector_type(N))) T;
@@ -105,31 +92,46 @@ __device__ __forceinline__ void store_row(T* p, int left, const float (&v)[N]) {
   }
 }
 
-// 1 / (1 + exp(-z)) and the same of -z, each to the last bits of f32 (EXACT) or of the hardware's exp and reciprocal (2^-22: far
-// below the rounding of a 16-bit result).
+// 1 / (1 + exp(-z)).  For 16-bit results the hardware's exp2 and reciprocal as they are (2^-22 of the value: far below the result's rounding);
+// EXACT (f32): the argument's rounding put back (exp2(t + r) = exp2(t) (1 + r ln 2)) and one Newton step on the reciprocal.
 template <bool EXACT>
 __device__ __forceinline__ float sigmoid(float z) {
-  if constexpr (EXACT) return 1.f / (1.f + expf(-z));
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
+  const float t = z * -1.44269504088896340736f;
+  float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (!EXACT) return __builtin_amdgcn_rcpf(1.f + e);
+  e = __builtin_fmaf(e, __builtin_fmaf(z, -1.44269504088896340736f, -t) * 0.693147180559945309417f, e);
+  const float d = 1.f + e, r = __builtin_amdgcn_rcpf(d);
+  const float s = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.f), r);
+  return t > 126.f ? 0.f : (t < -126.f ? 1.f : s);  // where exp2 over- or underflows the two steps would meet inf - inf
 }
 
-// Phi(z) = (1 + erf(z / sqrt 2)) / 2.  EXACT: erfcf, which keeps the relative accuracy of the tail of z -> -inf.  Else the rational
-// approximation of Abramowitz & Stegun 7.1.26 of erfc(|z| / sqrt 2) = poly(t) exp(-z^2 / 2), |error| <= 1.5e-7 before the exponential;
-// `gauss` = exp(-z^2 / 2) comes with it (the derivative needs it as well).
+// Phi(z) = erfc(-z / sqrt 2) / 2, and gauss = exp(-z^2 / 2), which its derivative needs as well.  EXACT (f32): the Chebyshev fit of Press et al.
+// (Numerical Recipes, erfcc), 1.2e-7 of the value everywhere, the tail of z -> -inf included.  Else Abramowitz & Stegun 7.1.26, 1.5e-7 absolute.
 template <bool EXACT>
 __device__ __forceinline__ float normal_cdf(float z, float& gauss) {
-  const float h = -0.72134752044448170368f * z * z;  // -z^2 / 2 / ln 2
+  gauss = __builtin_amdgcn_exp2f(-0.72134752044448170368f * z * z);  // -z^2 / 2 / ln 2
+  const float x = 0.70710678118654752440f * __builtin_fabsf(z);
+  float tail;
   if constexpr (EXACT) {
-    gauss = expf(-0.5f * z * z);
-    return 0.5f * erfcf(z * -0.70710678118654752440f);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, x, 1.f));
+    float p = __builtin_fmaf(0.17087277f, t, -0.82215223f);
+    p = __builtin_fmaf(p, t, 1.48851587f);
+    p = __builtin_fmaf(p, t, -1.13520398f);
+    p = __builtin_fmaf(p, t, 0.27886807f);
+    p = __builtin_fmaf(p, t, -0.18628806f);
+    p = __builtin_fmaf(p, t, 0.09678418f);
+    p = __builtin_fmaf(p, t, 0.37409196f);
+    p = __builtin_fmaf(p, t, 1.00002368f);
+    p = __builtin_fmaf(p, t, -1.26551223f);
+    tail = 0.5f * t * gauss * __builtin_amdgcn_exp2f(p * 1.44269504088896340736f);
+  } else {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f);
+    tail = 0.5f * p * t * gauss;
   }
-  gauss = __builtin_amdgcn_exp2f(h);
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752440f, __builtin_fabsf(z), 1.f));
-  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-  p = __builtin_fmaf(p, t, 1.421413741f);
-  p = __builtin_fmaf(p, t, -0.284496736f);
-  p = __builtin_fmaf(p, t, 0.254829592f);
-  const float tail = 0.5f * p * t * gauss;
   return z < 0.f ? tail : 1.f - tail;
 }
 
