@@ -13,8 +13,8 @@
 //   [dWg; dWu] = [dg; du]^T x                  contracts over the samples: the wave's dz goes to LDS and every wave accumulates its own
 //                                              rows of dW over all samples of the tile, in registers until the workgroup's last tile.
 // One pass: x and dh are read once, dx is written once; each workgroup's partial dW goes to a workspace and a second launch adds the
-// partials in a fixed order (no atomics: the same bits every run).  The biases' gradients are one more column of dW: x gets a column
-// of ones behind its last (and W the bias there, so the recomputed g and u have it too).
+// partials in a fixed order (no atomics: the same bits every run).  The biases' gradients are the same product against a column of ones
+// and travel as column k of the partials.
 // dz is rounded to the operands' type for the two products -- 2^-9 (bf16) / 2^-12 (f16) per term, below the rounding of the results
 // themselves; f32 stays f32.  f16 has the precision but not the range: see tile_scale.
 #include "gated_device.h"
@@ -23,34 +23,48 @@ namespace {
 
 constexpr int kWaves = 4;
 
+template <int V>
+struct Constant {
+  static constexpr int value = V;
+};
+// f for the activation's own constant: the choice is made once, outside of what f does.
+template <typename F>
+__device__ __forceinline__ void for_act(int act, F f) {
+  switch (act) {
+    case GATED_SILU: return f(Constant<GATED_SILU>{});
+    case GATED_GELU: return f(Constant<GATED_GELU>{});
+    case GATED_RELU: return f(Constant<GATED_RELU>{});
+    default: return f(Constant<GATED_SIGMOID>{});
+  }
+}
+
 // row i of tile t <-> hidden feature 32 p + 8 (i >> 2) + 4 t + (i & 3); the LDS image keeps rows in tile order
 __device__ __forceinline__ int image_feature(int row) { return (row & ~31) + 8 * ((row & 15) >> 2) + 4 * ((row >> 4) & 1) + (row & 3); }
 
 // [2 matrices][HC rows][KS units + one piece]: the odd number of pieces a row keeps 16 rows' equal pieces on different banks.
 template <typename T, int KS>
-__device__ __forceinline__ void stage_weights(char* lds, const T* wg, const T* wu, const T* bg, const T* bu, int k, int h, int h0, int hc) {
-  constexpr int PIECES = 4 * KS, ROW = PIECES * 16 + 16, E = Piece<T>::E;
+__device__ __forceinline__ void stage_weights(char* lds, const T* wg, const T* wu, int k, int h, int h0, int hc) {
+  constexpr int PIECES = 4 * KS, ROW = PIECES * 16 + 16;
   for (int e = threadIdx.x; e < 2 * hc * PIECES; e += blockDim.x) {
     const int row = e / PIECES, c = e - row * PIECES, m = row >= hc;
     const int f = h0 + image_feature(row - m * hc);
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (f < h) {
-      v = row_piece(((m ? wu : wg) + (int64_t)f * k), c, k);
-      if (bg && k / E == c) {  // the bias, behind the last weight
-        T t[E];
-        __builtin_memcpy(t, &v, 16);
-#pragma unroll
-        for (int i = 0; i < E; i++)
-          if (i == k % E) t[i] = (m ? bu : bg)[f];
-        __builtin_memcpy(&v, t, 16);
-      }
-    }
-    *reinterpret_cast<u32x4*>(lds + row * ROW + c * 16) = v;
+    *reinterpret_cast<u32x4*>(lds + row * ROW + c * 16) = f < h ? row_piece(((m ? wu : wg) + (int64_t)f * k), c, k) : u32x4{0u, 0u, 0u, 0u};
+  }
+}
+// the biases as f32, [2][hc] in the images' order (zeros without): where the accumulators start
+template <typename T>
+__device__ __forceinline__ void stage_bias(float* bias, const T* bg, const T* bu, int h, int h0, int hc) {
+  for (int e = threadIdx.x; e < 2 * hc; e += blockDim.x) {
+    const int m = e >= hc, f = h0 + image_feature(e - m * hc);
+    bias[e] = bg && f < h ? (float)(m ? bu : bg)[f] : 0.f;
   }
 }
 
+// workgroups of the forward that share a CU: registers for four, or for two where the rows are long
+constexpr int fwd_per_cu(int ks) { return ks <= 2 ? 4 : 2; }
+
 template <typename T, int KS, int G>
-__global__ __launch_bounds__(64 * kWaves) void gated_fwd_kernel(int64_t n_max, const int32_t* __restrict__ n_dev, const T* __restrict__ x, int64_t ldx,
+__global__ __launch_bounds__(64 * kWaves, fwd_per_cu(KS)) void gated_fwd_kernel(int64_t n_max, const int32_t* __restrict__ n_dev, const T* __restrict__ x, int64_t ldx,
                                                                const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg,
                                                                const T* __restrict__ bu, int k, int h, int hc, int act, T* __restrict__ out, int64_t ldo) {
   constexpr int ROW = KS * 64 + 16;
@@ -58,11 +72,8 @@ __global__ __launch_bounds__(64 * kWaves) void gated_fwd_kernel(int64_t n_max, c
   extern __shared__ __attribute__((aligned(16))) char lds[];
   float* bias = reinterpret_cast<float*>(lds + 2 * hc * ROW);  // [2][hc] in tile order
   const int h0 = blockIdx.y * hc;
-  stage_weights<T, KS>(lds, wg, wu, (const T*)nullptr, (const T*)nullptr, k, h, h0, hc);
-  for (int e = threadIdx.x; e < 2 * hc; e += blockDim.x) {
-    const int m = e >= hc, f = h0 + image_feature(e - m * hc);
-    bias[e] = bg && f < h ? (float)(m ? bu : bg)[f] : 0.f;
-  }
+  stage_weights<T, KS>(lds, wg, wu, k, h, h0, hc);
+  stage_bias(bias, bg, bu, h, h0, hc);
   __syncthreads();
   const int64_t n = gfn_live_n(n_max, n_dev);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, kg = lane >> 4;
@@ -70,21 +81,26 @@ __global__ __launch_bounds__(64 * kWaves) void gated_fwd_kernel(int64_t n_max, c
   const char* wrow = lds + j * ROW + kg * 16;
   const int64_t stride = (int64_t)gridDim.x * kWaves * 16 * G;
   int64_t s0 = ((int64_t)blockIdx.x * kWaves + wave) * 16 * G;
+  const int cut = cut_piece<T>(k);
   u32x4 xr[G][KS], next[G][KS];
   auto fetch = [&](u32x4 (&to)[G][KS], int64_t first) {
 #pragma unroll
     for (int g = 0; g < G; g++) {
       const int64_t s = first + 16 * g + j;
 #pragma unroll
-      for (int u = 0; u < KS; u++) to[g][u] = s < n ? row_piece(x + s * ldx, 4 * u + kg, k) : u32x4{0u, 0u, 0u, 0u};
+      for (int u = 0; u < KS; u++) to[g][u] = s < n ? piece_request(x + s * ldx, 4 * u + kg, k) : u32x4{0u, 0u, 0u, 0u};
     }
   };
   if (s0 < n) fetch(next, s0);
+  auto pass = [&](auto act_c) {
   for (; s0 < n; s0 += stride) {
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
-      for (int u = 0; u < KS; u++) xr[g][u] = next[g][u];
+      for (int u = 0; u < KS; u++) {
+        xr[g][u] = next[g][u];
+        if (u == cut >> 2 && kg == (cut & 3)) xr[g][u] = piece_shift<T>(next[g][u], k);
+      }
     if (s0 + stride < n) fetch(next, s0 + stride);  // on its way under this tile's work
     for (int p = 0; p < pairs; p++) {
       f32x4 acc[2][2][G];  // [matrix][tile]
@@ -111,11 +127,12 @@ __global__ __launch_bounds__(64 * kWaves) void gated_fwd_kernel(int64_t n_max, c
       for (int g = 0; g < G; g++) {
         const int64_t s = s0 + 16 * g + j;
         float v[8];
-        gated8<EXACT>(act, [&](int i) { return acc[0][i >> 2][g][i & 3]; }, [&](int i) { return acc[1][i >> 2][g][i & 3]; }, v);
+        gated8<decltype(act_c)::value, EXACT>([&](int i) { return acc[0][i >> 2][g][i & 3]; }, [&](int i) { return acc[1][i >> 2][g][i & 3]; }, v);
         if (s < n) store_row<T, 8>(out + s * ldo + f, h - f, v);
       }
     }
-  }
+  }  };
+  for_act(act, pass);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------------
@@ -130,6 +147,22 @@ __device__ __forceinline__ int tile_scale_exponent(float largest, int before) {
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23); }
 
+// use(i, load(i)) for i = 0 .. N - 1 with the loads AHEAD of their use, in this order: a read from LDS passes under the products of the
+// ones before it (left to itself, and short of registers, the compiler reads right before each use and waits every time).
+template <int N, int AHEAD, typename L, typename U>
+__device__ __forceinline__ void read_ahead(L load, U use) {
+  u32x4 v[AHEAD + 1];
+#pragma unroll
+  for (int i = 0; i < (AHEAD < N ? AHEAD : N); i++) v[i] = load(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    if (i + AHEAD < N) v[(i + AHEAD) % (AHEAD + 1)] = load(i + AHEAD);
+    use(i, v[i % (AHEAD + 1)]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // four rows r0 .. r0 + 3 (one for each lane quarter of a 16-lane group) x 16 columns come back column-major: lane i gets column
 // (i & 3) of the 8-byte piece lane 4 q + (i >> 2) points at, rows q = 0 .. 3.
 __device__ __forceinline__ u32x2 tr4(const char* a) {
@@ -137,7 +170,7 @@ __device__ __forceinline__ u32x2 tr4(const char* a) {
 }
 
 // waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit
-constexpr int bwd_waves(int ks) { return ks >= 3 && ks <= 5 ? 8 : 4; }
+constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 
 struct GatedBwd {
   int64_t n_max;
@@ -149,60 +182,57 @@ struct GatedBwd {
   float* dx_sum;      // f32 [n_max][k] between the launches of several feature blocks, or null
   int dx_first, dx_last;
   int z_buffers;      // 1 or 2 tiles of dz in LDS
-  float* part;        // [workgroup][64 NP][KP] f32, or null
+  float* part;        // [workgroup][64 NP][kp] f32, or null: column k is the bias's
+  int kp;
 };
 
 template <typename T, int KS, int NP>
 __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_kernel(GatedBwd a) {
   constexpr int WAVES = bwd_waves(KS);
   constexpr int E = Piece<T>::E, TPU = sizeof(T) == 4 ? 1 : 2;  // 16-column tiles a unit
-  constexpr int KP = KS * 4 * E, KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP;
+  constexpr int KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP;
   constexpr int SAMPLES = 16 * WAVES, ZROW = 64 * (int)sizeof(T) + 16;
   constexpr int FT_WAVES = WAVES / 4, KT_WAVE = (KT + FT_WAVES - 1) / FT_WAVES;  // waves that share a row tile of dW, its column tiles a wave
   constexpr bool EXACT = sizeof(T) == 4, SCALED = sizeof(T) == 2 && !__is_same(T, __bf16);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* xs = lds + 2 * HB * ROW;        // [SAMPLES][ROW]
   char* zs = xs + SAMPLES * ROW;        // [z_buffers][SAMPLES][dg 32 | du 32]
-  float* top = reinterpret_cast<float*>(zs + a.z_buffers * SAMPLES * ZROW);  // [WAVES]
+  float* bias = reinterpret_cast<float*>(zs + a.z_buffers * SAMPLES * ZROW);  // [2][HB]
+  float* top = bias + 2 * HB;                                                 // [WAVES]
   const T *x = static_cast<const T*>(a.x), *dh = static_cast<const T*>(a.dh);
-  const bool ones = a.bg != nullptr;
+  const bool biased = a.bg != nullptr;
   const int k = a.k, h = a.h, h0 = a.h0, act = a.act;
-  stage_weights<T, KS>(lds, static_cast<const T*>(a.wg), static_cast<const T*>(a.wu), static_cast<const T*>(a.bg), static_cast<const T*>(a.bu), k, h, h0, HB);
+  stage_weights<T, KS>(lds, static_cast<const T*>(a.wg), static_cast<const T*>(a.wu), k, h, h0, HB);
+  stage_bias(bias, static_cast<const T*>(a.bg), static_cast<const T*>(a.bu), h, h0, HB);
   const int64_t n = gfn_live_n(a.n_max, a.n_dev);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, kg = lane >> 4;
   const int ft = wave & 3, kt0 = (wave >> 2) * KT_WAVE;
-  f32x4 dw[NP][KT_WAVE];
+  f32x4 dw[NP][KT_WAVE], db = {0.f, 0.f, 0.f, 0.f};  // db: the sums of dz itself, pair p's in column p
 #pragma unroll
-  for (int p = 0; p < NP; p++)
+  for (int p = 0; p < NP; p++) {
 #pragma unroll
     for (int t = 0; t < KT_WAVE; t++) dw[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const bool sums = biased && wave < 4;  // one wave for each row tile
   int run_e = 0;  // dw holds the sums times 2^run_e
   const char* wrow = lds + j * ROW + kg * 16;
   const int64_t tiles = (n + SAMPLES - 1) / SAMPLES;
   constexpr int DP = 8 / E;  // pieces of eight features
   const int width = h - h0 < HB ? h - h0 : HB;
-  constexpr bool AHEAD = KS < 4;  // dh of the next tile is requested with its x where registers are left for it
-  u32x4 xr[KS], xn[KS], dr[NP][DP], dn[AHEAD ? NP : 1][DP];
+  const int cut = cut_piece<T>(k), dh_cut = cut_piece<T>(width);
+  constexpr int IN_FLIGHT = 3;  // reads from LDS ahead of the products
+  constexpr bool AHEAD = KS < 4;  // the next tile's x and dh are requested under this one's work, where registers are left for them
+  u32x4 xr[KS], xn[AHEAD ? KS : 1], dr[NP][DP], dn[AHEAD ? NP : 1][DP];
+  auto fetch_x = [&](int64_t s, u32x4& to, int u) { to = s < n ? piece_request(x + s * a.ldx, 4 * u + kg, k) : u32x4{0u, 0u, 0u, 0u}; };
   auto fetch_dh = [&](int64_t s, u32x4 (&to)[DP], int p) {
 #pragma unroll
-    for (int q = 0; q < DP; q++) to[q] = s < n ? row_piece(dh + s * a.lddh + h0, (32 * p + 8 * kg) / E + q, width) : u32x4{0u, 0u, 0u, 0u};
+    for (int q = 0; q < DP; q++) to[q] = s < n ? piece_request(dh + s * a.lddh + h0, (32 * p + 8 * kg) / E + q, width) : u32x4{0u, 0u, 0u, 0u};
   };
   auto fetch = [&](int64_t tile) {
-    const int64_t s = tile * SAMPLES + wave * 16 + j;
-#pragma unroll
-    for (int u = 0; u < KS; u++) {
-      const int c = 4 * u + kg;
-      xn[u] = s < n ? row_piece(x + s * a.ldx, c, k) : u32x4{0u, 0u, 0u, 0u};
-      if (ones && s < n && k / E == c) {
-        T t[E];
-        __builtin_memcpy(t, &xn[u], 16);
-#pragma unroll
-        for (int i = 0; i < E; i++)
-          if (i == k % E) t[i] = (T)1.f;
-        __builtin_memcpy(&xn[u], t, 16);
-      }
-    }
     if constexpr (AHEAD) {
+      const int64_t s = tile * SAMPLES + wave * 16 + j;
+#pragma unroll
+      for (int u = 0; u < KS; u++) fetch_x(s, xn[u], u);
 #pragma unroll
       for (int p = 0; p < NP; p++) fetch_dh(s, dn[p], p);
     }
@@ -211,7 +241,10 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int64_t s = tile * SAMPLES + wave * 16 + j;
 #pragma unroll
-    for (int u = 0; u < KS; u++) xr[u] = xn[u];
+    for (int u = 0; u < KS; u++) {
+      if constexpr (AHEAD) xr[u] = xn[u];
+      else fetch_x(s, xr[u], u);
+    }
 #pragma unroll
     for (int p = 0; p < NP; p++) {
       if constexpr (AHEAD) {
@@ -221,6 +254,14 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         fetch_dh(s, dr[p], p);
       }
     }
+#pragma unroll
+    for (int u = 0; u < KS; u++)
+      if (u == cut >> 2 && kg == (cut & 3)) xr[u] = piece_shift<T>(xr[u], k);
+#pragma unroll
+    for (int p = 0; p < NP; p++)
+#pragma unroll
+      for (int q = 0; q < DP; q++)
+        if (p == dh_cut >> (DP + 1) && DP * kg + q == (dh_cut & (4 * DP - 1))) dr[p][q] = piece_shift<T>(dr[p][q], width);
     __syncthreads();  // the weights are staged (first tile); the tile before has been read from xs, zs and top
 #pragma unroll
     for (int u = 0; u < KS; u++) *reinterpret_cast<u32x4*>(xs + (wave * 16 + j) * ROW + u * 64 + kg * 16) = xr[u];
@@ -253,6 +294,7 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         for (int p = 0; p < NP; p++)
 #pragma unroll
           for (int t = 0; t < KT_WAVE; t++) dw[p][t] *= by;
+        db *= by;
         run_e = e;
       }
     }
@@ -265,33 +307,27 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int t = 0; t < 2; t++) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < KS; u++)
-#pragma unroll
-        for (int m = 0; m < 2; m++)
-#pragma unroll
-          for (int t = 0; t < 2; t++)
-            acc[m][t] = mma(*reinterpret_cast<const u32x4*>(wrow + (m * HB + 32 * p + 16 * t) * ROW + u * 64), xr[u], acc[m][t], (T*)nullptr);
+        for (int t = 0; t < 2; t++) acc[m][t] = *reinterpret_cast<const f32x4*>(bias + m * HB + 32 * p + 16 * t + 4 * kg);
+      read_ahead<4 * KS, IN_FLIGHT>(
+          [&](int i) { return *reinterpret_cast<const u32x4*>(wrow + (((i >> 1) & 1) * HB + 32 * p + 16 * (i & 1)) * ROW + (i >> 2) * 64); },
+          [&](int i, const u32x4& w) { acc[(i >> 1) & 1][i & 1] = mma(w, xr[i >> 2], acc[(i >> 1) & 1][i & 1], (T*)nullptr); });
       T z[2][8];
       float d[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) d[i] = SCALED ? grad(p, i) * to : grad(p, i);
-      gated8_grad<EXACT>(act, [&](int i) { return acc[0][i >> 2][i & 3]; }, [&](int i) { return acc[1][i >> 2][i & 3]; }, d, z[0], z[1]);
+      for_act(act, [&](auto act_c) { gated8_grad<decltype(act_c)::value, EXACT>([&](int i) { return acc[0][i >> 2][i & 3]; }, [&](int i) { return acc[1][i >> 2][i & 3]; }, d, z[0], z[1]); });
       if (a.dx || a.dx_sum) {  // dx[k] += sum over these 32 features
         if constexpr (sizeof(T) == 2) {
-#pragma unroll
-          for (int m = 0; m < 2; m++) {
-            const u32x4 b = __builtin_bit_cast(u32x4, z[m]);
-            // features 8 kg .. + 3 are image rows 4 kg .. + 3 of tile 0, the next four those of tile 1
-            const char* r = lds + (m * HB + 32 * p + 4 * kg + (j >> 2)) * ROW;
-#pragma unroll
-            for (int t = 0; t < KT; t++) {
-              const char* q = r + (32 * (t >> 1) + 8 * (j & 3) + 4 * (t & 1)) * 2;
-              const u32x2 lo = tr4(q), hi = tr4(q + 16 * ROW);
-              dx[t] = mma(u32x4{lo[0], lo[1], hi[0], hi[1]}, b, dx[t], (T*)nullptr);
-            }
-          }
+          // features 8 kg .. + 3 are image rows 4 kg .. + 3 of tile 0, the next four those of tile 1
+          const char* r = lds + (32 * p + 4 * kg + (j >> 2)) * ROW + 8 * (j & 3);
+          const u32x4 b[2] = {__builtin_bit_cast(u32x4, z[0]), __builtin_bit_cast(u32x4, z[1])};
+          read_ahead<2 * KT, IN_FLIGHT>(
+              [&](int i) {
+                const char* q = r + (i / KT) * HB * ROW + 32 * (i % KT);
+                const u32x2 lo = tr4(q), hi = tr4(q + 16 * ROW);
+                return u32x4{lo[0], lo[1], hi[0], hi[1]};
+              },
+              [&](int i, const u32x4& w) { dx[i % KT] = mma(w, b[i / KT], dx[i % KT], (T*)nullptr); });
         } else {
 #pragma unroll
           for (int m = 0; m < 2; m++)
@@ -311,52 +347,62 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         __builtin_memcpy(__builtin_assume_aligned(zr, 16), z[0], sizeof(z[0]));
         __builtin_memcpy(__builtin_assume_aligned(zr + 32 * sizeof(T), 16), z[1], sizeof(z[1]));
         __syncthreads();
+        f32x4 total = {0.f, 0.f, 0.f, 0.f};  // dz summed over the samples, the same in every column
         if constexpr (sizeof(T) == 2) {
-#pragma unroll
-          for (int c = 0; c < SAMPLES; c += 32) {  // rows 8 kg .. 8 kg + 7 of these 32 samples
-            const char* r = zb + (c + 8 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
-            const u32x2 l = tr4(r), u = tr4(r + 4 * ZROW);
-            const u32x4 av = {l[0], l[1], u[0], u[1]};
-            const char* q = xs + (c + 8 * kg + (j >> 2)) * ROW + 4 * (j & 3) * 2;
-#pragma unroll
-            for (int t = 0; t < KT_WAVE; t++)
-              if (KT % FT_WAVES == 0 || kt0 + t < KT) {
-                const u32x2 lo = tr4(q + 32 * (kt0 + t)), hi = tr4(q + 32 * (kt0 + t) + 4 * ROW);
-                dw[p][t] = mma(av, u32x4{lo[0], lo[1], hi[0], hi[1]}, dw[p][t], (T*)nullptr);
-              }
-          }
+          // 32 samples at a time, in the order 4 kg .. + 3, 16 + 4 kg .. + 3: a read covers 16 rows, on different banks
+          const char* r = zb + (4 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
+          const char* q = xs + (4 * kg + (j >> 2)) * ROW + 8 * (j & 3) + 32 * kt0;
+          constexpr uint32_t one = __is_same(T, __bf16) ? 0x3f803f80u : 0x3c003c00u;
+          u32x4 av[2];
+          read_ahead<SAMPLES / 32 * KT_WAVE, IN_FLIGHT>(
+              [&](int i) {
+                const int c = i / KT_WAVE, t = i % KT_WAVE;
+                if (t == 0) {
+                  const u32x2 l = tr4(r + 32 * c * ZROW), u = tr4(r + (32 * c + 16) * ZROW);
+                  av[c & 1] = u32x4{l[0], l[1], u[0], u[1]};
+                }
+                const u32x2 lo = tr4(q + 32 * c * ROW + 32 * t), hi = tr4(q + (32 * c + 16) * ROW + 32 * t);
+                return u32x4{lo[0], lo[1], hi[0], hi[1]};
+              },
+              [&](int i, const u32x4& b) {
+                const u32x4& a4 = av[i / KT_WAVE & 1];
+                if (i % KT_WAVE == 0) total = mma(a4, u32x4{one, one, one, one}, total, (T*)nullptr);
+                dw[p][i % KT_WAVE] = mma(a4, b, dw[p][i % KT_WAVE], (T*)nullptr);
+              });
         } else {
 #pragma unroll 4
           for (int c = 0; c < SAMPLES; c += 4) {
             const float av = *reinterpret_cast<const float*>(zb + (c + kg) * ZROW + (16 * ft + j) * 4);
             const char* q = xs + (c + kg) * ROW + j * 4;
+            total = __builtin_amdgcn_mfma_f32_16x16x4f32(av, 1.f, total, 0, 0, 0);
 #pragma unroll
             for (int t = 0; t < KT_WAVE; t++)
               if (KT % FT_WAVES == 0 || kt0 + t < KT)
                 dw[p][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av, *reinterpret_cast<const float*>(q + 64 * (kt0 + t)), dw[p][t], 0, 0, 0);
           }
         }
+#pragma unroll
+        for (int r = 0; r < 4; r++) db[r] = j == p ? db[r] + total[r] : db[r];
       }
     }
-    if ((a.dx || a.dx_sum) && s < n) {  // lane (j, kg) holds columns 16 t' + 4 kg + r of sample j; two 16-bit tiles a unit: 32 u + 8 kg + 4 t + r
+    if ((a.dx || a.dx_sum) && s < n) {  // lane (j, kg) holds columns 16 t + 4 kg + r of sample j
 #pragma unroll
-      for (int u = 0; u < KS; u++) {
-        constexpr int W = 4 * TPU;
-        const int col = KP / KS * u + W * kg;
-        float v[W];
+      for (int t = 0; t < KT; t++) {
+        const int col = 16 * t + 4 * kg;
+        float v[4];
 #pragma unroll
-        for (int i = 0; i < W; i++) v[i] = dx[TPU * u + (i >> 2)][i & 3] * back;
+        for (int i = 0; i < 4; i++) v[i] = dx[t][i] * back;
         if (col < k) {
           if (!a.dx_first) {
 #pragma unroll
-            for (int i = 0; i < W; i++)
+            for (int i = 0; i < 4; i++)
               if (col + i < k) v[i] += a.dx_sum[s * k + col + i];
           }
           if (a.dx_last) {
-            store_row<T, W>(static_cast<T*>(a.dx) + s * a.lddx + col, k - col, v);
+            store_row<T, 4>(static_cast<T*>(a.dx) + s * a.lddx + col, k - col, v);
           } else {
 #pragma unroll
-            for (int i = 0; i < W; i++)
+            for (int i = 0; i < 4; i++)
               if (col + i < k) a.dx_sum[s * k + col + i] = v[i];
           }
         }
@@ -365,14 +411,20 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
   }
   if (a.part) {
     const float back = pow2(-run_e);
-    float* o = a.part + (int64_t)blockIdx.x * (64 * NP * KP);
+    const int kp = a.kp;
+    float* o = a.part + (int64_t)blockIdx.x * (64 * NP * kp);
 #pragma unroll
     for (int p = 0; p < NP; p++)
 #pragma unroll
-      for (int t = 0; t < KT_WAVE; t++)
-        if (KT % FT_WAVES == 0 || kt0 + t < KT)
+      for (int t = 0; t < KT_WAVE; t++) {
+        const int col = 16 * (kt0 + t) + j;
+        if (col < k)
 #pragma unroll
-          for (int r = 0; r < 4; r++) o[(64 * p + 16 * ft + 4 * kg + r) * KP + 16 * (kt0 + t) + j] = dw[p][t][r] * back;
+          for (int r = 0; r < 4; r++) o[(64 * p + 16 * ft + 4 * kg + r) * kp + col] = dw[p][t][r] * back;
+      }
+    if (sums && j < NP)
+#pragma unroll
+      for (int r = 0; r < 4; r++) o[(64 * j + 16 * ft + 4 * kg + r) * kp + k] = db[r] * back;
   }
 }
 
@@ -458,7 +510,7 @@ int dispatch_fwd(const GatedFwd& a, hipStream_t st) {
   GFN_GATED(2, 2);
   if constexpr (sizeof(T) == 4) {
     GFN_GATED(4, 2);
-    GFN_GATED(8, 2);
+    GFN_GATED(8, 1);
   } else {
     GFN_GATED(3, 2);
     GFN_GATED(4, 2);
@@ -467,9 +519,9 @@ int dispatch_fwd(const GatedFwd& a, hipStream_t st) {
   return GFN_ERR_ARG;
 }
 
-// The backward's plan for (n, k + bias, h, type): units a row, feature blocks of 32 NP, waves and workgroups.
+// The backward's plan for (n, k, h, type): units a row, feature blocks of 32 NP, waves and workgroups.
 struct BwdPlan {
-  int ks, np, waves, blocks, launches, z_buffers;
+  int ks, np, waves, blocks, launches, z_buffers, kp;
   size_t lds, part_floats;
   bool dx_sum;
 };
@@ -477,25 +529,24 @@ struct BwdPlan {
 BwdPlan plan_bwd(int64_t n, int k, int h, int dtype, bool bias) {
   BwdPlan p;
   const int e = dtype == GFN_F32 ? 4 : 8, size = dtype == GFN_F32 ? 4 : 2;
-  const int units = (k + (bias ? 1 : 0) + 4 * e - 1) / (4 * e);
-  p.ks = units;
-  if (dtype == GFN_F32 && units > 5) p.ks = 9;
+  p.ks = (k + 4 * e - 1) / (4 * e);
+  if (p.ks > 4) p.ks = 8;  // f32 only
   p.waves = bwd_waves(p.ks);
+  p.kp = (k + (bias ? 1 : 0) + 15) & ~15;
   const int most = p.ks > 4 ? 2 : 4;  // 32-feature pairs a launch: the weights and dW's accumulators fit
   const int pairs = (h + 31) / 32;
   p.np = pairs >= 3 && most == 4 ? 4 : pairs >= 2 ? 2 : 1;
   p.launches = (pairs + p.np - 1) / p.np;
   const int row = p.ks * 64 + 16, samples = 16 * p.waves;
   const size_t z = (size_t)samples * (64 * size + 16);
-  p.lds = (size_t)64 * p.np * row + (size_t)samples * row + z + 64;
+  p.lds = (size_t)64 * p.np * (row + 4) + (size_t)samples * row + z + 32;
   // a second buffer for dz (one barrier a pair of tiles instead of two) where it does not cost the CU its second workgroup
   p.z_buffers = p.np > 1 && (p.lds + z <= 80 * 1024 || (p.lds > 80 * 1024 && p.lds + z <= 160 * 1024)) ? 2 : 1;
   p.lds += (p.z_buffers - 1) * z;
   const int64_t tiles = (n + samples - 1) / samples;
   const int at_once = 256 * (p.lds <= 80 * 1024 ? 2 : 1);
-  p.blocks = (int)(tiles < at_once ? tiles : at_once);
-  if (p.blocks < 1) p.blocks = 1;
-  p.part_floats = (size_t)p.blocks * 64 * p.np * (p.ks * 4 * e);
+  p.blocks = tiles < 1 ? 1 : (int)(tiles < at_once ? tiles : at_once);
+  p.part_floats = (size_t)p.blocks * 64 * p.np * p.kp;
   p.dx_sum = p.launches > 1;
   return p;
 }
@@ -522,11 +573,9 @@ int dispatch_bwd(const GatedBwd& a, const BwdPlan& p, hipStream_t st) {
   GFN_GATED(2);
   GFN_GATED(3);
   GFN_GATED(4);
-  GFN_GATED_NP(5, 1);
-  GFN_GATED_NP(5, 2);
   if constexpr (sizeof(T) == 4) {
-    GFN_GATED_NP(9, 1);
-    GFN_GATED_NP(9, 2);
+    GFN_GATED_NP(8, 1);
+    GFN_GATED_NP(8, 2);
   }
 #undef GFN_GATED
 #undef GFN_GATED_NP
@@ -535,7 +584,7 @@ int dispatch_bwd(const GatedBwd& a, const BwdPlan& p, hipStream_t st) {
 }
 
 template <typename T>
-int gated_bwd_typed(GatedBwd a, const BwdPlan& p, int kp, void* dwg, void* dwu, void* dbg, void* dbu, hipStream_t st) {
+int gated_bwd_typed(GatedBwd a, const BwdPlan& p, void* dwg, void* dwu, void* dbg, void* dbu, hipStream_t st) {
   const int cols = a.k + (a.bg ? 1 : 0);
   for (int l = 0; l < p.launches; l++) {
     a.h0 = l * 32 * p.np;
@@ -544,7 +593,7 @@ int gated_bwd_typed(GatedBwd a, const BwdPlan& p, int kp, void* dwg, void* dwu, 
     if (int rc = dispatch_bwd<T>(a, p, st)) return rc;
     if (a.part) {
       gated_reduce_kernel<T><<<dim3((unsigned)((cols + 31) / 32), (unsigned)(64 * p.np)), 1024, 0, st>>>(
-          a.part, p.blocks, 64 * p.np, kp, a.k, a.h, a.h0, cols, static_cast<T*>(dwg), static_cast<T*>(dwu), static_cast<T*>(dbg), static_cast<T*>(dbu));
+          a.part, p.blocks, 64 * p.np, p.kp, a.k, a.h, a.h0, cols, static_cast<T*>(dwg), static_cast<T*>(dwu), static_cast<T*>(dbg), static_cast<T*>(dbu));
       GFN_CHECK_LAUNCH();
     }
   }
@@ -598,6 +647,7 @@ int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, co
   a.k = in_dim; a.h = hidden; a.act = act;
   a.dx = dx;
   a.z_buffers = p.z_buffers;
+  a.kp = p.kp;
   float* ws = static_cast<float*>(workspace);
   if (dwg) {
     a.part = ws;
@@ -605,10 +655,9 @@ int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, co
   }
   if (dx && p.dx_sum) a.dx_sum = ws;
   hipStream_t st = gfn_stream(stream);
-  const int kp = p.ks * 4 * (dtype == GFN_F32 ? 4 : 8);
-  if (dtype == GFN_F32) return gated_bwd_typed<float>(a, p, kp, dwg, dwu, dbg, dbu, st);
-  if (dtype == GFN_BF16) return gated_bwd_typed<__bf16>(a, p, kp, dwg, dwu, dbg, dbu, st);
-  return gated_bwd_typed<_Float16>(a, p, kp, dwg, dwu, dbg, dbu, st);
+  if (dtype == GFN_F32) return gated_bwd_typed<float>(a, p, dwg, dwu, dbg, dbu, st);
+  if (dtype == GFN_BF16) return gated_bwd_typed<__bf16>(a, p, dwg, dwu, dbg, dbu, st);
+  return gated_bwd_typed<_Float16>(a, p, dwg, dwu, dbg, dbu, st);
 }
 
 }  // extern "C"

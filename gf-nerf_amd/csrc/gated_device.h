@@ -42,33 +42,48 @@ __device__ __forceinline__ u32x4 load16(const void* p) {  // rows of odd width s
   return v;
 }
 
-// Piece c (elements c E .. c E + E - 1) of a row of `k` elements, zeros behind its end; nothing outside the row is read.  The piece
-// that the row's end cuts is read as the row's last 16 bytes and shifted down (`k` is the same for every lane: a scalar shift).
+// Piece c (elements c E .. c E + E - 1) of a row of `k` elements, zeros behind its end; nothing outside the row is read.  In two steps,
+// so that a piece can be requested long before it is looked at: the piece that the row's end cuts is REQUESTED as the row's last 16
+// bytes, and CUT (shifted down by what it holds too early: the same shift in every lane) where it is used.
 template <typename T>
-__device__ __forceinline__ u32x4 row_piece(const T* row, int c, int k) {
+__device__ __forceinline__ u32x4 piece_request(const T* row, int c, int k) {
   constexpr int E = Piece<T>::E;
-  const int left = k - c * E;
   u32x4 v = {0u, 0u, 0u, 0u};
-  if (left >= E) return load16(row + c * E);
-  if (left <= 0) return v;
-  if (k >= E) {
-    const u32x4 w = load16(row + k - E);
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < 3; i++)  // element i of the piece = element i + E - left of the row's last E
-        v[i] = i < left ? (left == 3 ? w[i + 1] : left == 2 ? w[(i + 2) & 3] : w[3]) : 0u;
-    } else {
-      typedef unsigned __int128 u128;
-      const u128 s = __builtin_bit_cast(u128, w) >> (16 * (E - left));
-      v = __builtin_bit_cast(u32x4, s);
-    }
-    return v;
-  }
+  if (c * E >= k) return v;
+  if (k >= E) return load16(row + (c * E + E <= k ? c * E : k - E));
   T e[E];
 #pragma unroll
-  for (int i = 0; i < E; i++) e[i] = i < left ? row[c * E + i] : (T)0.f;
+  for (int i = 0; i < E; i++) e[i] = i < k ? row[i] : (T)0.f;
   __builtin_memcpy(&v, e, 16);
   return v;
+}
+// the piece that the end of a row of `k` elements cuts, or -1; the same in every lane
+template <typename T>
+__device__ __forceinline__ int cut_piece(int k) {
+  constexpr int E = Piece<T>::E;
+  return k > E && k % E ? k / E : -1;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 piece_shift(u32x4 w, int k) {
+  constexpr int E = Piece<T>::E;
+  const int left = k % E;
+  u32x4 v;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 3; i++)  // element i of the piece = element i + E - left of the row's last E
+      v[i] = i < left ? (left == 3 ? w[i + 1] : left == 2 ? w[(i + 2) & 3] : w[3]) : 0u;
+    v[3] = 0u;
+  } else {
+    typedef unsigned __int128 u128;
+    const u128 s = __builtin_bit_cast(u128, w) >> (16 * (E - left));
+    v = __builtin_bit_cast(u32x4, s);
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 row_piece(const T* row, int c, int k) {
+  const u32x4 w = piece_request(row, c, k);
+  return c == cut_piece<T>(k) ? piece_shift<T>(w, k) : w;
 }
 
 template <typename T, int N>
@@ -78,6 +93,7 @@ __device__ __forceinline__ void store_row(T* p, int left, const float (&v)[N]) {
 #pragma unroll
   for (int i = 0; i < N; i++) e[i] = (T)v[i];
   if (left >= N) {
+    if constexpr (sizeof(Row) == 8) __builtin_memcpy(p, &e, 8);
 #pragma unroll
     for (int c = 0; c < (int)sizeof(Row) / 16; c++) {
       using Rows = __attribute__((ext_vector_type(sizeof(Row) / 4))) uint32_t;
@@ -105,40 +121,43 @@ __device__ __forceinline__ float sigmoid(float z) {
   return t > 126.f ? 0.f : (t < -126.f ? 1.f : s);  // where exp2 over- or underflows the two steps would meet inf - inf
 }
 
-// Phi(z) = erfc(-z / sqrt 2) / 2, and gauss = exp(-z^2 / 2), which its derivative needs as well.  EXACT (f32): the Chebyshev fit of Press et al.
-// (Numerical Recipes, erfcc), 1.2e-7 of the value everywhere, the tail of z -> -inf included.  Else Abramowitz & Stegun 7.1.26, 1.5e-7 absolute.
+// Phi(z) = erfc(-z / sqrt 2) / 2, and gauss = exp(-z^2 / 2), which its derivative needs as well.  With x = |z| / sqrt 2 and
+// t = 1 / (1 + c x), erfc(x) = t exp(-x^2) P(t): exp(x^2) erfc(x) / t is smooth on (0, 1] and P is its least-largest-relative-error
+// polynomial, fitted to 64-bit values.  EXACT (f32): degree 8, c = 0.4, 1.3e-7 of the tail, and 2.2e-7 with the rounding of its sums;
+// else degree 7, c = 0.46, 7.6e-7.
 template <bool EXACT>
 __device__ __forceinline__ float normal_cdf(float z, float& gauss) {
   gauss = __builtin_amdgcn_exp2f(-0.72134752044448170368f * z * z);  // -z^2 / 2 / ln 2
   const float x = 0.70710678118654752440f * __builtin_fabsf(z);
-  float tail;
+  float t, p;
   if constexpr (EXACT) {
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, x, 1.f));
-    float p = __builtin_fmaf(0.17087277f, t, -0.82215223f);
-    p = __builtin_fmaf(p, t, 1.48851587f);
-    p = __builtin_fmaf(p, t, -1.13520398f);
-    p = __builtin_fmaf(p, t, 0.27886807f);
-    p = __builtin_fmaf(p, t, -0.18628806f);
-    p = __builtin_fmaf(p, t, 0.09678418f);
-    p = __builtin_fmaf(p, t, 0.37409196f);
-    p = __builtin_fmaf(p, t, 1.00002368f);
-    p = __builtin_fmaf(p, t, -1.26551223f);
-    tail = 0.5f * t * gauss * __builtin_amdgcn_exp2f(p * 1.44269504088896340736f);
+    t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.4f, x, 1.f));
+    p = __builtin_fmaf(0.0502589586f, t, -0.182889897f);
+    p = __builtin_fmaf(p, t, 0.169068453f);
+    p = __builtin_fmaf(p, t, -0.00559473326f);
+    p = __builtin_fmaf(p, t, 0.141426169f);
+    p = __builtin_fmaf(p, t, 0.168543132f);
+    p = __builtin_fmaf(p, t, 0.207842577f);
+    p = __builtin_fmaf(p, t, 0.225669603f);
+    p = __builtin_fmaf(p, t, 0.225675862f);
   } else {
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
-    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    p = __builtin_fmaf(p, t, 1.421413741f);
-    p = __builtin_fmaf(p, t, -0.284496736f);
-    p = __builtin_fmaf(p, t, 0.254829592f);
-    tail = 0.5f * p * t * gauss;
+    t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.46f, x, 1.f));
+    p = __builtin_fmaf(0.0677144445f, t, -0.226629622f);
+    p = __builtin_fmaf(p, t, 0.16919146f);
+    p = __builtin_fmaf(p, t, 0.0526103041f);
+    p = __builtin_fmaf(p, t, 0.186847901f);
+    p = __builtin_fmaf(p, t, 0.231181864f);
+    p = __builtin_fmaf(p, t, 0.259557267f);
+    p = __builtin_fmaf(p, t, 0.259527059f);
   }
+  const float tail = 0.5f * p * t * gauss;
   return z < 0.f ? tail : 1.f - tail;
 }
 
-// v[i] = act(g[i]) u[i] for eight values: the choice of act is the same for every lane, taken once.  A NaN stays one.
-template <bool EXACT, typename F, typename U>
-__device__ __forceinline__ void gated8(int act, F g, U u, float (&v)[8]) {
-  switch (act) {
+// v[i] = act(g[i]) u[i] for eight values.  A NaN stays one.
+template <int ACT, bool EXACT, typename F, typename U>
+__device__ __forceinline__ void gated8(F g, U u, float (&v)[8]) {
+  switch (ACT) {
     case GATED_SILU:
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] = g(i) * sigmoid<EXACT>(g(i)) * u(i);
@@ -160,9 +179,9 @@ __device__ __forceinline__ void gated8(int act, F g, U u, float (&v)[8]) {
   }
 }
 // dg[i] = d[i] u[i] act'(g[i]), du[i] = d[i] act(g[i])
-template <bool EXACT, typename F, typename U, typename T>
-__device__ __forceinline__ void gated8_grad(int act, F g, U u, const float (&d)[8], T (&dg)[8], T (&du)[8]) {
-  switch (act) {
+template <int ACT, bool EXACT, typename F, typename U, typename T>
+__device__ __forceinline__ void gated8_grad(F g, U u, const float (&d)[8], T (&dg)[8], T (&du)[8]) {
+  switch (ACT) {
     case GATED_SILU:
 #pragma unroll
       for (int i = 0; i < 8; i++) {

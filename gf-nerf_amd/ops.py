@@ -1395,67 +1395,79 @@ SCAN_GATE = {"linear": 0, "sigmoid": 1, "decay": 2}
 SCAN_BLOCK = 8  # GFN_SCAN_BLOCK: rows a saved state covers
 
 
-def _place(tensors):
-    """Every tensor on the current device (the launch goes to the current stream of the current device)."""
+# The smallest of these calls are bound by what the host does for them (a kernel of 4 us behind 8 to 10 us of checks, allocation and
+# launch), so a good argument is recognised with few attribute reads; what is wrong with a bad one is found out afterwards.
+def _place(*tensors):
+    """Every tensor on the current device (the launch goes to its current stream) -> that stream."""
     here = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != here:
+        if t is not None and t.get_device() != here:
             raise _lib.GfnError(f"a tensor on {t.device} in a call on device {here}: make it current (torch.cuda.device) first")
+    return _raw_stream(here) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t, name, dtype=None, width=None, n=None):
-    """A 2-D tensor whose rows are contiguous, any row stride that keeps them apart -> its row stride in elements."""
+    """A 2-D tensor whose rows are contiguous, any row stride that keeps them apart -> (rows, columns, row stride in elements)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise _lib.GfnError(f"{name}: expected a CUDA(HIP) tensor")
-    if t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype):
-        raise _lib.GfnError(f"{name}: expected dtype {'float32, bfloat16 or float16' if dtype is None else dtype}, got {t.dtype}")
-    if t.dim() != 2 or (width is not None and t.shape[1] != width) or (n is not None and t.shape[0] != n):
-        raise _lib.GfnError(f"{name}: expected shape [{'n' if n is None else n}, {'columns' if width is None else width}], got {tuple(t.shape)}")
-    if t.shape[0] > 1 and (t.stride(0) < t.shape[1]) or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise _lib.GfnError(f"{name}: rows must be contiguous and apart, got strides {t.stride()} for shape {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    have = t.dtype
+    if have not in DTYPES or (dtype is not None and have != dtype):
+        raise _lib.GfnError(f"{name}: expected dtype {'float32, bfloat16 or float16' if dtype is None else dtype}, got {have}")
+    shape = t.shape
+    if len(shape) != 2 or (width is not None and shape[1] != width) or (n is not None and shape[0] != n):
+        raise _lib.GfnError(f"{name}: expected shape [{'n' if n is None else n}, {'columns' if width is None else width}], got {tuple(shape)}")
+    rows, columns = shape
+    ld, step = t.stride()
+    if rows > 1 and ld < columns or (columns > 1 and step != 1):
+        raise _lib.GfnError(f"{name}: rows must be contiguous and apart, got strides {t.stride()} for shape {tuple(shape)}")
+    return rows, columns, ld if rows > 1 else max(columns, 1)
 
 
 def _flat(t, dtype, name, shape):
     """A contiguous tensor (or None) of exactly this dtype and shape."""
+    if t is None or (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.shape == shape and t.is_contiguous()):
+        return
     _chk(t, dtype, name)
-    if t is not None and tuple(t.shape) != tuple(shape):
-        raise _lib.GfnError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise _lib.GfnError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _apart(out, *inputs):
-    """The output is not one of the inputs (rows are read by other workgroups while it is written)."""
-    for t in inputs:
-        if t is not None and out.numel() and t.data_ptr() == out.data_ptr():
-            raise _lib.GfnError("out is one of the inputs")
+    """The output is not one of the inputs (rows are read by other workgroups while it is written): their addresses -> out's."""
+    if out and out in inputs:
+        raise _lib.GfnError("out is one of the inputs")
+    return out
 
 
 def _gated_args(x, Wg, Wu, bg, bu, act, n_dev, what):
-    ldx = _rows(x, "x")
+    n, k, ldx = _rows(x, "x")
     if act not in GATED_ACT:
         raise _lib.GfnError(f"{what}: act {act!r} is none of {sorted(GATED_ACT)}")
-    if not isinstance(Wg, torch.Tensor) or Wg.dim() != 2 or Wg.shape[1] != x.shape[1]:
-        raise _lib.GfnError(f"{what}: Wg must be [hidden, {x.shape[1]}], got {tuple(getattr(Wg, 'shape', ()))}")
-    h, k = Wg.shape
-    _flat(Wg, x.dtype, "Wg", (h, k)); _flat(Wu, x.dtype, "Wu", (h, k)); _flat(bg, x.dtype, "bg", (h,)); _flat(bu, x.dtype, "bu", (h,))
+    shape, dtype = getattr(Wg, "shape", ()), x.dtype
+    if not isinstance(Wg, torch.Tensor) or len(shape) != 2 or shape[1] != k:
+        raise _lib.GfnError(f"{what}: Wg must be [hidden, {k}], got {tuple(shape)}")
+    h = shape[0]
+    _flat(Wg, dtype, "Wg", shape); _flat(Wu, dtype, "Wu", shape); _flat(bg, dtype, "bg", (h,)); _flat(bu, dtype, "bu", (h,))
     if Wu is None or (bg is None) != (bu is None):
         raise _lib.GfnError(f"{what}: Wg needs Wu, and bg needs bu")
     _flat(n_dev, torch.int32, "n_dev", (1,))
-    _place((x, Wg, Wu, bg, bu, n_dev))
-    return x.shape[0], k, h, ldx
+    return n, k, h, ldx, dtype
 
 
 def gated_fwd(x, Wg, Wu, bg=None, bu=None, act="silu", out=None, n_dev=None):
     """h = act(x Wg^T + bg) * (x Wu^T + bu): both projections, the activation and the product in one launch.  x [n, in] (rows at any
     stride), Wg / Wu [hidden, in], bg / bu [hidden] or both None; f32, bf16 or f16 throughout, sums in f32; act "silu", "gelu" (erf),
     "relu" or "sigmoid"; in 1..128, hidden 1..1024.  n_dev i32 [1]: live rows (those behind are left alone)."""
-    n, k, h, ldx = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_fwd")
+    n, k, h, ldx, dtype = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_fwd")
     if out is None:
-        out = torch.empty((n, h), dtype=x.dtype, device=x.device)
-    ldo = _rows(out, "out", x.dtype, h, n)
-    _place((out,)); _apart(out, x, Wg, Wu, bg, bu)
-    rc = _lib.lib().gfn_gated_fwd(_ptr(x), ldx, _ptr(Wg), _ptr(Wu), _ptr(bg), _ptr(bu), n, _ptr(n_dev), k, h, DTYPES[x.dtype], GATED_ACT[act], _ptr(out), ldo,
-                                  _stream())
+        out = x.new_empty((n, h))
+    ldo = _rows(out, "out", dtype, h, n)[2]
+    stream = _place(x, Wg, Wu, bg, bu, n_dev, out)
+    at = [_at(t) for t in (x, Wg, Wu, bg, bu)]
+    rc = _lib.lib().gfn_gated_fwd(at[0], ldx, at[1], at[2], at[3], at[4], n, _at(n_dev), k, h, DTYPES[dtype], GATED_ACT[act], _apart(out.data_ptr(), *at), ldo, stream)
     _lib.check(rc, "gfn_gated_fwd")
     return out
 
@@ -1463,30 +1475,30 @@ def gated_fwd(x, Wg, Wu, bg=None, bu=None, act="silu", out=None, n_dev=None):
 def gated_bwd(x, Wg, Wu, dh, bg=None, bu=None, act="silu", need_dx=True, need_dw=True, n_dev=None):
     """Gradients of gated_fwd for dh -> (dx, dWg, dWu, dbg, dbu); None for what is not wanted or not there.  The projections are formed
     again from x (the forward saves nothing); the weights' gradients are sums in a fixed order, rounded once to x's dtype."""
-    n, k, h, ldx = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_bwd")
-    lddh = _rows(dh, "dh", x.dtype, h, n)
-    _place((dh,))
-    new = lambda *shape: torch.empty(shape, dtype=x.dtype, device=x.device)  # noqa: E731
-    dx = new(n, k) if need_dx else None
-    dWg, dWu = (new(h, k), new(h, k)) if need_dw else (None, None)
-    dbg, dbu = (new(h), new(h)) if need_dw and bg is not None else (None, None)
+    n, k, h, ldx, dtype = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_bwd")
+    lddh = _rows(dh, "dh", dtype, h, n)[2]
+    stream = _place(x, Wg, Wu, bg, bu, n_dev, dh)
+    dx = x.new_empty((n, k)) if need_dx else None
+    dWg, dWu = (x.new_empty((h, k)), x.new_empty((h, k))) if need_dw else (None, None)
+    dbg, dbu = (x.new_empty((h,)), x.new_empty((h,))) if need_dw and bg is not None else (None, None)
     lib = _lib.lib()
-    size = lib.gfn_gated_bwd_workspace(n, k, h, DTYPES[x.dtype], bg is not None, need_dx, need_dw)
+    size = lib.gfn_gated_bwd_workspace(n, k, h, DTYPES[dtype], bg is not None, need_dx, need_dw)
     _lib.check(min(size, 0), "gfn_gated_bwd_workspace")
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    rc = lib.gfn_gated_bwd(_ptr(x), ldx, _ptr(Wg), _ptr(Wu), _ptr(bg), _ptr(bu), _ptr(dh), lddh, n, _ptr(n_dev), k, h, DTYPES[x.dtype], GATED_ACT[act], _ptr(dx), k,
-                           _ptr(dWg), _ptr(dWu), _ptr(dbg), _ptr(dbu), _ptr(ws), size, _stream())
+    ws = x.new_empty((size,), dtype=torch.uint8) if size else None
+    rc = lib.gfn_gated_bwd(_at(x), ldx, _at(Wg), _at(Wu), _at(bg), _at(bu), _at(dh), lddh, n, _at(n_dev), k, h, DTYPES[dtype], GATED_ACT[act], _at(dx), k,
+                           _at(dWg), _at(dWu), _at(dbg), _at(dbu), _at(ws), size, stream)
     _lib.check(rc, "gfn_gated_bwd")
     return dx, dWg, dWu, dbg, dbu
 
 
-def _scan_args(f, c, gate, what, n=None):
-    ldf, ldc = _rows(f, "f", None, None, n), _rows(c, "c", getattr(f, "dtype", None), None, f.shape[0])
+def _scan_args(f, c, gate, what):
+    n, g, ldf = _rows(f, "f")
+    _, d, ldc = _rows(c, "c", f.dtype, None, n)
     if gate not in SCAN_GATE:
         raise _lib.GfnError(f"{what}: gate {gate!r} is none of {sorted(SCAN_GATE)}")
-    if f.shape[1] == 0 or c.shape[1] % f.shape[1]:
-        raise _lib.GfnError(f"{what}: {f.shape[1]} gates for {c.shape[1]} channels")
-    return ldf, ldc
+    if g == 0 or d % g:
+        raise _lib.GfnError(f"{what}: {g} gates for {d} channels")
+    return n, d, g, ldf, ldc, c.dtype
 
 
 def _scan_rays(pts_offsets, what):
@@ -1496,10 +1508,10 @@ def _scan_rays(pts_offsets, what):
     return pts_offsets.numel() - 1
 
 
-def _scan_workspace(rays, n, d, g, device):
+def _scan_workspace(rays, n, d, g, like):
     size = _lib.lib().gfn_ray_scan_workspace(rays, n, d, g)
     _lib.check(min(size, 0), "gfn_ray_scan_workspace")
-    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+    return (like.new_empty((size,), dtype=torch.uint8) if size else None), size
 
 
 def ray_scan_fwd(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, out=None, save=False):
@@ -1510,17 +1522,17 @@ def ray_scan_fwd(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, out=
     h0 f32 [rays, channels] or None (0).  -> dict(h [n, channels], state f32 [rays, channels] (every ray's last state), saved (save=True:
     what ray_scan_bwd needs)).  Rows behind the last ray's: 0 in an h allocated here, left alone in `out`."""
     R = _scan_rays(pts_offsets, "ray_scan_fwd")
-    ldf, ldc = _scan_args(f, c, gate, "ray_scan_fwd")
-    (n, d), g, dev = c.shape, f.shape[1], c.device
+    n, d, g, ldf, ldc, dtype = _scan_args(f, c, gate, "ray_scan_fwd")
     _flat(h0, torch.float32, "h0", (R, d))
-    h = torch.empty((n, d), dtype=c.dtype, device=dev) if out is None else out
-    ldh = _rows(h, "out", c.dtype, d, n)
-    _place((pts_offsets, f, c, h0, h)); _apart(h, f, c, h0)
-    state = torch.empty((R, d), dtype=torch.float32, device=dev)
-    ws, size = _scan_workspace(R, n, d, g, dev)
-    saved = torch.empty(((n + SCAN_BLOCK - 1) // SCAN_BLOCK, d), dtype=torch.float32, device=dev) if save else None
-    rc = _lib.lib().gfn_ray_scan_fwd(_ptr(pts_offsets), R, _ptr(f), ldf, _ptr(c), ldc, n, d, g, DTYPES[c.dtype], SCAN_GATE[gate], int(reverse), _ptr(h0), _ptr(h), ldh,
-                                     _ptr(state), _ptr(saved), out is None, _ptr(ws), size, _stream())
+    h = c.new_empty((n, d)) if out is None else out
+    ldh = _rows(h, "out", dtype, d, n)[2]
+    stream = _place(pts_offsets, f, c, h0, h)
+    state = c.new_empty((R, d), dtype=torch.float32)
+    ws, size = _scan_workspace(R, n, d, g, c)
+    saved = c.new_empty(((n + SCAN_BLOCK - 1) // SCAN_BLOCK, d), dtype=torch.float32) if save else None
+    at = _at(f), _at(c), _at(h0)
+    rc = _lib.lib().gfn_ray_scan_fwd(_at(pts_offsets), R, at[0], ldf, at[1], ldc, n, d, g, DTYPES[dtype], SCAN_GATE[gate], int(reverse), at[2], _apart(h.data_ptr(), *at), ldh,
+                                     _at(state), _at(saved), out is None, _at(ws), size, stream)
     _lib.check(rc, "gfn_ray_scan_fwd")
     return dict(h=h, state=state, saved=saved)
 
@@ -1529,19 +1541,18 @@ def ray_scan_bwd(pts_offsets, f, c, dh, saved, gate="sigmoid", reverse=False, h0
     """Gradients of ray_scan_fwd (same f, c, h0, flags; `saved` from its save=True) for dh [n, channels] and d_state f32 [rays, channels] or
     None (0) -> dict(df [n, gates], dc [n, channels], dh0 f32 [rays, channels]).  Rows behind the last ray's are 0."""
     R = _scan_rays(pts_offsets, "ray_scan_bwd")
-    ldf, ldc = _scan_args(f, c, gate, "ray_scan_bwd")
-    (n, d), g, dev = c.shape, f.shape[1], c.device
-    lddh = _rows(dh, "dh", c.dtype, d, n)
+    n, d, g, ldf, ldc, dtype = _scan_args(f, c, gate, "ray_scan_bwd")
+    lddh = _rows(dh, "dh", dtype, d, n)[2]
     _flat(h0, torch.float32, "h0", (R, d)); _flat(d_state, torch.float32, "d_state", (R, d))
     if saved is None:
         raise _lib.GfnError("ray_scan_bwd: saved is missing (ray_scan_fwd with save=True)")
     _flat(saved, torch.float32, "saved", ((n + SCAN_BLOCK - 1) // SCAN_BLOCK, d))
-    _place((pts_offsets, f, c, dh, saved, h0, d_state))
-    df, dc = torch.empty((n, g), dtype=c.dtype, device=dev), torch.empty((n, d), dtype=c.dtype, device=dev)
-    dh0 = torch.empty((R, d), dtype=torch.float32, device=dev)
-    ws, size = _scan_workspace(R, n, d, g, dev)
-    rc = _lib.lib().gfn_ray_scan_bwd(_ptr(pts_offsets), R, _ptr(f), ldf, _ptr(c), ldc, _ptr(dh), lddh, n, d, g, DTYPES[c.dtype], SCAN_GATE[gate], int(reverse), _ptr(h0),
-                                     _ptr(d_state), _ptr(saved), _ptr(df), g, _ptr(dc), d, _ptr(dh0), 1, _ptr(ws), size, _stream())
+    stream = _place(pts_offsets, f, c, dh, saved, h0, d_state)
+    df, dc = c.new_empty((n, g)), c.new_empty((n, d))
+    dh0 = c.new_empty((R, d), dtype=torch.float32)
+    ws, size = _scan_workspace(R, n, d, g, c)
+    rc = _lib.lib().gfn_ray_scan_bwd(_at(pts_offsets), R, _at(f), ldf, _at(c), ldc, _at(dh), lddh, n, d, g, DTYPES[dtype], SCAN_GATE[gate], int(reverse), _at(h0),
+                                     _at(d_state), _at(saved), _at(df), g, _at(dc), d, _at(dh0), 1, _at(ws), size, stream)
     _lib.check(rc, "gfn_ray_scan_bwd")
     return dict(df=df, dc=dc, dh0=dh0)
 
@@ -1549,15 +1560,15 @@ def ray_scan_bwd(pts_offsets, f, c, dh, saved, gate="sigmoid", reverse=False, h0
 def ray_scan_step(f, c, state, gate="sigmoid", out=None):
     """One more sample of every ray: state [rays, channels] f32 <- a state + b, in place; -> h [rays, channels] in c's dtype.  f [rays, gates],
     c [rays, channels] as in ray_scan_fwd."""
-    ldf, ldc = _scan_args(f, c, gate, "ray_scan_step")
-    n, d = c.shape
+    n, d, g, ldf, ldc, dtype = _scan_args(f, c, gate, "ray_scan_step")
     if state is None:
         raise _lib.GfnError("ray_scan_step: state is missing")
     _flat(state, torch.float32, "state", (n, d))
-    h = torch.empty((n, d), dtype=c.dtype, device=c.device) if out is None else out
-    ldh = _rows(h, "out", c.dtype, d, n)
-    _place((f, c, state, h)); _apart(h, f, state)
-    rc = _lib.lib().gfn_ray_scan_step(_ptr(f), ldf, _ptr(c), ldc, n, d, f.shape[1], DTYPES[c.dtype], SCAN_GATE[gate], _ptr(state), _ptr(h), ldh, _stream())
+    h = c.new_empty((n, d)) if out is None else out
+    ldh = _rows(h, "out", dtype, d, n)[2]
+    stream = _place(f, c, state, h)
+    at = _at(f), _at(state)
+    rc = _lib.lib().gfn_ray_scan_step(at[0], ldf, _at(c), ldc, n, d, g, DTYPES[dtype], SCAN_GATE[gate], at[1], _apart(h.data_ptr(), *at), ldh, stream)
     _lib.check(rc, "gfn_ray_scan_step")
     return h
 
@@ -1568,9 +1579,9 @@ def dropout_call(counter):
     _flat(counter, torch.int64, "counter", (1,))
     if counter is None:
         raise _lib.GfnError("dropout_call: counter is missing")
-    _place((counter,))
-    call = torch.empty(1, dtype=torch.int64, device=counter.device)
-    _lib.check(_lib.lib().gfn_dropout_call(_ptr(counter), _ptr(call), _stream()), "gfn_dropout_call")
+    stream = _place(counter)
+    call = counter.new_empty((1,))
+    _lib.check(_lib.lib().gfn_dropout_call(_at(counter), _at(call), stream), "gfn_dropout_call")
     return call
 
 
@@ -1578,14 +1589,15 @@ def dropout(x, p, seed, call, out=None):
     """y = x where the element is kept, times 65536 / (65536 - t), t = round(65536 p); 0 where it is dropped.  Which elements are kept is a
     function of (seed, call, row, column) -- Philox4x32-10, 16 bits an element -- and never stored: the gradient is the same call on dy.
     x [n, columns] (f32, bf16 or f16, rows at any stride), call i64 [1] (dropout_call); out may be x."""
-    ldx = _rows(x, "x")
+    n, d, ldx = _rows(x, "x")
     if call is None:
         raise _lib.GfnError("dropout: call is missing")
     _flat(call, torch.int64, "call", (1,))
-    y = torch.empty((x.shape[0], x.shape[1]), dtype=x.dtype, device=x.device) if out is None else out
-    ldy = _rows(y, "out", x.dtype, x.shape[1], x.shape[0])
-    _place((x, call, y))
-    rc = _lib.lib().gfn_dropout(_ptr(x), ldx, x.shape[0], x.shape[1], DTYPES[x.dtype], float(p), int(seed) & 0xFFFFFFFFFFFFFFFF, _ptr(call), _ptr(y), ldy, _stream())
+    y = x.new_empty((n, d)) if out is None else out
+    dtype = x.dtype
+    ldy = _rows(y, "out", dtype, d, n)[2]
+    stream = _place(x, call, y)
+    rc = _lib.lib().gfn_dropout(_at(x), ldx, n, d, DTYPES[dtype], float(p), int(seed) & 0xFFFFFFFFFFFFFFFF, _at(call), _at(y), ldy, stream)
     _lib.check(rc, "gfn_dropout")
     return y
 
