@@ -23,6 +23,10 @@ namespace {
 
 constexpr int kWaves = 4;
 
+// Waits for the rows requested ahead, before this tile's last results are stored: loads and stores are counted together and in order, so a
+// wait for those rows behind the stores would be a wait for the stores.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 template <int V>
 struct Constant {
   static constexpr int value = V;
@@ -172,6 +176,19 @@ __device__ __forceinline__ u32x2 tr4(const char* a) {
 // waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit
 constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 
+// bytes behind a row of dz: the rows that one read covers start on different banks (16 rows of 8-byte pieces; f32: 2 rows of 64 bytes)
+constexpr int bwd_pad(int size) { return size == 4 ? 64 : 16; }
+// LDS of a workgroup of the backward with room for the dz of `buffers` pairs of feature tiles
+constexpr int bwd_lds(int size, int ks, int np, int buffers) {
+  return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * 64 * size + bwd_pad(size)) + 32;
+}
+// Pairs whose dz are kept: all of them (one barrier a tile before dW's product, which then reads x once for all pairs), or two (a
+// barrier a pair) or one (two), whichever still fits and does not cost the CU its second workgroup.
+constexpr int bwd_buffers(int size, int ks, int np) {
+  const int room = bwd_lds(size, ks, np, 1) <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
+  return bwd_lds(size, ks, np, np) <= room ? np : np > 2 && bwd_lds(size, ks, np, 2) <= room ? 2 : 1;
+}
+
 struct GatedBwd {
   int64_t n_max;
   const int32_t* n_dev;
@@ -181,7 +198,6 @@ struct GatedBwd {
   void* dx;           // T, or null
   float* dx_sum;      // f32 [n_max][k] between the launches of several feature blocks, or null
   int dx_first, dx_last;
-  int z_buffers;      // 1 or 2 tiles of dz in LDS
   float* part;        // [workgroup][64 NP][kp] f32, or null: column k is the bias's
   int kp;
 };
@@ -190,14 +206,14 @@ template <typename T, int KS, int NP>
 __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_kernel(GatedBwd a) {
   constexpr int WAVES = bwd_waves(KS);
   constexpr int E = Piece<T>::E, TPU = sizeof(T) == 4 ? 1 : 2;  // 16-column tiles a unit
-  constexpr int KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP;
-  constexpr int SAMPLES = 16 * WAVES, ZROW = 64 * (int)sizeof(T) + 16;
+  constexpr int KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP, NB = bwd_buffers(sizeof(T), KS, NP);
+  constexpr int SAMPLES = 16 * WAVES, ZTILE = 64 * (int)sizeof(T), ZROW = NB * ZTILE + bwd_pad(sizeof(T));
   constexpr int FT_WAVES = WAVES / 4, KT_WAVE = (KT + FT_WAVES - 1) / FT_WAVES;  // waves that share a row tile of dW, its column tiles a wave
   constexpr bool EXACT = sizeof(T) == 4, SCALED = sizeof(T) == 2 && !__is_same(T, __bf16);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* xs = lds + 2 * HB * ROW;        // [SAMPLES][ROW]
-  char* zs = xs + SAMPLES * ROW;        // [z_buffers][SAMPLES][dg 32 | du 32]
-  float* bias = reinterpret_cast<float*>(zs + a.z_buffers * SAMPLES * ZROW);  // [2][HB]
+  char* zs = xs + SAMPLES * ROW;        // [SAMPLES][NB][dg 32 | du 32]
+  float* bias = reinterpret_cast<float*>(zs + SAMPLES * ZROW);  // [2][HB]
   float* top = bias + 2 * HB;                                                 // [WAVES]
   const T *x = static_cast<const T*>(a.x), *dh = static_cast<const T*>(a.dh);
   const bool biased = a.bg != nullptr;
@@ -298,6 +314,61 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         run_e = e;
       }
     }
+    // dW's rows of the pairs p0 .. p0 + PN - 1 += their dz^T x over the tile's samples, and db their sums
+    auto product = [&](int p0, auto pairs_c) {
+      constexpr int PN = decltype(pairs_c)::value;
+      f32x4 total[PN];  // the same in every column
+#pragma unroll
+      for (int i = 0; i < PN; i++) total[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (sizeof(T) == 2) {
+        // 32 samples at a time, in the order 4 kg .. + 3, 16 + 4 kg .. + 3: a read covers 16 rows, on different banks
+        const char* r = zs + (4 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
+        const char* q = xs + (4 * kg + (j >> 2)) * ROW + 8 * (j & 3) + 32 * kt0;
+        constexpr uint32_t one = __is_same(T, __bf16) ? 0x3f803f80u : 0x3c003c00u;
+        u32x4 av[PN];
+        read_ahead<SAMPLES / 32 * KT_WAVE, IN_FLIGHT>(
+            [&](int i) {
+              const char* e = q + 32 * (i / KT_WAVE) * ROW + 32 * (i % KT_WAVE);
+              const u32x2 lo = tr4(e), hi = tr4(e + 16 * ROW);
+              return u32x4{lo[0], lo[1], hi[0], hi[1]};
+            },
+            [&](int i, const u32x4& b) {
+              const int c = i / KT_WAVE, t = i % KT_WAVE;
+#pragma unroll
+              for (int o = 0; o < PN; o++) {
+                if (t == 0) {
+                  const char* e = r + 32 * c * ZROW + (p0 + o) % NB * ZTILE;
+                  const u32x2 lo = tr4(e), hi = tr4(e + 16 * ZROW);
+                  av[o] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                  total[o] = mma(av[o], u32x4{one, one, one, one}, total[o], (T*)nullptr);
+                }
+                dw[p0 + o][t] = mma(av[o], b, dw[p0 + o][t], (T*)nullptr);
+              }
+            });
+      } else {
+#pragma unroll 4
+        for (int c = 0; c < SAMPLES; c += 4) {
+          const char* q = xs + (c + kg) * ROW + j * 4;
+          float av[PN];
+#pragma unroll
+          for (int o = 0; o < PN; o++) {
+            av[o] = *reinterpret_cast<const float*>(zs + (c + kg) * ZROW + (p0 + o) % NB * ZTILE + (16 * ft + j) * 4);
+            total[o] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[o], 1.f, total[o], 0, 0, 0);
+          }
+#pragma unroll
+          for (int t = 0; t < KT_WAVE; t++)
+            if (KT % FT_WAVES == 0 || kt0 + t < KT) {
+              const float b = *reinterpret_cast<const float*>(q + 64 * (kt0 + t));
+#pragma unroll
+              for (int o = 0; o < PN; o++) dw[p0 + o][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[o], b, dw[p0 + o][t], 0, 0, 0);
+            }
+        }
+      }
+#pragma unroll
+      for (int o = 0; o < PN; o++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) db[i] = j == p0 + o ? db[i] + total[o][i] : db[i];
+    };
     f32x4 dx[KT];
 #pragma unroll
     for (int t = 0; t < KT; t++) dx[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -341,50 +412,21 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         }
       }
       if (a.part) {
-        if (p && a.z_buffers == 1) __syncthreads();  // the features before have been read; of two buffers, the one before those
-        char* zb = zs + (p & (a.z_buffers - 1)) * SAMPLES * ZROW;
-        char* zr = zb + (wave * 16 + j) * ZROW + 8 * kg * sizeof(T);
+        if (NB == 1 && p) __syncthreads();  // the pair before has been read; of two buffers, the one before that
+        char* zr = zs + (wave * 16 + j) * ZROW + p % NB * ZTILE + 8 * kg * sizeof(T);
         __builtin_memcpy(__builtin_assume_aligned(zr, 16), z[0], sizeof(z[0]));
         __builtin_memcpy(__builtin_assume_aligned(zr + 32 * sizeof(T), 16), z[1], sizeof(z[1]));
-        __syncthreads();
-        f32x4 total = {0.f, 0.f, 0.f, 0.f};  // dz summed over the samples, the same in every column
-        if constexpr (sizeof(T) == 2) {
-          // 32 samples at a time, in the order 4 kg .. + 3, 16 + 4 kg .. + 3: a read covers 16 rows, on different banks
-          const char* r = zb + (4 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
-          const char* q = xs + (4 * kg + (j >> 2)) * ROW + 8 * (j & 3) + 32 * kt0;
-          constexpr uint32_t one = __is_same(T, __bf16) ? 0x3f803f80u : 0x3c003c00u;
-          u32x4 av[2];
-          read_ahead<SAMPLES / 32 * KT_WAVE, IN_FLIGHT>(
-              [&](int i) {
-                const int c = i / KT_WAVE, t = i % KT_WAVE;
-                if (t == 0) {
-                  const u32x2 l = tr4(r + 32 * c * ZROW), u = tr4(r + (32 * c + 16) * ZROW);
-                  av[c & 1] = u32x4{l[0], l[1], u[0], u[1]};
-                }
-                const u32x2 lo = tr4(q + 32 * c * ROW + 32 * t), hi = tr4(q + (32 * c + 16) * ROW + 32 * t);
-                return u32x4{lo[0], lo[1], hi[0], hi[1]};
-              },
-              [&](int i, const u32x4& b) {
-                const u32x4& a4 = av[i / KT_WAVE & 1];
-                if (i % KT_WAVE == 0) total = mma(a4, u32x4{one, one, one, one}, total, (T*)nullptr);
-                dw[p][i % KT_WAVE] = mma(a4, b, dw[p][i % KT_WAVE], (T*)nullptr);
-              });
-        } else {
-#pragma unroll 4
-          for (int c = 0; c < SAMPLES; c += 4) {
-            const float av = *reinterpret_cast<const float*>(zb + (c + kg) * ZROW + (16 * ft + j) * 4);
-            const char* q = xs + (c + kg) * ROW + j * 4;
-            total = __builtin_amdgcn_mfma_f32_16x16x4f32(av, 1.f, total, 0, 0, 0);
-#pragma unroll
-            for (int t = 0; t < KT_WAVE; t++)
-              if (KT % FT_WAVES == 0 || kt0 + t < KT)
-                dw[p][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av, *reinterpret_cast<const float*>(q + 64 * (kt0 + t)), dw[p][t], 0, 0, 0);
-          }
+        if constexpr (NB < NP) {
+          __syncthreads();
+          product(p, Constant<1>{});
         }
-#pragma unroll
-        for (int r = 0; r < 4; r++) db[r] = j == p ? db[r] + total[r] : db[r];
       }
     }
+    if (NB == NP && a.part) {
+      __syncthreads();
+      product(0, Constant<NP>{});
+    }
+    if constexpr (AHEAD) loads_done();
     if ((a.dx || a.dx_sum) && s < n) {  // lane (j, kg) holds columns 16 t + 4 kg + r of sample j
 #pragma unroll
       for (int t = 0; t < KT; t++) {
@@ -521,7 +563,7 @@ int dispatch_fwd(const GatedFwd& a, hipStream_t st) {
 
 // The backward's plan for (n, k, h, type): units a row, feature blocks of 32 NP, waves and workgroups.
 struct BwdPlan {
-  int ks, np, waves, blocks, launches, z_buffers, kp;
+  int ks, np, waves, blocks, launches, kp;
   size_t lds, part_floats;
   bool dx_sum;
 };
@@ -537,12 +579,8 @@ BwdPlan plan_bwd(int64_t n, int k, int h, int dtype, bool bias) {
   const int pairs = (h + 31) / 32;
   p.np = pairs >= 3 && most == 4 ? 4 : pairs >= 2 ? 2 : 1;
   p.launches = (pairs + p.np - 1) / p.np;
-  const int row = p.ks * 64 + 16, samples = 16 * p.waves;
-  const size_t z = (size_t)samples * (64 * size + 16);
-  p.lds = (size_t)64 * p.np * (row + 4) + (size_t)samples * row + z + 32;
-  // a second buffer for dz (one barrier a pair of tiles instead of two) where it does not cost the CU its second workgroup
-  p.z_buffers = p.np > 1 && (p.lds + z <= 80 * 1024 || (p.lds > 80 * 1024 && p.lds + z <= 160 * 1024)) ? 2 : 1;
-  p.lds += (p.z_buffers - 1) * z;
+  const int samples = 16 * p.waves;
+  p.lds = bwd_lds(size, p.ks, p.np, bwd_buffers(size, p.ks, p.np));
   const int64_t tiles = (n + samples - 1) / samples;
   const int at_once = 256 * (p.lds <= 80 * 1024 ? 2 : 1);
   p.blocks = tiles < 1 ? 1 : (int)(tiles < at_once ? tiles : at_once);
@@ -646,7 +684,6 @@ int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, co
   a.ldx = ldx; a.lddh = lddh; a.lddx = lddx;
   a.k = in_dim; a.h = hidden; a.act = act;
   a.dx = dx;
-  a.z_buffers = p.z_buffers;
   a.kp = p.kp;
   float* ws = static_cast<float*>(workspace);
   if (dwg) {
