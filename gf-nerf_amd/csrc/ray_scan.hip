@@ -76,11 +76,14 @@ struct ScanArgs {
   int lanes, slot, parts;
   float* partial;
   int64_t run_rows, runs;  // 0: a walk is a ray; else rows of a run (a multiple of kBlock) and their number
-  float2* agg;             // [runs][d]: AGG writes (A, S); then .y is the state in front of the run
+  float2* agg;             // [d][runs]: AGG writes (A, S); then .y is the state in front of the run
 };
 
 // a state that meets a ray's beginning (a = 0) stays out of it, infinite or not
 __device__ __forceinline__ float compose(float a, float b, float s) { return a == 0.f || s == 0.f ? b : __builtin_fmaf(a, s, b); }
+
+// the A of a step a1 and then a2: zero (a ray's beginning) stays zero
+__device__ __forceinline__ float carry(float a1, float a2) { return a1 == 0.f ? 0.f : a1 * a2; }
 
 struct Place {
   int64_t walk;  // the ray or run
@@ -237,11 +240,21 @@ struct Gates {
   }
 };
 
+// Walks along runs never meet a ray without rows: its last state is the one it starts with (its adjoint likewise).
+__device__ __forceinline__ void empty_rays(const ScanArgs& a, const float* __restrict__ from, float* __restrict__ to) {
+  const int lane = threadIdx.x & 63;
+  const int64_t waves = (int64_t)gridDim.x * blockDim.x / 64;
+  for (int64_t ray = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 64; ray < a.rays; ray += waves)
+    if (a.offsets[ray + 1] <= a.offsets[ray])
+      for (int i = lane; i < a.d; i += 64) to[ray * a.d + i] = from ? from[ray * a.d + i] : 0.f;
+}
+
 template <typename T, int GATE, int VEC, bool SHARED, bool AGG>
 __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
   using V = Vec<T, VEC>;
   __shared__ float2 pool[SHARED ? kScanThreads : 1];
   if (!AGG && a.clear) clear_rows(a, static_cast<T*>(a.h), a.ldh, a.d);
+  if (!AGG && a.run_rows && a.state) empty_rays(a, a.h0, a.state);
   Place at;
   if (!scan_place<VEC, SHARED>(a, at)) return;
   const bool asc = !a.reverse, dealt = SHARED && a.slot >= kBlock;
@@ -252,7 +265,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
   float s[VEC], A[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; v++) {
-    s[v] = !AGG && a.run_rows ? a.agg[at.walk * a.d + at.ch + v].y : 0.f;
+    s[v] = !AGG && a.run_rows ? a.agg[(at.ch + v) * a.runs + at.walk].y : 0.f;
     A[v] = 1.f;
   }
   Pieces pieces(a, at.walk, asc);
@@ -290,7 +303,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
         for (int v = 0; v < VEC; v++) {
           const float n = __builtin_fmaf(x[v], s[v], y[v] * now.in(r, v));
           s[v] = in ? n : s[v];
-          if (AGG) A[v] = in ? A[v] * x[v] : A[v];
+          if (AGG) A[v] = in ? carry(A[v], x[v]) : A[v];
           o.v[v] = (T)s[v];
         }
         if (!AGG) {
@@ -306,7 +319,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
   }
   if (AGG && at.active)
 #pragma unroll
-    for (int v = 0; v < VEC; v++) a.agg[at.walk * a.d + at.ch + v] = make_float2(A[v], s[v]);
+    for (int v = 0; v < VEC; v++) a.agg[(at.ch + v) * a.runs + at.walk] = make_float2(A[v], s[v]);
 }
 
 template <typename T, int GATE, int VEC, bool SHARED, bool AGG>
@@ -317,6 +330,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
     clear_rows(a, static_cast<T*>(a.df), a.lddf, a.g);
     clear_rows(a, static_cast<T*>(a.dc), a.lddc, a.d);
   }
+  if (!AGG && a.run_rows && a.dh0) empty_rays(a, a.d_state, a.dh0);
   Place at;
   if (!scan_place<VEC, SHARED>(a, at)) return;
   const bool asc = a.reverse != 0, dealt = SHARED && a.slot >= kBlock;  // against the recurrence
@@ -327,7 +341,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
   float l[VEC], A[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; v++) {
-    l[v] = !AGG && a.run_rows ? a.agg[at.walk * a.d + at.ch + v].y : 0.f;
+    l[v] = !AGG && a.run_rows ? a.agg[(at.ch + v) * a.runs + at.walk].y : 0.f;
     A[v] = 1.f;
   }
   Pieces pieces(a, at.walk, asc);
@@ -396,7 +410,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
             else of.v[v] = (T)d;
           }
           l[v] = in ? xv * lt : l[v];
-          if (AGG) A[v] = in ? A[v] * xv : A[v];
+          if (AGG) A[v] = in ? carry(A[v], xv) : A[v];
         }
         if (!AGG) {
           if (whole) {
@@ -445,47 +459,57 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
   }
   if (AGG && at.active)
 #pragma unroll
-    for (int v = 0; v < VEC; v++) a.agg[at.walk * a.d + at.ch + v] = make_float2(A[v], l[v]);
+    for (int v = 0; v < VEC; v++) a.agg[(at.ch + v) * a.runs + at.walk] = make_float2(A[v], l[v]);
 }
 
-// AGG's steps -> the state in front of every run (in the walk's order).  A workgroup: 4 channels, 256 stretches of runs, each composed in registers
-// (up to kHeld runs of a stretch; more are read twice), joined in order through LDS.
-constexpr int kHeld = 16;
-__global__ __launch_bounds__(1024) void run_prefix_kernel(float2* __restrict__ agg, int64_t runs, int d) {
-  __shared__ float2 part[256][4];
-  const int lane = threadIdx.x & 3, stretch = threadIdx.x >> 2, ch = blockIdx.x * 4 + lane;
-  const int64_t per = (runs + 255) / 256, lo = stretch * per, hi = lo + per < runs ? lo + per : runs;
+// AGG's steps -> the state in front of every run (in the walk's order).  A workgroup: one channel, 1,024 stretches of neighbouring runs, each
+// composed in registers (up to kHeld runs of a stretch; more are read twice), the stretches joined by doubling within a wave and the
+// waves' steps one after the other.  Latency bound: 5 us for 4,096 runs of 64 channels; with the steps as [runs][channels], four
+// channels a workgroup, 18 us -- every load then takes 32 bytes of a line, on a quarter of the CUs.
+constexpr int kHeld = 4, kPrefixWaves = 16;
+__global__ __launch_bounds__(64 * kPrefixWaves) void run_prefix_kernel(float2* __restrict__ steps, int64_t runs) {
+  __shared__ float2 last[kPrefixWaves];
+  float2* __restrict__ agg = steps + (int64_t)blockIdx.x * runs;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t per = (runs + 64 * kPrefixWaves - 1) / (64 * kPrefixWaves), lo = threadIdx.x * per, hi = lo + per < runs ? lo + per : runs;
   float2 held[kHeld];
   float a = 1.f, s = 0.f;
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) held[i] = ch < d && lo + i < hi ? agg[(lo + i) * d + ch] : make_float2(1.f, 0.f);
+  for (int i = 0; i < kHeld; i++) held[i] = lo + i < hi ? agg[lo + i] : make_float2(1.f, 0.f);
 #pragma unroll
   for (int i = 0; i < kHeld; i++)
     if (lo + i < hi) {
       s = compose(held[i].x, held[i].y, s);
-      a *= held[i].x;
+      a = carry(a, held[i].x);
     }
-  if (ch < d)
-    for (int64_t i = lo + kHeld; i < hi; i++) {
-      const float2 q = agg[i * d + ch];
-      s = compose(q.x, q.y, s);
-      a *= q.x;
+  for (int64_t i = lo + kHeld; i < hi; i++) {
+    const float2 q = agg[i];
+    s = compose(q.x, q.y, s);
+    a = carry(a, q.x);
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {  // then (a, s) is the step of the wave's stretches up to this one
+    const float a1 = __shfl_up(a, off, 64), s1 = __shfl_up(s, off, 64);
+    if (lane >= off) {
+      s = compose(a, s, s1);
+      a = carry(a1, a);
     }
-  part[stretch][lane] = make_float2(a, s);
+  }
+  if (lane == 63) last[wave] = make_float2(a, s);
   __syncthreads();
-  if (ch >= d || lo >= hi) return;
-  s = 0.f;
-#pragma unroll 8
-  for (int r = 0; r < stretch; r++) s = compose(part[r][lane].x, part[r][lane].y, s);
+  float front = 0.f;  // the state in front of the wave's first stretch, then of this one
+  for (int w = 0; w < wave; w++) front = compose(last[w].x, last[w].y, front);
+  const float a1 = __shfl_up(a, 1, 64), s1 = __shfl_up(s, 1, 64);
+  s = lane ? compose(a1, s1, front) : front;
 #pragma unroll
   for (int i = 0; i < kHeld; i++)
     if (lo + i < hi) {
-      agg[(lo + i) * d + ch].y = s;
+      agg[lo + i].y = s;
       s = compose(held[i].x, held[i].y, s);
     }
   for (int64_t i = lo + kHeld; i < hi; i++) {
-    const float2 q = agg[i * d + ch];
-    agg[i * d + ch].y = s;
+    const float2 q = agg[i];
+    agg[i].y = s;
     s = compose(q.x, q.y, s);
   }
 }
@@ -502,14 +526,6 @@ __global__ __launch_bounds__(256) void scan_gate_sums_kernel(ScanArgs a, const f
       for (int i = 0; i < parts; i++) s += partial[i * n + e];
     static_cast<T*>(a.df)[e / a.g * a.lddf + e % a.g] = (T)s;
   }
-}
-
-// rays without samples: their state is what it starts from
-__global__ __launch_bounds__(256) void empty_rays_kernel(const int32_t* __restrict__ offsets, int64_t rays, int d, const float* __restrict__ from, float* __restrict__ to) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t ray = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); ray < rays; ray += (int64_t)gridDim.x * 4)
-    if (offsets[ray + 1] <= offsets[ray])
-      for (int i = lane; i < d; i += 64) to[ray * d + i] = from ? from[ray * d + i] : 0.f;
 }
 
 // one more row of every ray: state[r] = a state[r] + b
@@ -565,7 +581,7 @@ ScanPlan plan_scan(int64_t rays, int64_t n_max, int d, int g, int vec) {
     p.lanes = g * p.slot * p.parts;
   }
   if (use_runs(rays, n_max, d)) {
-    p.run_rows = n_max * p.lanes / (128 * 1024);  // two waves a SIMD
+    p.run_rows = n_max * p.lanes / (128 * 1024);  // two waves a SIMD (four: each reading 1 to 3 us shorter, the prefix 6 us longer)
     p.run_rows = (p.run_rows + kBlock - 1) / kBlock * kBlock;
     if (p.run_rows < 4 * kBlock) p.run_rows = 4 * kBlock;
     p.runs = (n_max + p.run_rows - 1) / p.run_rows;
@@ -601,7 +617,7 @@ int launch_scan(ScanArgs a, bool bwd, char* ws, hipStream_t st) {
     if (bwd) scan_bwd_kernel<T, GATE, VEC, SHARED, true><<<grid, kScanThreads, 0, st>>>(a);
     else scan_fwd_kernel<T, GATE, VEC, SHARED, true><<<grid, kScanThreads, 0, st>>>(a);
     GFN_CHECK_LAUNCH();
-    run_prefix_kernel<<<(unsigned)((a.d + 3) / 4), 1024, 0, st>>>(a.agg, p.runs, a.d);
+    run_prefix_kernel<<<(unsigned)a.d, 64 * kPrefixWaves, 0, st>>>(a.agg, p.runs);
     GFN_CHECK_LAUNCH();
   }
   if (bwd) scan_bwd_kernel<T, GATE, VEC, SHARED, false><<<grid, kScanThreads, 0, st>>>(a);
@@ -610,12 +626,6 @@ int launch_scan(ScanArgs a, bool bwd, char* ws, hipStream_t st) {
   if (bwd && p.parts > 1 && a.n_max > 0) {
     const int64_t groups = (a.n_max * a.g + 255) / 256;
     scan_gate_sums_kernel<T><<<(unsigned)(groups < 4096 ? groups : 4096), 256, 0, st>>>(a, a.partial, p.parts);
-    GFN_CHECK_LAUNCH();
-  }
-  float* to = bwd ? a.dh0 : a.state;
-  if (p.run_rows && to) {  // a walk along a ray sees to an empty ray itself
-    const int64_t groups = (a.rays + 3) / 4;
-    empty_rays_kernel<<<(unsigned)(groups < 512 ? groups : 512), 256, 0, st>>>(a.offsets, a.rays, a.d, bwd ? a.d_state : a.h0, to);
     GFN_CHECK_LAUNCH();
   }
   return GFN_OK;
