@@ -182,8 +182,8 @@ constexpr int bwd_pad(int size) { return size == 4 ? 64 : 16; }
 constexpr int bwd_lds(int size, int ks, int np, int buffers) {
   return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * 64 * size + bwd_pad(size)) + 32;
 }
-// Pairs whose dz are kept: all of them (one barrier a tile before dW's product, which then reads x once for all pairs), or two (a
-// barrier a pair) or one (two), whichever still fits and does not cost the CU its second workgroup.
+// Pairs of feature tiles whose dz are kept at once, all, two or one, as many as fit without costing the CU its second workgroup: dW's product
+// reads x once for them, between two barriers.
 constexpr int bwd_buffers(int size, int ks, int np) {
   const int room = bwd_lds(size, ks, np, 1) <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
   return bwd_lds(size, ks, np, np) <= room ? np : np > 2 && bwd_lds(size, ks, np, 2) <= room ? 2 : 1;
@@ -237,47 +237,33 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
   const int width = h - h0 < HB ? h - h0 : HB;
   const int cut = cut_piece<T>(k), dh_cut = cut_piece<T>(width);
   constexpr int IN_FLIGHT = 3;  // reads from LDS ahead of the products
-  constexpr bool AHEAD = KS < 4;  // the next tile's x and dh are requested under this one's work, where registers are left for them
-  u32x4 xr[KS], xn[AHEAD ? KS : 1], dr[NP][DP], dn[AHEAD ? NP : 1][DP];
-  auto fetch_x = [&](int64_t s, u32x4& to, int u) { to = s < n ? piece_request(x + s * a.ldx, 4 * u + kg, k) : u32x4{0u, 0u, 0u, 0u}; };
-  auto fetch_dh = [&](int64_t s, u32x4 (&to)[DP], int p) {
-#pragma unroll
-    for (int q = 0; q < DP; q++) to[q] = s < n ? piece_request(dh + s * a.lddh + h0, (32 * p + 8 * kg) / E + q, width) : u32x4{0u, 0u, 0u, 0u};
-  };
+  constexpr bool HELD = KS < 4;   // this tile's x stays in registers as well; else the projections read it from LDS
+  u32x4 xr[KS], xn[KS], dr[NP][DP], dn[NP][DP];
   auto fetch = [&](int64_t tile) {
-    if constexpr (AHEAD) {
-      const int64_t s = tile * SAMPLES + wave * 16 + j;
+    const int64_t s = tile * SAMPLES + wave * 16 + j;
 #pragma unroll
-      for (int u = 0; u < KS; u++) fetch_x(s, xn[u], u);
+    for (int u = 0; u < KS; u++) xn[u] = s < n ? piece_request(x + s * a.ldx, 4 * u + kg, k) : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int p = 0; p < NP; p++) fetch_dh(s, dn[p], p);
-    }
+    for (int p = 0; p < NP; p++)
+#pragma unroll
+      for (int q = 0; q < DP; q++)
+        dn[p][q] = s < n ? piece_request(dh + s * a.lddh + h0, (32 * p + 8 * kg) / E + q, width) : u32x4{0u, 0u, 0u, 0u};
   };
   if ((int64_t)blockIdx.x < tiles) fetch(blockIdx.x);
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int64_t s = tile * SAMPLES + wave * 16 + j;
 #pragma unroll
     for (int u = 0; u < KS; u++) {
-      if constexpr (AHEAD) xr[u] = xn[u];
-      else fetch_x(s, xr[u], u);
-    }
-#pragma unroll
-    for (int p = 0; p < NP; p++) {
-      if constexpr (AHEAD) {
-#pragma unroll
-        for (int q = 0; q < DP; q++) dr[p][q] = dn[p][q];
-      } else {
-        fetch_dh(s, dr[p], p);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < KS; u++)
+      xr[u] = xn[u];
       if (u == cut >> 2 && kg == (cut & 3)) xr[u] = piece_shift<T>(xr[u], k);
+    }
 #pragma unroll
     for (int p = 0; p < NP; p++)
 #pragma unroll
-      for (int q = 0; q < DP; q++)
+      for (int q = 0; q < DP; q++) {
+        dr[p][q] = dn[p][q];
         if (p == dh_cut >> (DP + 1) && DP * kg + q == (dh_cut & (4 * DP - 1))) dr[p][q] = piece_shift<T>(dr[p][q], width);
+      }
     __syncthreads();  // the weights are staged (first tile); the tile before has been read from xs, zs and top
 #pragma unroll
     for (int u = 0; u < KS; u++) *reinterpret_cast<u32x4*>(xs + (wave * 16 + j) * ROW + u * 64 + kg * 16) = xr[u];
@@ -314,18 +300,17 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         run_e = e;
       }
     }
-    // dW's rows of the pairs p0 .. p0 + PN - 1 += their dz^T x over the tile's samples, and db their sums
-    auto product = [&](int p0, auto pairs_c) {
-      constexpr int PN = decltype(pairs_c)::value;
-      f32x4 total[PN];  // the same in every column
+    // dW's rows of the pairs p0 .. p0 + NB - 1 += their dz^T x over the tile's samples, and db their sums
+    auto product = [&](int p0) {
+      f32x4 total[NB];  // the same in every column
 #pragma unroll
-      for (int i = 0; i < PN; i++) total[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < NB; i++) total[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       if constexpr (sizeof(T) == 2) {
         // 32 samples at a time, in the order 4 kg .. + 3, 16 + 4 kg .. + 3: a read covers 16 rows, on different banks
         const char* r = zs + (4 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
         const char* q = xs + (4 * kg + (j >> 2)) * ROW + 8 * (j & 3) + 32 * kt0;
         constexpr uint32_t one = __is_same(T, __bf16) ? 0x3f803f80u : 0x3c003c00u;
-        u32x4 av[PN];
+        u32x4 av[NB];
         read_ahead<SAMPLES / 32 * KT_WAVE, IN_FLIGHT>(
             [&](int i) {
               const char* e = q + 32 * (i / KT_WAVE) * ROW + 32 * (i % KT_WAVE);
@@ -335,9 +320,9 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
             [&](int i, const u32x4& b) {
               const int c = i / KT_WAVE, t = i % KT_WAVE;
 #pragma unroll
-              for (int o = 0; o < PN; o++) {
+              for (int o = 0; o < NB; o++) {
                 if (t == 0) {
-                  const char* e = r + 32 * c * ZROW + (p0 + o) % NB * ZTILE;
+                  const char* e = r + 32 * c * ZROW + o * ZTILE;
                   const u32x2 lo = tr4(e), hi = tr4(e + 16 * ZROW);
                   av[o] = u32x4{lo[0], lo[1], hi[0], hi[1]};
                   total[o] = mma(av[o], u32x4{one, one, one, one}, total[o], (T*)nullptr);
@@ -346,26 +331,31 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
               }
             });
       } else {
+        float sum[NB];
+#pragma unroll
+        for (int o = 0; o < NB; o++) sum[o] = 0.f;
 #pragma unroll 4
         for (int c = 0; c < SAMPLES; c += 4) {
           const char* q = xs + (c + kg) * ROW + j * 4;
-          float av[PN];
+          float av[NB];
 #pragma unroll
-          for (int o = 0; o < PN; o++) {
-            av[o] = *reinterpret_cast<const float*>(zs + (c + kg) * ZROW + (p0 + o) % NB * ZTILE + (16 * ft + j) * 4);
-            total[o] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[o], 1.f, total[o], 0, 0, 0);
+          for (int o = 0; o < NB; o++) {
+            av[o] = *reinterpret_cast<const float*>(zs + (c + kg) * ZROW + o * ZTILE + (16 * ft + j) * 4);
+            sum[o] += av[o];
           }
 #pragma unroll
           for (int t = 0; t < KT_WAVE; t++)
             if (KT % FT_WAVES == 0 || kt0 + t < KT) {
               const float b = *reinterpret_cast<const float*>(q + 64 * (kt0 + t));
 #pragma unroll
-              for (int o = 0; o < PN; o++) dw[p0 + o][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[o], b, dw[p0 + o][t], 0, 0, 0);
+              for (int o = 0; o < NB; o++) dw[p0 + o][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[o], b, dw[p0 + o][t], 0, 0, 0);
             }
         }
+#pragma unroll
+        for (int o = 0; o < NB; o++) total[o] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum[o], 1.f, total[o], 0, 0, 0);
       }
 #pragma unroll
-      for (int o = 0; o < PN; o++)
+      for (int o = 0; o < NB; o++)
 #pragma unroll
         for (int i = 0; i < 4; i++) db[i] = j == p0 + o ? db[i] + total[o][i] : db[i];
     };
@@ -379,9 +369,13 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
       for (int m = 0; m < 2; m++)
 #pragma unroll
         for (int t = 0; t < 2; t++) acc[m][t] = *reinterpret_cast<const f32x4*>(bias + m * HB + 32 * p + 16 * t + 4 * kg);
+      u32x4 xb[2];
       read_ahead<4 * KS, IN_FLIGHT>(
-          [&](int i) { return *reinterpret_cast<const u32x4*>(wrow + (((i >> 1) & 1) * HB + 32 * p + 16 * (i & 1)) * ROW + (i >> 2) * 64); },
-          [&](int i, const u32x4& w) { acc[(i >> 1) & 1][i & 1] = mma(w, xr[i >> 2], acc[(i >> 1) & 1][i & 1], (T*)nullptr); });
+          [&](int i) {
+            if (!HELD && i % 4 == 0) xb[i >> 2 & 1] = *reinterpret_cast<const u32x4*>(xs + (wave * 16 + j) * ROW + (i >> 2) * 64 + kg * 16);
+            return *reinterpret_cast<const u32x4*>(wrow + ((i >> 1 & 1) * HB + 32 * p + 16 * (i & 1)) * ROW + (i >> 2) * 64);
+          },
+          [&](int i, const u32x4& w) { acc[i >> 1 & 1][i & 1] = mma(w, HELD ? xr[i >> 2] : xb[i >> 2 & 1], acc[i >> 1 & 1][i & 1], (T*)nullptr); });
       T z[2][8];
       float d[8];
 #pragma unroll
@@ -412,21 +406,17 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         }
       }
       if (a.part) {
-        if (NB == 1 && p) __syncthreads();  // the pair before has been read; of two buffers, the one before that
+        if (p && p % NB == 0) __syncthreads();  // the pairs before have been read
         char* zr = zs + (wave * 16 + j) * ZROW + p % NB * ZTILE + 8 * kg * sizeof(T);
         __builtin_memcpy(__builtin_assume_aligned(zr, 16), z[0], sizeof(z[0]));
         __builtin_memcpy(__builtin_assume_aligned(zr + 32 * sizeof(T), 16), z[1], sizeof(z[1]));
-        if constexpr (NB < NP) {
+        if (p % NB == NB - 1) {
           __syncthreads();
-          product(p, Constant<1>{});
+          product(p - NB + 1);
         }
       }
     }
-    if (NB == NP && a.part) {
-      __syncthreads();
-      product(0, Constant<NP>{});
-    }
-    if constexpr (AHEAD) loads_done();
+    loads_done();
     if ((a.dx || a.dx_sum) && s < n) {  // lane (j, kg) holds columns 16 t + 4 kg + r of sample j
 #pragma unroll
       for (int t = 0; t < KT; t++) {
