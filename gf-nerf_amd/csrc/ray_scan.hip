@@ -562,10 +562,12 @@ bool two_channels(const ScanArgs& a, bool shared, bool bwd) {
   return strides % 2 == 0 && at % 4 == 0;
 }
 
-// Rays or runs: a lane a ray as long as that fills the chip with walks that are not too long to wait for.
+// Rays or runs.  A walk along a ray waits 0.27 us a row where rays do not fill the chip; runs read everything twice and stop at every ray's
+// beginning.  us, bf16 forward, runs / rays: 16 rays x 2048 rows x 32 channels 19 / 453, 512 x 512 x 128 87 / 139, 1024 x 192 x 64 58 / 55,
+// 512 x 128 x 64 33 / 37, 1024 x 100 x 8 42 / 31, 2048 x 128 x 32 65 / 40, 4096 x 192 x 128 245 / 154.
 bool use_runs(int64_t rays, int64_t n_max, int d) {
   const int64_t mean = rays > 0 ? n_max / rays : 0;
-  return n_max > 0 && mean > 64 && rays * d < 64 * 1024;
+  return mean >= 96 && rays < 6 * mean && rays * d < 128 * 1024;
 }
 
 struct ScanPlan {
@@ -587,6 +589,12 @@ ScanPlan plan_scan(int64_t rays, int64_t n_max, int d, int g, int vec) {
     p.runs = (n_max + p.run_rows - 1) / p.run_rows;
   }
   return p;
+}
+// Two waves a SIMD with `vec` channels a lane: wider loads pay from there on (two channels / one, us, bf16 forward: 4096 rays x 192 rows x 128
+// channels 154 / 170, 2 x 131072 x 64 45 / 50; below, 512 x 128 x 64 41 / 33, 4096 x 128 x 8 52 / 40).
+bool enough_lanes(const ScanArgs& a, int vec) {
+  const ScanPlan p = plan_scan(a.rays, a.n_max, a.d, a.g, vec);
+  return (p.run_rows ? p.runs : a.rays) * p.lanes >= 128 * 1024;
 }
 // workspace: the runs' steps, df's sums over parts of gates
 int64_t scan_workspace(int64_t rays, int64_t n_max, int d, int g) {
@@ -635,7 +643,7 @@ template <typename T, int GATE>
 int dispatch_vec(const ScanArgs& a, bool bwd, char* ws, hipStream_t st) {
   const bool shared = a.g != a.d;
   if constexpr (sizeof(T) == 2) {  // two 16-bit channels a lane; f32: one is 256 bytes a wave already
-    if (two_channels(a, shared, bwd)) return shared ? launch_scan<T, GATE, 2, true>(a, bwd, ws, st) : launch_scan<T, GATE, 2, false>(a, bwd, ws, st);
+    if (two_channels(a, shared, bwd) && enough_lanes(a, 2)) return shared ? launch_scan<T, GATE, 2, true>(a, bwd, ws, st) : launch_scan<T, GATE, 2, false>(a, bwd, ws, st);
   }
   return shared ? launch_scan<T, GATE, 1, true>(a, bwd, ws, st) : launch_scan<T, GATE, 1, false>(a, bwd, ws, st);
 }

@@ -294,6 +294,26 @@ def test_ray_scan_of_a_batch_of_rays(T, ops, kind, d, g):
         assert rel <= (2e-6 if got.dtype == T.float32 else oseq.HALF[kind]), (name, rel)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d,g", [(96, 96), (32, 1), (10, 5), (256, 2)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_ray_scan_in_runs_with_many_rays_in_each(T, ops, kind, d, g, reverse):
+    """Rays too few to fill the chip and long on average, but most of them short: runs of rows that several rays begin and end in, rays without
+    rows among, before and behind them."""
+    rng = np.random.default_rng(11)
+    lens = np.where(rng.random(90) < 0.7, rng.integers(0, 9, 90), rng.integers(200, 700, 90))
+    lens[:3], lens[-2:], lens[40:44] = 0, 0, (1, 0, 0, 8)
+    assert lens.sum() > 100 * len(lens)
+    offt, off, f, c, dh, h0, ds = scan_inputs(T, kind, lens, d, g, "sigmoid")
+    want = oseq.ray_scan(off, f[1], c[1], "sigmoid", reverse, kind, h0[1], dh[1], ds[1])
+    r = ops.ray_scan_fwd(offt, f[0], c[0], reverse=reverse, h0=h0[0], save=True)
+    close(r["h"], want["h"], "h")
+    close(r["state"], want["state"], "state")
+    b = ops.ray_scan_bwd(offt, f[0], c[0], dh[0], r["saved"], reverse=reverse, h0=h0[0], d_state=ds[0])
+    for name in ("df", "dc", "dh0"):
+        close(b[name], want[name], name)
+
+
 def test_ray_scan_composites_like_the_renderer(T, ops):
     """Back to front with the density's gate the recurrence is the framework's own compositing: three channels against gfn_composite_fwd / _bwd."""
     rng = np.random.default_rng(5)
