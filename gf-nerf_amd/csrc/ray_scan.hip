@@ -198,9 +198,10 @@ struct Rows {
       for (int r = 0; r < kBlock; r++) to[r] = __builtin_nontemporal_load(reinterpret_cast<const R*>(from + clamp_row(asc ? row0 + r : row0 - r, s, e - 1) * ld));
     }
   }
+  template <bool INNER>
   __device__ __forceinline__ void load(const ScanArgs& a, const T* pf, const T* pc, const T* pd, int64_t base, bool asc, int64_t s, int64_t e, int deal) {
     const int64_t row0 = base + (asc ? 0 : kBlock - 1);
-    const bool whole = __all(base >= s && base + kBlock <= e);
+    const bool whole = INNER || __all(base >= s && base + kBlock <= e);
     if (SHARED && deal >= 0) fd = pf[clamp_row(asc ? row0 + deal : row0 - deal, s, e - 1) * a.ldf];
     else column(f, pf, a.ldf, row0, asc, whole, s, e);
     if constexpr (!(BWD && AGG)) column(c, pc, a.ldc, row0, asc, whole, s, e);
@@ -239,6 +240,18 @@ struct Gates {
     }
   }
 };
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+// Whether this block and the next are whole rows of the piece in every lane, with one more behind them.  Such blocks are worked on without
+// a branch, so that a wait for the next block's rows is not one for the stores behind their requests (loads and stores are counted together,
+// in order): backward of 4096 rays x 192 rows x 128 channels in bf16 255 -> 237 us, a first reading 21 -> 19 and 20 -> 18 us.
+template <typename F>
+__device__ __forceinline__ bool inner(int64_t i, int64_t blocks, int64_t lo, int64_t hi, F base_of, bool active) {
+  if (!__all(active && i + 2 < blocks)) return false;
+  const int64_t p = base_of(i), q = base_of(i + 1);
+  return __all(p >= lo && p + kBlock <= hi && q >= lo && q + kBlock <= hi);
+}
 
 // Walks along runs never meet a ray without rows: its last state is the one it starts with (its adjoint likewise).
 __device__ __forceinline__ void empty_rays(const ScanArgs& a, const float* __restrict__ from, float* __restrict__ to) {
@@ -281,15 +294,16 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
     const int64_t b0 = lo / kBlock, blocks = hi > lo ? (hi - 1) / kBlock - b0 + 1 : 0;
     Rows<T, VEC, SHARED, false, AGG> now, next;
     auto base_of = [&](int64_t i) { return (asc ? b0 + i : b0 + blocks - 1 - i) * kBlock; };
-    if (blocks) now.load(a, f, c, nullptr, base_of(0), asc, lo, hi, deal);
-    for (int64_t i = 0; i < blocks; i++) {
+    if (blocks) now.template load<false>(a, f, c, nullptr, base_of(0), asc, lo, hi, deal);
+    auto work = [&](int64_t i, auto inner_c) {
+      constexpr bool INNER = decltype(inner_c)::value;
       const int64_t base = base_of(i), row0 = base + (asc ? 0 : kBlock - 1);
-      if (i + 1 < blocks) next.load(a, f, c, nullptr, base_of(i + 1), asc, lo, hi, deal);
-      if (!AGG && a.saved && at.active && row0 >= lo && row0 < hi)
+      if (!AGG && a.saved && (INNER || (at.active && row0 >= lo && row0 < hi)))
 #pragma unroll
         for (int v = 0; v < VEC; v++) a.saved[base / kBlock * a.d + at.ch + v] = s[v];
+      if (INNER || i + 1 < blocks) next.template load<INNER>(a, f, c, nullptr, base_of(i + 1), asc, lo, hi, deal);
       gates.begin(now.fd);
-      const bool whole = __all(base >= lo && base + kBlock <= hi && at.active);
+      const bool whole = INNER || __all(base >= lo && base + kBlock <= hi && at.active);
       T* out = h + row0 * a.ldh;
       const int64_t step = asc ? a.ldh : -a.ldh;
 #pragma unroll
@@ -311,7 +325,12 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
           else if (in && at.active) *reinterpret_cast<V*>(out + r * step) = o;
         }
       }
-      if (i + 1 < blocks) now = next;
+      if (INNER || i + 1 < blocks) now = next;
+    };
+    for (int64_t i = 0; i < blocks; i++) {
+      if constexpr (AGG)  // (writing h as well it costs a wave a SIMD: 180 instead of 158 us for 4096 rays x 192 rows x 128 channels, bf16)
+        for (; inner(i, blocks, lo, hi, base_of, at.active); i++) work(i, Yes{});
+      work(i, No{});
     }
     if (!AGG && ends && a.state && at.active)
 #pragma unroll
@@ -357,21 +376,34 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
     const int64_t b0 = lo / kBlock, blocks = hi > lo ? (hi - 1) / kBlock - b0 + 1 : 0;
     Rows<T, VEC, SHARED, true, AGG> now, next;
     auto base_of = [&](int64_t i) { return (asc ? b0 + i : b0 + blocks - 1 - i) * kBlock; };
-    if (blocks) now.load(a, f, c, dh, base_of(0), asc, lo, hi, deal);
-    for (int64_t i = 0; i < blocks; i++) {
-      const int64_t base = base_of(i), row0 = base + (asc ? 0 : kBlock - 1);
-      const bool ray_starts = ends && i == blocks - 1;  // the recurrence's first row of the ray is in this block
-      float before[AGG ? 1 : kBlock][VEC], st[VEC];
-      if (!AGG) {
-        const int64_t first = asc ? hi - 1 : lo;  // the recurrence's first row of the piece, in its last block
+    float entry[VEC];  // the state in front of the next block's rows (in the recurrence's order), requested with them
+    auto enter = [&](int64_t i, auto inner_c) {
+      if constexpr (!AGG) {
+        const bool ray_starts = !decltype(inner_c)::value && ends && i == blocks - 1;  // the recurrence's first row of the ray is in this block
+        const int64_t base = base_of(i), first = asc ? hi - 1 : lo;                       // the recurrence's first row of the piece, in its last block
         const float* from = ray_starts ? a.h0 : a.saved_in;
         const int64_t of = ray_starts ? ray : (asc ? (base + kBlock - 1 < first ? base + kBlock - 1 : first) : (base > first ? base : first)) / kBlock;
 #pragma unroll
-        for (int v = 0; v < VEC; v++) st[v] = from ? from[of * a.d + at.ch + v] : 0.f;
+        for (int v = 0; v < VEC; v++) entry[v] = decltype(inner_c)::value || from ? from[of * a.d + at.ch + v] : 0.f;
       }
-      if (i + 1 < blocks) next.load(a, f, c, dh, base_of(i + 1), asc, lo, hi, deal);
+    };
+    if (blocks) {
+      now.template load<false>(a, f, c, dh, base_of(0), asc, lo, hi, deal);
+      enter(0, No{});
+    }
+    auto work = [&](int64_t i, auto inner_c) {
+      constexpr bool INNER = decltype(inner_c)::value;
+      const int64_t base = base_of(i), row0 = base + (asc ? 0 : kBlock - 1);
+      float before[AGG ? 1 : kBlock][VEC], st[VEC];
+      if (!AGG)
+#pragma unroll
+        for (int v = 0; v < VEC; v++) st[v] = entry[v];
+      if (INNER || i + 1 < blocks) {
+        next.template load<INNER>(a, f, c, dh, base_of(i + 1), asc, lo, hi, deal);
+        enter(i + 1, inner_c);
+      }
       gates.begin(now.fd);
-      const bool whole = __all(base >= lo && base + kBlock <= hi && at.active);
+      const bool whole = INNER || __all(base >= lo && base + kBlock <= hi && at.active);
       float x[kBlock][VEC], y[kBlock][VEC];
 #pragma unroll
       for (int r = kBlock - 1; r >= 0; r--) {  // the recurrence's order
@@ -451,7 +483,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
             }
           }
       }
-      if (i + 1 < blocks) now = next;
+      if (INNER || i + 1 < blocks) now = next;
+    };
+    for (int64_t i = 0; i < blocks; i++) {
+      for (; inner(i, blocks, lo, hi, base_of, at.active); i++) work(i, Yes{});
+      work(i, No{});
     }
     if (!AGG && ends && a.dh0 && at.active)
 #pragma unroll
