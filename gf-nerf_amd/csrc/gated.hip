@@ -15,8 +15,15 @@
 // One pass: x and dh are read once, dx is written once; each workgroup's partial dW goes to a workspace and a second launch adds the
 // partials in a fixed order (no atomics: the same bits every run).  The biases' gradients are the same product against a column of ones
 // and travel as column k of the partials.
-// dz is rounded to the operands' type for the two products -- 2^-9 (bf16) / 2^-12 (f16) per term, below the rounding of the results
-// themselves; f32 stays f32.  f16 has the precision but not the range: see tile_scale.
+// dz is rounded to the operands' type for the two products -- half a step, 2^-8 (bf16) / 2^-11 (f16) of each term, what the matrix unit's
+// operands ask for, as the results' own rounding; f32 stays f32.  f16 has the precision but not the range: see tile_scale_exponent.
+//
+// What bounds them.  Forward, 786k x 63 -> 128 bf16 silu: 92 us for 300 MB (a copy of that size: 55); four waves a SIMD, requests a tile
+// ahead; relu takes as long, rows of 64 instead of 63 16 % less (odd rows start at any 2 bytes).  262k x 32 -> 128 f32 gelu: 66 us, of
+// which the matrix pipe is busy 27 (f32 products run at 1/8 of bf16's rate) and vector instructions issue for 30; the two hardly overlap.
+// Backward, 524k x 63 -> 128 bf16: 115 us and 7 for the reduction, 266 MB (a copy: 49).  Two waves a SIMD (W's image, x, dz and dW's
+// accumulators fill LDS and registers); a tile's vector instructions (2.7 us of its 6.3), LDS reads (2.5) and products (1.4) add up rather
+// than overlap.  100k x 128 -> 128 f16: 61 + 13; 50k x 32 -> 64 f32: 29 + 5, 64 % of it the matrix pipe.
 #include "gated_device.h"
 
 namespace {
@@ -64,7 +71,8 @@ __device__ __forceinline__ void stage_bias(float* bias, const T* bg, const T* bu
   }
 }
 
-// workgroups of the forward that share a CU: registers for four, or for two where the rows are long
+// workgroups of the forward that share a CU: registers for four, or for two where the rows are long.  (A launch without the bound keeps its
+// accumulators apart from the vector registers and copies them: 117 us instead of 105 for 786k x 63 -> 128 bf16.)
 constexpr int fwd_per_cu(int ks) { return ks <= 2 ? 4 : 2; }
 
 template <typename T, int KS, int G>
@@ -173,7 +181,8 @@ __device__ __forceinline__ u32x2 tr4(const char* a) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a));
 }
 
-// waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit
+// waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit (two workgroups wait for
+// their barriers apart from each other)
 constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 
 // bytes behind a row of dz: the rows that one read covers start on different banks (16 rows of 8-byte pieces; f32: 2 rows of 64 bytes)
@@ -514,7 +523,8 @@ int launch_fwd(const GatedFwd& a, hipStream_t st) {
   constexpr int ROW = KS * 64 + 16;
   const int hp = (a.h + 31) & ~31;
   const int64_t tiles = (a.n_max + 16 * G * kWaves - 1) / (16 * G * kWaves);
-  // features a workgroup: all of them (x is read once) while there are samples enough for every CU, else blocks of 32
+  // features a workgroup: all of them (x is read once) while there are samples enough for every CU, else blocks of 32 (63 -> 128 bf16,
+  // blocks / all: 128 rows 4.3 / 7.5 us, 16384 7.3 / 9.4, 32768 11.4 / 10.2, 65536 20.5 / 14.4)
   int hc = hp < 128 ? hp : 128;
   if ((size_t)2 * hc * ROW > 80 * 1024) hc = 64;
   if (tiles < 256) hc = 32;
@@ -535,7 +545,9 @@ int launch_fwd(const GatedFwd& a, hipStream_t st) {
 template <typename T>
 int dispatch_fwd(const GatedFwd& a, hipStream_t st) {
   const int units = (a.k + 4 * Piece<T>::E - 1) / (4 * Piece<T>::E);
-  const bool few = a.n_max < 16384;  // a sample group a wave: more workgroups
+  // one group of 16 samples a wave or two (each weight read once for both): us for 63 -> 128 bf16, one / two: 4096 rows 4.5 / 5.3, 16384
+  // 7.4 / 7.3, 32768 13.6 / 11.4
+  const bool few = a.n_max < 16384;
 #define GFN_GATED(KS, G)                                                             \
   if (units <= KS) return few ? launch_fwd<T, KS, 1>(a, st) : launch_fwd<T, KS, G>(a, st)
   GFN_GATED(1, 2);
