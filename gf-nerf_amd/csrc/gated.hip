@@ -105,45 +105,46 @@ __global__ __launch_bounds__(64 * kWaves, fwd_per_cu(KS)) void gated_fwd_kernel(
   };
   if (s0 < n) fetch(next, s0);
   auto pass = [&](auto act_c) {
-  for (; s0 < n; s0 += stride) {
+    for (; s0 < n; s0 += stride) {
 #pragma unroll
-    for (int g = 0; g < G; g++)
+      for (int g = 0; g < G; g++)
 #pragma unroll
-      for (int u = 0; u < KS; u++) {
-        xr[g][u] = next[g][u];
-        if (u == cut >> 2 && kg == (cut & 3)) xr[g][u] = piece_shift<T>(next[g][u], k);
-      }
-    if (s0 + stride < n) fetch(next, s0 + stride);  // on its way under this tile's work
-    for (int p = 0; p < pairs; p++) {
-      f32x4 acc[2][2][G];  // [matrix][tile]
-#pragma unroll
-      for (int m = 0; m < 2; m++)
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          const f32x4 b = *reinterpret_cast<const f32x4*>(bias + m * hc + 32 * p + 16 * t + 4 * kg);
-#pragma unroll
-          for (int g = 0; g < G; g++) acc[m][t][g] = b;
+        for (int u = 0; u < KS; u++) {
+          xr[g][u] = next[g][u];
+          if (u == cut >> 2 && kg == (cut & 3)) xr[g][u] = piece_shift<T>(next[g][u], k);
         }
-#pragma unroll
-      for (int u = 0; u < KS; u++)
+      if (s0 + stride < n) fetch(next, s0 + stride);  // on its way under this tile's work
+      for (int p = 0; p < pairs; p++) {
+        f32x4 acc[2][2][G];  // [matrix][tile]
 #pragma unroll
         for (int m = 0; m < 2; m++)
 #pragma unroll
           for (int t = 0; t < 2; t++) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(wrow + (m * hc + 32 * p + 16 * t) * ROW + u * 64);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(bias + m * hc + 32 * p + 16 * t + 4 * kg);
 #pragma unroll
-            for (int g = 0; g < G; g++) acc[m][t][g] = mma(w, xr[g][u], acc[m][t][g], (T*)nullptr);
+            for (int g = 0; g < G; g++) acc[m][t][g] = b;
           }
-      const int f = h0 + 32 * p + 8 * kg;
 #pragma unroll
-      for (int g = 0; g < G; g++) {
-        const int64_t s = s0 + 16 * g + j;
-        float v[8];
-        gated8<decltype(act_c)::value, EXACT>([&](int i) { return acc[0][i >> 2][g][i & 3]; }, [&](int i) { return acc[1][i >> 2][g][i & 3]; }, v);
-        if (s < n) store_row<T, 8>(out + s * ldo + f, h - f, v);
+        for (int u = 0; u < KS; u++)
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+              const u32x4 w = *reinterpret_cast<const u32x4*>(wrow + (m * hc + 32 * p + 16 * t) * ROW + u * 64);
+#pragma unroll
+              for (int g = 0; g < G; g++) acc[m][t][g] = mma(w, xr[g][u], acc[m][t][g], (T*)nullptr);
+            }
+        const int f = h0 + 32 * p + 8 * kg;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          const int64_t s = s0 + 16 * g + j;
+          float v[8];
+          gated8<decltype(act_c)::value, EXACT>([&](int i) { return acc[0][i >> 2][g][i & 3]; }, [&](int i) { return acc[1][i >> 2][g][i & 3]; }, v);
+          if (s < n) store_row<T, 8>(out + s * ldo + f, h - f, v);
+        }
       }
     }
-  }  };
+  };
   for_act(act, pass);
 }
 
@@ -181,8 +182,9 @@ __device__ __forceinline__ u32x2 tr4(const char* a) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a));
 }
 
-// waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit (two workgroups wait for
-// their barriers apart from each other)
+// waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit and wait for their
+// barriers apart from each other (us, eight / four: 524k x 63 -> 128 bf16 178 / 150, 262k x 96 -> 128 bf16 93 / 148, 100k x 128 -> 128
+// f16 76 / 87)
 constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 
 // bytes behind a row of dz: the rows that one read covers start on different banks (16 rows of 8-byte pieces; f32: 2 rows of 64 bytes)
@@ -192,7 +194,7 @@ constexpr int bwd_lds(int size, int ks, int np, int buffers) {
   return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * 64 * size + bwd_pad(size)) + 32;
 }
 // Pairs of feature tiles whose dz are kept at once, all, two or one, as many as fit without costing the CU its second workgroup: dW's product
-// reads x once for them, between two barriers.
+// reads x once for them, between two barriers.  (As many / one at a time: 524k x 63 -> 128 bf16 150 / 161 us, 100k x 48 -> 128 f32 134 / 146.)
 constexpr int bwd_buffers(int size, int ks, int np) {
   const int room = bwd_lds(size, ks, np, 1) <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
   return bwd_lds(size, ks, np, np) <= room ? np : np > 2 && bwd_lds(size, ks, np, 2) <= room ? 2 : 1;
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
   char* xs = lds + 2 * HB * ROW;        // [SAMPLES][ROW]
   char* zs = xs + SAMPLES * ROW;        // [SAMPLES][NB][dg 32 | du 32]
   float* bias = reinterpret_cast<float*>(zs + SAMPLES * ZROW);  // [2][HB]
-  float* top = bias + 2 * HB;                                                 // [WAVES]
+  float* top = bias + 2 * HB;                                   // [WAVES]
   const T *x = static_cast<const T*>(a.x), *dh = static_cast<const T*>(a.dh);
   const bool biased = a.bg != nullptr;
   const int k = a.k, h = a.h, h0 = a.h0, act = a.act;
@@ -234,10 +236,9 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
   const int ft = wave & 3, kt0 = (wave >> 2) * KT_WAVE;
   f32x4 dw[NP][KT_WAVE], db = {0.f, 0.f, 0.f, 0.f};  // db: the sums of dz itself, pair p's in column p
 #pragma unroll
-  for (int p = 0; p < NP; p++) {
+  for (int p = 0; p < NP; p++)
 #pragma unroll
     for (int t = 0; t < KT_WAVE; t++) dw[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
   const bool sums = biased && wave < 4;  // one wave for each row tile
   int run_e = 0;  // dw holds the sums times 2^run_e
   const char* wrow = lds + j * ROW + kg * 16;

@@ -37,7 +37,8 @@ def ray_scan(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None):
 def render_features(pts_offsets, sigma, dt, features):
     """Composite `features` [n, channels] along each ray with the weights T_i alpha_i, alpha = 1 - exp(-sigma dt) (RaySamples.get_weights_f2nerf,
     nerfstudio/cameras/rays.py:178-200) -> f32 [rays, channels]; gradients for sigma, dt and features.  The sum over a ray is the recurrence
-    h = exp(-sigma dt) h + alpha c taken back to front: no weights array, any number of channels."""
+    h = exp(-sigma dt) h + alpha c taken back to front: no weights array, any number of channels.  sigma dt is formed in f32 and rounded once
+    to the features' dtype (the recurrence takes its gates and inputs in one type): with 16-bit features a weight is off by half a step of it."""
     thickness = (sigma.reshape(-1) * dt.reshape(-1)).to(features.dtype)
     return ray_scan(pts_offsets, thickness[:, None], features, "decay", reverse=True)[1]
 
