@@ -15,15 +15,16 @@
 // One pass: x and dh are read once, dx is written once; each workgroup's partial dW goes to a workspace and a second launch adds the
 // partials in a fixed order (no atomics: the same bits every run).  The biases' gradients are the same product against a column of ones
 // and travel as column k of the partials.
-// dz is rounded to the operands' type for the two products -- half a step, 2^-8 (bf16) / 2^-11 (f16) of each term, what the matrix unit's
-// operands ask for, as the results' own rounding; f32 stays f32.  f16 has the precision but not the range: see tile_scale_exponent.
+// 16-bit: dz goes into both products as two operands, its rounding to the type and the rounding of what that left, so nothing of it is
+// lost beside the results' own rounding (one operand: errors of 2.4e-3 instead of 1.7e-3 of the norm in bf16 -- what one rounding of the
+// results leaves -- and 115 instead of 145 us in the case below).  f16 has the precision but not the range: see tile_scale_exponent.
 //
 // What bounds them.  Forward, 786k x 63 -> 128 bf16 silu: 92 us for 300 MB (a copy of that size: 55); four waves a SIMD, requests a tile
 // ahead; relu takes as long, rows of 64 instead of 63 16 % less (odd rows start at any 2 bytes).  262k x 32 -> 128 f32 gelu: 66 us, of
 // which the matrix pipe is busy 27 (f32 products run at 1/8 of bf16's rate) and vector instructions issue for 30; the two hardly overlap.
-// Backward, 524k x 63 -> 128 bf16: 115 us and 7 for the reduction, 266 MB (a copy: 49).  Two waves a SIMD (W's image, x, dz and dW's
-// accumulators fill LDS and registers); a tile's vector instructions (2.7 us of its 6.3), LDS reads (2.5) and products (1.4) add up rather
-// than overlap.  100k x 128 -> 128 f16: 61 + 13; 50k x 32 -> 64 f32: 29 + 5, 64 % of it the matrix pipe.
+// Backward, 524k x 63 -> 128 bf16: 145 us and 7 for the reduction, 266 MB (a copy: 49).  Two waves a SIMD (W's image, x, dz and dW's
+// accumulators fill LDS and registers); a tile's vector instructions, LDS reads and products, a third of its time each, add up rather
+// than overlap.  100k x 128 -> 128 f16: 76 + 13; 50k x 32 -> 64 f32: 29 + 5, 64 % of it the matrix pipe.
 #include "gated_device.h"
 
 namespace {
@@ -191,7 +192,7 @@ constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 constexpr int bwd_pad(int size) { return size == 4 ? 64 : 16; }
 // LDS of a workgroup of the backward with room for the dz of `buffers` pairs of feature tiles
 constexpr int bwd_lds(int size, int ks, int np, int buffers) {
-  return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * 64 * size + bwd_pad(size)) + 32;
+  return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * 256 + bwd_pad(size)) + 32;
 }
 // Pairs of feature tiles whose dz are kept at once, all, two or one, as many as fit without costing the CU its second workgroup: dW's product
 // reads x once for them, between two barriers.  (As many / one at a time: 524k x 63 -> 128 bf16 150 / 161 us, 100k x 48 -> 128 f32 134 / 146.)
@@ -218,12 +219,12 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
   constexpr int WAVES = bwd_waves(KS);
   constexpr int E = Piece<T>::E, TPU = sizeof(T) == 4 ? 1 : 2;  // 16-column tiles a unit
   constexpr int KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP, NB = bwd_buffers(sizeof(T), KS, NP);
-  constexpr int SAMPLES = 16 * WAVES, ZTILE = 64 * (int)sizeof(T), ZROW = NB * ZTILE + bwd_pad(sizeof(T));
+  constexpr int SAMPLES = 16 * WAVES, ZTILE = 256, ZROW = NB * ZTILE + bwd_pad(sizeof(T));
   constexpr int FT_WAVES = WAVES / 4, KT_WAVE = (KT + FT_WAVES - 1) / FT_WAVES;  // waves that share a row tile of dW, its column tiles a wave
   constexpr bool EXACT = sizeof(T) == 4, SCALED = sizeof(T) == 2 && !__is_same(T, __bf16);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* xs = lds + 2 * HB * ROW;        // [SAMPLES][ROW]
-  char* zs = xs + SAMPLES * ROW;        // [SAMPLES][NB][dg 32 | du 32]
+  char* zs = xs + SAMPLES * ROW;        // [SAMPLES][NB][dg 32 | du 32], 16-bit: the same of what their rounding left
   float* bias = reinterpret_cast<float*>(zs + SAMPLES * ZROW);  // [2][HB]
   float* top = bias + 2 * HB;                                   // [WAVES]
   const T *x = static_cast<const T*>(a.x), *dh = static_cast<const T*>(a.dh);
@@ -320,24 +321,33 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         const char* r = zs + (4 * kg + (j >> 2)) * ZROW + (16 * ft + 4 * (j & 3)) * 2;
         const char* q = xs + (4 * kg + (j >> 2)) * ROW + 8 * (j & 3) + 32 * kt0;
         constexpr uint32_t one = __is_same(T, __bf16) ? 0x3f803f80u : 0x3c003c00u;
-        u32x4 av[NB];
+        constexpr int DEEP = KS < 4 ? 2 : 1;  // dz of the next 32 samples requested with the last x of these, where registers are left for it
+        u32x4 av[DEEP][NB][2];
+        auto samples = [&](int c) {
+#pragma unroll
+          for (int o = 0; o < NB; o++)
+#pragma unroll
+            for (int q = 0; q < 2; q++) {  // dz's 16 bits, then what they left
+              const char* e = r + 32 * c * ZROW + o * ZTILE + 128 * q;
+              const u32x2 lo = tr4(e), hi = tr4(e + 16 * ZROW);
+              av[c % DEEP][o][q] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+            }
+        };
         read_ahead<SAMPLES / 32 * KT_WAVE, IN_FLIGHT>(
             [&](int i) {
+              if (DEEP == 2 && i % KT_WAVE == 0) samples(i / KT_WAVE);
               const char* e = q + 32 * (i / KT_WAVE) * ROW + 32 * (i % KT_WAVE);
               const u32x2 lo = tr4(e), hi = tr4(e + 16 * ROW);
               return u32x4{lo[0], lo[1], hi[0], hi[1]};
             },
             [&](int i, const u32x4& b) {
               const int c = i / KT_WAVE, t = i % KT_WAVE;
+              if (DEEP == 1 && t == 0) samples(c);
 #pragma unroll
               for (int o = 0; o < NB; o++) {
-                if (t == 0) {
-                  const char* e = r + 32 * c * ZROW + o * ZTILE;
-                  const u32x2 lo = tr4(e), hi = tr4(e + 16 * ZROW);
-                  av[o] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-                  total[o] = mma(av[o], u32x4{one, one, one, one}, total[o], (T*)nullptr);
-                }
-                dw[p0 + o][t] = mma(av[o], b, dw[p0 + o][t], (T*)nullptr);
+                const u32x4(&z)[2] = av[c % DEEP][o];
+                if (t == 0) total[o] = mma(z[0], u32x4{one, one, one, one}, mma(z[1], u32x4{one, one, one, one}, total[o], (T*)nullptr), (T*)nullptr);
+                dw[p0 + o][t] = mma(z[0], b, mma(z[1], b, dw[p0 + o][t], (T*)nullptr), (T*)nullptr);
               }
             });
       } else {
@@ -386,23 +396,33 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
             return *reinterpret_cast<const u32x4*>(wrow + ((i >> 1 & 1) * HB + 32 * p + 16 * (i & 1)) * ROW + (i >> 2) * 64);
           },
           [&](int i, const u32x4& w) { acc[i >> 1 & 1][i & 1] = mma(w, HELD ? xr[i >> 2] : xb[i >> 2 & 1], acc[i >> 1 & 1][i & 1], (T*)nullptr); });
-      T z[2][8];
-      float d[8];
+      float d[8], z[2][8];
 #pragma unroll
       for (int i = 0; i < 8; i++) d[i] = SCALED ? grad(p, i) * to : grad(p, i);
       for_act(act, [&](auto act_c) { gated8_grad<decltype(act_c)::value, EXACT>([&](int i) { return acc[0][i >> 2][i & 3]; }, [&](int i) { return acc[1][i >> 2][i & 3]; }, d, z[0], z[1]); });
+      T hi[2][8], lo[2][8];
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            hi[m][i] = (T)z[m][i];
+            lo[m][i] = (T)(z[m][i] - (float)hi[m][i]);
+          }
+      }
       if (a.dx || a.dx_sum) {  // dx[k] += sum over these 32 features
         if constexpr (sizeof(T) == 2) {
           // features 8 kg .. + 3 are image rows 4 kg .. + 3 of tile 0, the next four those of tile 1
           const char* r = lds + (32 * p + 4 * kg + (j >> 2)) * ROW + 8 * (j & 3);
-          const u32x4 b[2] = {__builtin_bit_cast(u32x4, z[0]), __builtin_bit_cast(u32x4, z[1])};
+          const u32x4 bh[2] = {__builtin_bit_cast(u32x4, hi[0]), __builtin_bit_cast(u32x4, hi[1])};
+          const u32x4 bl[2] = {__builtin_bit_cast(u32x4, lo[0]), __builtin_bit_cast(u32x4, lo[1])};
           read_ahead<2 * KT, IN_FLIGHT>(
               [&](int i) {
                 const char* q = r + (i / KT) * HB * ROW + 32 * (i % KT);
                 const u32x2 lo = tr4(q), hi = tr4(q + 16 * ROW);
                 return u32x4{lo[0], lo[1], hi[0], hi[1]};
               },
-              [&](int i, const u32x4& w) { dx[i % KT] = mma(w, b[i / KT], dx[i % KT], (T*)nullptr); });
+              [&](int i, const u32x4& w) { dx[i % KT] = mma(w, bh[i / KT], mma(w, bl[i / KT], dx[i % KT], (T*)nullptr), (T*)nullptr); });
         } else {
 #pragma unroll
           for (int m = 0; m < 2; m++)
@@ -411,15 +431,23 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
               const char* r = lds + (m * HB + 32 * p + 4 * kg + 16 * (i >> 2) + (i & 3)) * ROW;
 #pragma unroll
               for (int t = 0; t < KT; t++)
-                dx[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(*reinterpret_cast<const float*>(r + (16 * t + j) * 4), (float)z[m][i], dx[t], 0, 0, 0);
+                dx[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(*reinterpret_cast<const float*>(r + (16 * t + j) * 4), z[m][i], dx[t], 0, 0, 0);
             }
         }
       }
       if (a.part) {
         if (p && p % NB == 0) __syncthreads();  // the pairs before have been read
         char* zr = zs + (wave * 16 + j) * ZROW + p % NB * ZTILE + 8 * kg * sizeof(T);
-        __builtin_memcpy(__builtin_assume_aligned(zr, 16), z[0], sizeof(z[0]));
-        __builtin_memcpy(__builtin_assume_aligned(zr + 32 * sizeof(T), 16), z[1], sizeof(z[1]));
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int m = 0; m < 2; m++) {
+            __builtin_memcpy(__builtin_assume_aligned(zr + 64 * m, 16), hi[m], 16);
+            __builtin_memcpy(__builtin_assume_aligned(zr + 128 + 64 * m, 16), lo[m], 16);
+          }
+        } else {
+#pragma unroll
+          for (int m = 0; m < 2; m++) __builtin_memcpy(__builtin_assume_aligned(zr + 128 * m, 16), z[m], sizeof(z[m]));
+        }
         if (p % NB == NB - 1) {
           __syncthreads();
           product(p - NB + 1);

@@ -179,15 +179,15 @@ __device__ __forceinline__ void gated8(F g, U u, float (&v)[8]) {
   }
 }
 // dg[i] = d[i] u[i] act'(g[i]), du[i] = d[i] act(g[i])
-template <int ACT, bool EXACT, typename F, typename U, typename T>
-__device__ __forceinline__ void gated8_grad(F g, U u, const float (&d)[8], T (&dg)[8], T (&du)[8]) {
+template <int ACT, bool EXACT, typename F, typename U>
+__device__ __forceinline__ void gated8_grad(F g, U u, const float (&d)[8], float (&dg)[8], float (&du)[8]) {
   switch (ACT) {
     case GATED_SILU:
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const float s = sigmoid<EXACT>(g(i)), a = g(i) * s;
-        dg[i] = (T)(d[i] * u(i) * __builtin_fmaf(a, 1.f - s, s));
-        du[i] = (T)(d[i] * a);
+        dg[i] = (d[i] * u(i) * __builtin_fmaf(a, 1.f - s, s));
+        du[i] = (d[i] * a);
       }
       break;
     case GATED_GELU:
@@ -195,23 +195,23 @@ __device__ __forceinline__ void gated8_grad(F g, U u, const float (&d)[8], T (&d
       for (int i = 0; i < 8; i++) {
         float gauss;
         const float cdf = normal_cdf<EXACT>(g(i), gauss);
-        dg[i] = (T)(d[i] * u(i) * __builtin_fmaf(g(i) * 0.39894228040143267794f, gauss, cdf));
-        du[i] = (T)(d[i] * (g(i) * cdf));
+        dg[i] = (d[i] * u(i) * __builtin_fmaf(g(i) * 0.39894228040143267794f, gauss, cdf));
+        du[i] = (d[i] * (g(i) * cdf));
       }
       break;
     case GATED_RELU:
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        dg[i] = (T)(g(i) > 0.f ? d[i] * u(i) : 0.f);
-        du[i] = (T)(d[i] * (g(i) < 0.f ? 0.f : g(i)));
+        dg[i] = (g(i) > 0.f ? d[i] * u(i) : 0.f);
+        du[i] = (d[i] * (g(i) < 0.f ? 0.f : g(i)));
       }
       break;
     default:
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const float s = sigmoid<EXACT>(g(i));
-        dg[i] = (T)(d[i] * u(i) * (s * (1.f - s)));
-        du[i] = (T)(d[i] * s);
+        dg[i] = (d[i] * u(i) * (s * (1.f - s)));
+        du[i] = (d[i] * s);
       }
   }
 }
