@@ -184,8 +184,8 @@ __device__ __forceinline__ u32x2 tr4(const char* a) {
 }
 
 // waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit and wait for their
-// barriers apart from each other (us, eight / four: 524k x 63 -> 128 bf16 178 / 150, 262k x 96 -> 128 bf16 93 / 148, 100k x 128 -> 128
-// f16 76 / 87)
+// barriers apart from each other (us for both launches, ten calls in a row, eight / four: 262k x 63 -> 64 bf16 64 / 50, 524k x 20 -> 128
+// bf16 120 / 105, 262k x 96 -> 128 bf16 113 / 149, 100k x 128 -> 128 f16 89 / 98)
 constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 
 // bytes behind a row of dz: the rows that one read covers start on different banks (16 rows of 8-byte pieces; f32: 2 rows of 64 bytes)
@@ -195,7 +195,8 @@ constexpr int bwd_lds(int size, int ks, int np, int buffers) {
   return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * 256 + bwd_pad(size)) + 32;
 }
 // Pairs of feature tiles whose dz are kept at once, all, two or one, as many as fit without costing the CU its second workgroup: dW's product
-// reads x once for them, between two barriers.  (As many / one at a time: 524k x 63 -> 128 bf16 150 / 161 us, 100k x 48 -> 128 f32 134 / 146.)
+// reads x once for them, between two barriers.  (As many / one at a time: 262k x 96 -> 128 bf16 113 / 121 us, 262k x 63 -> 64 bf16 50 / 55,
+// 100k x 48 -> 128 f32 132 / 145.)
 constexpr int bwd_buffers(int size, int ks, int np) {
   const int room = bwd_lds(size, ks, np, 1) <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
   return bwd_lds(size, ks, np, np) <= room ? np : np > 2 && bwd_lds(size, ks, np, 2) <= room ? 2 : 1;

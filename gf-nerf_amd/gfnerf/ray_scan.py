@@ -27,9 +27,10 @@ class _RayScanFn(torch.autograd.Function):
         return None, g["df"], g["dc"], g["dh0"] if h0 is not None else None, None, None, None, None
 
 
-def ray_scan(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None):
-    """ops.ray_scan_fwd with gradients for f, c and h0 -> (h [n, channels], state f32 [rays, channels])."""
-    alive = one_graph_at_a_time(f, c, h0)
+def ray_scan(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, leaves=()):
+    """ops.ray_scan_fwd with gradients for f, c and h0 -> (h [n, channels], state f32 [rays, channels]).  leaves: the parameters that f and c were
+    made from, where nothing else keeps a capture of this forward apart from an eager graph of theirs (one_graph_at_a_time)."""
+    alive = one_graph_at_a_time(f, c, h0, *leaves)
     save = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, c, h0))
     return _RayScanFn.apply(pts_offsets, f.contiguous(), c.contiguous(), None if h0 is None else h0.contiguous(), gate, bool(reverse), save, alive)
 
@@ -59,7 +60,7 @@ class RayRecurrence(nn.Module):
     def forward(self, x, pts_offsets, state=None):
         """x [n, n_input_dims] packed -> (h [n, dim], state [rays, dim]); state: the rays' states in front of x (default 0)."""
         f, c = self._project(x)
-        return ray_scan(pts_offsets, f, c, "sigmoid", self.reverse, state)
+        return ray_scan(pts_offsets, f, c, "sigmoid", self.reverse, state, tuple(self.parameters()))
 
     @torch.no_grad()
     def step(self, x, state):

@@ -1474,7 +1474,8 @@ def gated_fwd(x, Wg, Wu, bg=None, bu=None, act="silu", out=None, n_dev=None):
 
 def gated_bwd(x, Wg, Wu, dh, bg=None, bu=None, act="silu", need_dx=True, need_dw=True, n_dev=None):
     """Gradients of gated_fwd for dh -> (dx, dWg, dWu, dbg, dbu); None for what is not wanted or not there.  The projections are formed
-    again from x (the forward saves nothing); the weights' gradients are sums in a fixed order, rounded once to x's dtype."""
+    again from x (the forward saves nothing); the weights' gradients are sums in a fixed order, rounded once to x's dtype.  n_dev as in the
+    forward: dx's rows behind the live ones are not written."""
     n, k, h, ldx, dtype = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_bwd")
     lddh = _rows(dh, "dh", dtype, h, n)[2]
     stream = _place(x, Wg, Wu, bg, bu, n_dev, dh)

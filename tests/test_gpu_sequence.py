@@ -579,6 +579,30 @@ def test_a_capture_beside_a_live_eager_graph_is_refused(T):
             net(x)
 
 
+def test_a_capture_of_a_recurrence_beside_its_live_eager_graph_is_refused(T):
+    """The same for a recurrence on its own: its projections' parameters are the leaves."""
+    from gfnerf_amd import _lib
+    from gfnerf_amd.gfnerf.ray_scan import RayRecurrence
+
+    rec = RayRecurrence(8, 16).cuda()
+    off = T.tensor([0, 5, 9], dtype=T.int32, device="cuda")
+    x = T.ones(9, 8, device="cuda")
+    h, state = rec(x, off)
+    with pytest.raises(_lib.GfnError, match="eager autograd graph"):
+        with T.cuda.graph(T.cuda.CUDAGraph()):
+            rec(x, off)
+    T.cuda.synchronize()
+    del h
+    with pytest.raises(_lib.GfnError, match="eager autograd graph"):  # the state is an output as well
+        with T.cuda.graph(T.cuda.CUDAGraph()):
+            rec(x, off)
+    T.cuda.synchronize()
+    del state
+    with T.cuda.graph(T.cuda.CUDAGraph()):
+        rec(x, off)
+    T.cuda.synchronize()
+
+
 def test_operators_on_a_stream_of_their_own(T, ops):
     """Two streams at once, each with its own calls and workspaces: the results are the default stream's."""
     ins = [gated_inputs(T, "bf16", 20000, 63, 128, True, "silu", seed=s) for s in (0, 1)]
