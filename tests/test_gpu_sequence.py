@@ -124,6 +124,36 @@ def test_gated_backward_of_many_samples(T, ops, kind):
         assert rel <= (1e-6 if kind == "f32" else 2 ** 0.5 * oseq.HALF[kind]), (name, rel)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("k", [8, 16, 31, 32, 33, 48, 64, 65, 80, 96, 100, 127, 128])
+def test_gated_layer_of_every_width(T, ops, kind, k):
+    """Each number of 64-byte units a row can have, whole and cut, with each number of feature blocks a workgroup keeps, whole and cut."""
+    for n, h, bias, act in ((333, 32, True, "silu"), (130, 40, True, "gelu"), (333, 64, False, "sigmoid"), (200, 96, True, "silu"), (333, 128, True, "relu"), (150, 200, True, "silu")):
+        x, wg, wu, bg, bu, dh = gated_inputs(T, kind, n, k, h, bias, act)
+        close(ops.gated_fwd(x[0], wg[0], wu[0], bg[0], bu[0], act), oseq.gated_fwd(x[1], wg[1], wu[1], bg[1], bu[1], act, kind), "h")
+        want = oseq.gated_bwd(x[1], wg[1], wu[1], dh[1], bg[1], bu[1], act, kind)
+        for name, got in zip(("dx", "dwg", "dwu", "dbg", "dbu"), ops.gated_bwd(x[0], wg[0], wu[0], dh[0], bg[0], bu[0], act)):
+            if name in want:
+                close(got, want[name], (name, n, k, h))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_gated_backward_loses_nothing_but_the_results_rounding(T, ops, kind):
+    """The 16-bit gradients are their 64-bit values rounded, but for a few that lie next to the middle between two numbers.  What the products lose
+    is at most half a step of dz's second operand: 2^-8 2^-8 = 2^-16 of a term in bf16; in f16, whose tile scale leaves terms of an ordinary size
+    at 2^-9 and more, half a subnormal step, 2^-25 / 2^-9 = 2^-16 as well.  The terms' errors add up to A times that of the sum, A = norm of the
+    terms over the sum: about 1 for terms of random sign, below 4 here.  A value within d of a middle may round the other way: of values spread
+    evenly over a step (at least 2^-8, f16 2^-11 of the value) a share of 2 A d / step: 2 4 2^-16 / 2^-8 = 3.1 %, f16 25 %.  (With dz rounded
+    to one operand, d is half a step and two values in five differ.)"""
+    n, k, h = 3000, 40, 72
+    x, wg, wu, bg, bu, dh = gated_inputs(T, kind, n, k, h, True, "silu")
+    want = oseq.gated_bwd(x[1], wg[1], wu[1], dh[1], bg[1], bu[1], "silu", kind)
+    for name, got in zip(("dx", "dwg", "dwu"), ops.gated_bwd(x[0], wg[0], wu[0], dh[0], bg[0], bu[0])):
+        exact = T.from_numpy(np.ascontiguousarray(want[name][0])).to(got.dtype)  # rounded once
+        differ = float((exact != got.cpu()).double().mean())
+        assert differ <= (0.031 if kind == "bf16" else 0.25), (name, differ)
+
+
 @pytest.mark.parametrize("scale", [2.0 ** -20, 2.0 ** 12])
 def test_gated_backward_f16_follows_the_gradient_scale(T, ops, scale):
     """f16 gradients far from 1: what the two projections' gradients are rounded to follows the tile's largest |dh|, so the weights' gradients keep
