@@ -15,14 +15,14 @@
 // One pass: x and dh are read once, dx is written once; each workgroup's partial dW goes to a workspace and a second launch adds the
 // partials in a fixed order (no atomics: the same bits every run).  The biases' gradients are the same product against a column of ones
 // and travel as column k of the partials.
-// 16-bit: dz goes into both products as two operands, its rounding to the type and the rounding of what that left, so nothing of it is
-// lost beside the results' own rounding (one operand: errors of 2.4e-3 instead of 1.7e-3 of the norm in bf16 -- what one rounding of the
-// results leaves -- and 115 instead of 145 us in the case below).  f16 has the precision but not the range: see tile_scale_exponent.
+// 16-bit: dz goes into both products as several operands of the type (dz_operands), not rounded to one.  bf16: three, which are dz itself;
+// of 33 million values of dx in the case below 5,300 then differ from their rounded 64-bit values (f32 torch: 7,600; two operands, 17 bits:
+// 80,000, and one: two in five), for 176 us instead of 141 and 115 a call.  f16: two, 22 bits, under a scale: see tile_scale_exponent.
 //
 // What bounds them.  Forward, 786k x 63 -> 128 bf16 silu: 92 us for 300 MB (a copy of that size: 55); four waves a SIMD, requests a tile
 // ahead; relu takes as long, rows of 64 instead of 63 16 % less (odd rows start at any 2 bytes).  262k x 32 -> 128 f32 gelu: 66 us, of
 // which the matrix pipe is busy 27 (f32 products run at 1/8 of bf16's rate) and vector instructions issue for 30; the two hardly overlap.
-// Backward, 524k x 63 -> 128 bf16: 145 us and 7 for the reduction, 266 MB (a copy: 49).  Two waves a SIMD (W's image, x, dz and dW's
+// Backward, 524k x 63 -> 128 bf16: 176 us with the reduction's 7, 266 MB (a copy: 49).  Two waves a SIMD (W's image, x, dz and dW's
 // accumulators fill LDS and registers); a tile's vector instructions, LDS reads and products, a third of its time each, add up rather
 // than overlap.  100k x 128 -> 128 f16: 76 + 13; 50k x 32 -> 64 f32: 29 + 5, 64 % of it the matrix pipe.
 #include "gated_device.h"
@@ -188,19 +188,43 @@ __device__ __forceinline__ u32x2 tr4(const char* a) {
 // bf16 120 / 105, 262k x 96 -> 128 bf16 113 / 149, 100k x 128 -> 128 f16 89 / 98)
 constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 
+// dz as the operands of its products.  bf16: three, each the upper eight of the bits that the one before left -- 24 in all, so their sum is dz
+// itself (cutting never overflows, as rounding next to the largest number does).  f16: its rounding, and the rounding of what that left.
+__device__ __forceinline__ void dz_operands(float z, __bf16 (&e)[3]) {
+  float left = z;
+#pragma unroll
+  for (int q = 0; q < 3; q++) {
+    const uint32_t top = __builtin_bit_cast(uint32_t, left) & 0xffff0000u;
+    e[q] = __builtin_bit_cast(__bf16, (uint16_t)(top >> 16));
+    // an infinity leaves inf - inf: a finite number in its place, which the infinity swallows
+    if (q == 0) left = __builtin_amdgcn_fmed3f(left - __builtin_bit_cast(float, top), -0x1p120f, 0x1p120f);
+    else left -= __builtin_bit_cast(float, top);
+  }
+}
+__device__ __forceinline__ void dz_operands(float z, _Float16 (&e)[2]) {
+  e[0] = (_Float16)z;
+  e[1] = (_Float16)(z - (float)e[0]);
+}
+__device__ __forceinline__ void dz_operands(float, float (&)[1]) {}
+
 // bytes behind a row of dz: the rows that one read covers start on different banks (16 rows of 8-byte pieces; f32: 2 rows of 64 bytes)
-constexpr int bwd_pad(int size) { return size == 4 ? 64 : 16; }
+constexpr int bwd_pad(int dtype) { return dtype == GFN_F32 ? 64 : 16; }
+// operands dz is made of in the products, and the bytes of one pair of feature tiles' dz of a sample
+constexpr int bwd_operands(int dtype) { return dtype == GFN_F32 ? 1 : dtype == GFN_BF16 ? 3 : 2; }
+constexpr int bwd_ztile(int dtype) { return dtype == GFN_F32 ? 256 : 128 * bwd_operands(dtype); }
 // LDS of a workgroup of the backward with room for the dz of `buffers` pairs of feature tiles
-constexpr int bwd_lds(int size, int ks, int np, int buffers) {
-  return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * 256 + bwd_pad(size)) + 32;
+constexpr int bwd_lds(int dtype, int ks, int np, int buffers) {
+  return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * bwd_ztile(dtype) + bwd_pad(dtype)) + 32;
 }
 // Pairs of feature tiles whose dz are kept at once, all, two or one, as many as fit without costing the CU its second workgroup: dW's product
 // reads x once for them, between two barriers.  (As many / one at a time: 262k x 96 -> 128 bf16 113 / 121 us, 262k x 63 -> 64 bf16 50 / 55,
 // 100k x 48 -> 128 f32 132 / 145.)
-constexpr int bwd_buffers(int size, int ks, int np) {
-  const int room = bwd_lds(size, ks, np, 1) <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
-  return bwd_lds(size, ks, np, np) <= room ? np : np > 2 && bwd_lds(size, ks, np, 2) <= room ? 2 : 1;
+constexpr int bwd_buffers(int dtype, int ks, int np) {
+  const int room = bwd_lds(dtype, ks, np, 1) <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
+  return bwd_lds(dtype, ks, np, np) <= room ? np : np > 2 && bwd_lds(dtype, ks, np, 2) <= room ? 2 : 1;
 }
+template <typename T>
+constexpr int dtype_of() { return sizeof(T) == 4 ? GFN_F32 : __is_same(T, __bf16) ? GFN_BF16 : GFN_F16; }
 
 struct GatedBwd {
   int64_t n_max;
@@ -219,8 +243,8 @@ template <typename T, int KS, int NP>
 __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_kernel(GatedBwd a) {
   constexpr int WAVES = bwd_waves(KS);
   constexpr int E = Piece<T>::E, TPU = sizeof(T) == 4 ? 1 : 2;  // 16-column tiles a unit
-  constexpr int KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP, NB = bwd_buffers(sizeof(T), KS, NP);
-  constexpr int SAMPLES = 16 * WAVES, ZTILE = 256, ZROW = NB * ZTILE + bwd_pad(sizeof(T));
+  constexpr int KT = KS * TPU, ROW = KS * 64 + 16, HB = 32 * NP, NB = bwd_buffers(dtype_of<T>(), KS, NP);
+  constexpr int OPS = bwd_operands(dtype_of<T>()), SAMPLES = 16 * WAVES, ZTILE = bwd_ztile(dtype_of<T>()), ZROW = NB * ZTILE + bwd_pad(dtype_of<T>());
   constexpr int FT_WAVES = WAVES / 4, KT_WAVE = (KT + FT_WAVES - 1) / FT_WAVES;  // waves that share a row tile of dW, its column tiles a wave
   constexpr bool EXACT = sizeof(T) == 4, SCALED = sizeof(T) == 2 && !__is_same(T, __bf16);
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -323,12 +347,12 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         const char* q = xs + (4 * kg + (j >> 2)) * ROW + 8 * (j & 3) + 32 * kt0;
         constexpr uint32_t one = __is_same(T, __bf16) ? 0x3f803f80u : 0x3c003c00u;
         constexpr int DEEP = KS < 4 ? 2 : 1;  // dz of the next 32 samples requested with the last x of these, where registers are left for it
-        u32x4 av[DEEP][NB][2];
+        u32x4 av[DEEP][NB][OPS];
         auto samples = [&](int c) {
 #pragma unroll
           for (int o = 0; o < NB; o++)
 #pragma unroll
-            for (int q = 0; q < 2; q++) {  // dz's 16 bits, then what they left
+            for (int q = 0; q < OPS; q++) {  // dz's 16 bits, then what they left
               const char* e = r + 32 * c * ZROW + o * ZTILE + 128 * q;
               const u32x2 lo = tr4(e), hi = tr4(e + 16 * ZROW);
               av[c % DEEP][o][q] = u32x4{lo[0], lo[1], hi[0], hi[1]};
@@ -346,9 +370,12 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
               if (DEEP == 1 && t == 0) samples(c);
 #pragma unroll
               for (int o = 0; o < NB; o++) {
-                const u32x4(&z)[2] = av[c % DEEP][o];
-                if (t == 0) total[o] = mma(z[0], u32x4{one, one, one, one}, mma(z[1], u32x4{one, one, one, one}, total[o], (T*)nullptr), (T*)nullptr);
-                dw[p0 + o][t] = mma(z[0], b, mma(z[1], b, dw[p0 + o][t], (T*)nullptr), (T*)nullptr);
+                const u32x4(&z)[OPS] = av[c % DEEP][o];
+#pragma unroll
+                for (int q = OPS - 1; q >= 0; q--) {
+                  if (t == 0) total[o] = mma(z[q], u32x4{one, one, one, one}, total[o], (T*)nullptr);
+                  dw[p0 + o][t] = mma(z[q], b, dw[p0 + o][t], (T*)nullptr);
+                }
               }
             });
       } else {
@@ -401,29 +428,32 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
 #pragma unroll
       for (int i = 0; i < 8; i++) d[i] = SCALED ? grad(p, i) * to : grad(p, i);
       for_act(act, [&](auto act_c) { gated8_grad<decltype(act_c)::value, EXACT>([&](int i) { return acc[0][i >> 2][i & 3]; }, [&](int i) { return acc[1][i >> 2][i & 3]; }, d, z[0], z[1]); });
-      T hi[2][8], lo[2][8];
+      T part[OPS][2][8];  // 16-bit: dz's rounding, then that of what it left, ..
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int m = 0; m < 2; m++)
 #pragma unroll
           for (int i = 0; i < 8; i++) {
-            hi[m][i] = (T)z[m][i];
-            lo[m][i] = (T)(z[m][i] - (float)hi[m][i]);
+            T e[OPS];
+            dz_operands(z[m][i], e);
+#pragma unroll
+            for (int q = 0; q < OPS; q++) part[q][m][i] = e[q];
           }
       }
       if (a.dx || a.dx_sum) {  // dx[k] += sum over these 32 features
         if constexpr (sizeof(T) == 2) {
           // features 8 kg .. + 3 are image rows 4 kg .. + 3 of tile 0, the next four those of tile 1
           const char* r = lds + (32 * p + 4 * kg + (j >> 2)) * ROW + 8 * (j & 3);
-          const u32x4 bh[2] = {__builtin_bit_cast(u32x4, hi[0]), __builtin_bit_cast(u32x4, hi[1])};
-          const u32x4 bl[2] = {__builtin_bit_cast(u32x4, lo[0]), __builtin_bit_cast(u32x4, lo[1])};
           read_ahead<2 * KT, IN_FLIGHT>(
               [&](int i) {
                 const char* q = r + (i / KT) * HB * ROW + 32 * (i % KT);
                 const u32x2 lo = tr4(q), hi = tr4(q + 16 * ROW);
                 return u32x4{lo[0], lo[1], hi[0], hi[1]};
               },
-              [&](int i, const u32x4& w) { dx[i % KT] = mma(w, bh[i / KT], mma(w, bl[i / KT], dx[i % KT], (T*)nullptr), (T*)nullptr); });
+              [&](int i, const u32x4& w) {
+#pragma unroll
+                for (int q = OPS - 1; q >= 0; q--) dx[i % KT] = mma(w, __builtin_bit_cast(u32x4, part[q][i / KT]), dx[i % KT], (T*)nullptr);
+              });
         } else {
 #pragma unroll
           for (int m = 0; m < 2; m++)
@@ -441,10 +471,9 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         char* zr = zs + (wave * 16 + j) * ZROW + p % NB * ZTILE + 8 * kg * sizeof(T);
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
-          for (int m = 0; m < 2; m++) {
-            __builtin_memcpy(__builtin_assume_aligned(zr + 64 * m, 16), hi[m], 16);
-            __builtin_memcpy(__builtin_assume_aligned(zr + 128 + 64 * m, 16), lo[m], 16);
-          }
+          for (int q = 0; q < OPS; q++)
+#pragma unroll
+            for (int m = 0; m < 2; m++) __builtin_memcpy(__builtin_assume_aligned(zr + 128 * q + 64 * m, 16), part[q][m], 16);
         } else {
 #pragma unroll
           for (int m = 0; m < 2; m++) __builtin_memcpy(__builtin_assume_aligned(zr + 128 * m, 16), z[m], sizeof(z[m]));
@@ -602,7 +631,7 @@ struct BwdPlan {
 
 BwdPlan plan_bwd(int64_t n, int k, int h, int dtype, bool bias) {
   BwdPlan p;
-  const int e = dtype == GFN_F32 ? 4 : 8, size = dtype == GFN_F32 ? 4 : 2;
+  const int e = dtype == GFN_F32 ? 4 : 8;
   p.ks = (k + 4 * e - 1) / (4 * e);
   if (p.ks > 4) p.ks = 8;  // f32 only
   p.waves = bwd_waves(p.ks);
@@ -612,7 +641,7 @@ BwdPlan plan_bwd(int64_t n, int k, int h, int dtype, bool bias) {
   p.np = pairs >= 3 && most == 4 ? 4 : pairs >= 2 ? 2 : 1;
   p.launches = (pairs + p.np - 1) / p.np;
   const int samples = 16 * p.waves;
-  p.lds = bwd_lds(size, p.ks, p.np, bwd_buffers(size, p.ks, p.np));
+  p.lds = bwd_lds(dtype, p.ks, p.np, bwd_buffers(dtype, p.ks, p.np));
   const int64_t tiles = (n + samples - 1) / samples;
   const int at_once = 256 * (p.lds <= 80 * 1024 ? 2 : 1);
   p.blocks = tiles < 1 ? 1 : (int)(tiles < at_once ? tiles : at_once);
