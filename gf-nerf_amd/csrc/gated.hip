@@ -17,14 +17,16 @@
 // and travel as column k of the partials.
 // 16-bit: dz goes into both products as several operands of the type (dz_operands), not rounded to one.  bf16: three, which are dz itself;
 // of 33 million values of dx in the case below 5,300 then differ from their rounded 64-bit values (f32 torch: 7,600; two operands, 17 bits:
-// 80,000, and one: two in five), for 176 us instead of 141 and 115 a call.  f16: two, 22 bits, under a scale: see tile_scale_exponent.
+// 80,000, and one: two in five), for 176 us instead of 141 and 115 a call.  f16: two, 22 bits, under powers of two taken from
+// the |dz| themselves (power_of); 28,400 of 12.8 million values of dx at 100k x 128 -> 128 differ (f32 torch: 28,200), for 89 instead of 83 us.
 //
 // What bounds them.  Forward, 786k x 63 -> 128 bf16 silu: 92 us for 300 MB (a copy of that size: 55); four waves a SIMD, requests a tile
 // ahead; relu takes as long, rows of 64 instead of 63 16 % less (odd rows start at any 2 bytes).  262k x 32 -> 128 f32 gelu: 66 us, of
 // which the matrix pipe is busy 27 (f32 products run at 1/8 of bf16's rate) and vector instructions issue for 30; the two hardly overlap.
 // Backward, 524k x 63 -> 128 bf16: 176 us with the reduction's 7, 266 MB (a copy: 49).  Two waves a SIMD (W's image, x, dz and dW's
 // accumulators fill LDS and registers); a tile's vector instructions, LDS reads and products, a third of its time each, add up rather
-// than overlap.  100k x 128 -> 128 f16: 76 + 13; 50k x 32 -> 64 f32: 29 + 5, 64 % of it the matrix pipe.
+// than overlap.  100k x 128 -> 128 f16: 89 with the reduction's 13; 50k x 32 -> 64 f32: 29 + 5, 64 % of it the
+// matrix pipe.
 #include "gated_device.h"
 
 namespace {
@@ -150,16 +152,54 @@ __global__ __launch_bounds__(64 * kWaves, fwd_per_cu(KS)) void gated_fwd_kernel(
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------------
-// dz in f16: dh may be anywhere in f16's range, so the tile's dz are formed under a power of two that brings its largest |dh| into
-// [2^-5, 1) -- |u act'(g)| and |act(g)| up to 65504 still fit, and what is 2^-20 of the tile's largest is still exact to 2^-4.  dx is
-// scaled back per tile; dW's accumulators follow the running scale (rescaled when a tile's differs: the power moves in steps of 2^4, so
-// hardly ever).
-__device__ __forceinline__ int tile_scale_exponent(float largest, int before) {
-  const int e = (int)((__builtin_bit_cast(uint32_t, largest) >> 23) & 0xffu) - 127;
-  if (e < -60 || e > 60) return before;  // zero, or not finite: nothing to preserve
-  return (-(e + 1) >> 2) * 4;
+// The powers of two that f16 operands of dz are formed under.  A sample's dz of one pair of feature tiles have their own: the multiple of 8 that
+// brings their largest into [2^7, 2^15).  Nothing overflows, two operands hold 22 bits of a number, and what f16's grid of 2^-24 cuts off is
+// small beside that largest.
+// dx: one column of its product is one sample, whose sums stand under the lowest power of its pairs so far (rescaled where that falls).  So a
+// sample's gradient does not depend on its neighbours, and at most 2^-30 of its largest |dz| is cut off of a term.
+// dW contracts over the samples of a tile, whose dz of a pair share the lowest of their powers: at most 2^-30 of the tile's largest is cut off (a
+// term below 2^-8 of it loses bits that f32 would hold, one below 2^-19 of it bits that f16 would).  The sums over the tiles are rescaled
+// where it moves; it never rises more than 2^64 above its lowest, so that they stay in f32.
+constexpr int kTopPower = 96, kNoPower = 104;  // no dz but zeros: no power
+__device__ __forceinline__ int power_of(float largest) {
+  const int e = (15 - __builtin_amdgcn_frexp_expf(largest)) & ~7;  // largest < 2^frexp_exp
+  return largest == 0.f ? kNoPower : e < kTopPower ? e : kTopPower;
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ void rescale(f32x4& v, int by) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = __builtin_amdgcn_ldexpf(v[i], by);
+}
+// the lowest of e over the lanes that share lane >> 4: neighbours, pairs of them, the half row and the row mirrored
+template <int CTRL>
+__device__ __forceinline__ int min_with(int e) {
+  const int o = __builtin_amdgcn_mov_dpp(e, CTRL, 0xf, 0xf, true);
+  return o < e ? o : e;
+}
+__device__ __forceinline__ int min_over_sixteen(int e) { return min_with<0x140>(min_with<0x141>(min_with<0x4e>(min_with<0xb1>(e)))); }
+// eight f16 times 2^by, by <= 0, in two steps: 2^by itself may be below f16's range where the products are not.  (2^-48 takes everything finite
+// to zero, and leaves infinities.)
+__device__ __forceinline__ u32x4 times_pow2(u32x4 v, int by) {
+  by = by < -48 ? -48 : by;
+  const _Float16 f = (_Float16)pow2(by >> 1), g = (_Float16)pow2(by - (by >> 1));
+  const f16x8 r = __builtin_bit_cast(f16x8, v) * f16x8{f, f, f, f, f, f, f, f} * f16x8{g, g, g, g, g, g, g, g};
+  return __builtin_bit_cast(u32x4, r);
+}
+// the largest finite |z|
+__device__ __forceinline__ float largest_of(const float (&z)[2][8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) m = fmaxf(m, fmaxf(__builtin_fabsf(z[0][i]), __builtin_fabsf(z[1][i])));
+  if (__builtin_isinf(m)) {
+    m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const float a = __builtin_fabsf(z[i >> 3][i & 7]);
+      m = a > m && !__builtin_isinf(a) ? a : m;
+    }
+  }
+  return m;
+}
 
 // use(i, load(i)) for i = 0 .. N - 1 with the loads AHEAD of their use, in this order: a read from LDS passes under the products of the
 // ones before it (left to itself, and short of registers, the compiler reads right before each use and waits every time).
@@ -190,7 +230,7 @@ constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 
 // dz as the operands of its products.  bf16: three, each the upper eight of the bits that the one before left -- 24 in all, so their sum is dz
 // itself (cutting never overflows, as rounding next to the largest number does).  f16: its rounding, and the rounding of what that left.
-__device__ __forceinline__ void dz_operands(float z, __bf16 (&e)[3]) {
+__device__ __forceinline__ void dz_operands(float z, float, __bf16 (&e)[3]) {
   float left = z;
 #pragma unroll
   for (int q = 0; q < 3; q++) {
@@ -201,11 +241,22 @@ __device__ __forceinline__ void dz_operands(float z, __bf16 (&e)[3]) {
     else left -= __builtin_bit_cast(float, top);
   }
 }
-__device__ __forceinline__ void dz_operands(float z, _Float16 (&e)[2]) {
-  e[0] = (_Float16)z;
-  e[1] = (_Float16)(z - (float)e[0]);
+__device__ __forceinline__ void dz_operands(float z, float by, _Float16 (&e)[2]) {  // |z by| < 2^15, or not finite; by a power of two
+  e[0] = (_Float16)(z * by);
+  e[1] = (_Float16)__builtin_amdgcn_fmed3f(__builtin_fmaf(z, by, -(float)e[0]), -64.f, 64.f);  // as above: what a finite one leaves is at most 2^4
 }
-__device__ __forceinline__ void dz_operands(float, float (&)[1]) {}
+template <typename T, int OPS>
+__device__ __forceinline__ void dz_operands(const float (&z)[2][8], float by, T (&part)[OPS][2][8]) {
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      T e[OPS];
+      dz_operands(z[m][i], by, e);
+#pragma unroll
+      for (int q = 0; q < OPS; q++) part[q][m][i] = e[q];
+    }
+}
 
 // bytes behind a row of dz: the rows that one read covers start on different banks (16 rows of 8-byte pieces; f32: 2 rows of 64 bytes)
 constexpr int bwd_pad(int dtype) { return dtype == GFN_F32 ? 64 : 16; }
@@ -214,7 +265,7 @@ constexpr int bwd_operands(int dtype) { return dtype == GFN_F32 ? 1 : dtype == G
 constexpr int bwd_ztile(int dtype) { return dtype == GFN_F32 ? 256 : 128 * bwd_operands(dtype); }
 // LDS of a workgroup of the backward with room for the dz of `buffers` pairs of feature tiles
 constexpr int bwd_lds(int dtype, int ks, int np, int buffers) {
-  return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * bwd_ztile(dtype) + bwd_pad(dtype)) + 32;
+  return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * bwd_ztile(dtype) + bwd_pad(dtype)) + 64;
 }
 // Pairs of feature tiles whose dz are kept at once, all, two or one, as many as fit without costing the CU its second workgroup: dW's product
 // reads x once for them, between two barriers.  (As many / one at a time: 262k x 96 -> 128 bf16 113 / 121 us, 262k x 63 -> 64 bf16 50 / 55,
@@ -251,7 +302,7 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
   char* xs = lds + 2 * HB * ROW;        // [SAMPLES][ROW]
   char* zs = xs + SAMPLES * ROW;        // [SAMPLES][NB][dg 32 | du 32], 16-bit: the same of what their rounding left
   float* bias = reinterpret_cast<float*>(zs + SAMPLES * ZROW);  // [2][HB]
-  float* top = bias + 2 * HB;                                   // [WAVES]
+  int* lowest = reinterpret_cast<int*>(bias + 2 * HB);          // [2][WAVES]: the waves' powers
   const T *x = static_cast<const T*>(a.x), *dh = static_cast<const T*>(a.dh);
   const bool biased = a.bg != nullptr;
   const int k = a.k, h = a.h, h0 = a.h0, act = a.act;
@@ -266,7 +317,9 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
 #pragma unroll
     for (int t = 0; t < KT_WAVE; t++) dw[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const bool sums = biased && wave < 4;  // one wave for each row tile
-  int run_e = 0;  // dw holds the sums times 2^run_e
+  int tile_power[NP], lowest_power = kTopPower;  // dw and db hold the sums of pair p times 2^tile_power[p]
+#pragma unroll
+  for (int p = 0; p < NP; p++) tile_power[p] = kTopPower;
   const char* wrow = lds + j * ROW + kg * 16;
   const int64_t tiles = (n + SAMPLES - 1) / SAMPLES;
   constexpr int DP = 8 / E;  // pieces of eight features
@@ -309,33 +362,6 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
       __builtin_memcpy(t, &dr[p][i / E], 16);
       return (float)t[i % E];
     };
-    float back = 1.f, to = 1.f;
-    if constexpr (SCALED) {
-      float m = 0.f;
-#pragma unroll
-      for (int p = 0; p < NP; p++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, __builtin_fabsf(grad(p, i)));
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-      if (lane == 0) top[wave] = m;
-      __syncthreads();
-      m = top[0];
-#pragma unroll
-      for (int w = 1; w < WAVES; w++) m = fmaxf(m, top[w]);
-      const int e = __builtin_amdgcn_readfirstlane(tile_scale_exponent(m, run_e));
-      to = pow2(e);
-      back = pow2(-e);
-      if (e != run_e) {
-        const float by = pow2(e - run_e);
-#pragma unroll
-        for (int p = 0; p < NP; p++)
-#pragma unroll
-          for (int t = 0; t < KT_WAVE; t++) dw[p][t] *= by;
-        db *= by;
-        run_e = e;
-      }
-    }
     // dW's rows of the pairs p0 .. p0 + NB - 1 += their dz^T x over the tile's samples, and db their sums
     auto product = [&](int p0) {
       f32x4 total[NB];  // the same in every column
@@ -407,6 +433,7 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
 #pragma unroll
         for (int i = 0; i < 4; i++) db[i] = j == p0 + o ? db[i] + total[o][i] : db[i];
     };
+    int power = kNoPower;  // dx holds the sample's sums times 2^power
     f32x4 dx[KT];
 #pragma unroll
     for (int t = 0; t < KT; t++) dx[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -426,21 +453,71 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
           [&](int i, const u32x4& w) { acc[i >> 1 & 1][i & 1] = mma(w, HELD ? xr[i >> 2] : xb[i >> 2 & 1], acc[i >> 1 & 1][i & 1], (T*)nullptr); });
       float d[8], z[2][8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) d[i] = SCALED ? grad(p, i) * to : grad(p, i);
+      for (int i = 0; i < 8; i++) d[i] = grad(p, i);
       for_act(act, [&](auto act_c) { gated8_grad<decltype(act_c)::value, EXACT>([&](int i) { return acc[0][i >> 2][i & 3]; }, [&](int i) { return acc[1][i >> 2][i & 3]; }, d, z[0], z[1]); });
-      T part[OPS][2][8];  // 16-bit: dz's rounding, then that of what it left, ..
-      if constexpr (sizeof(T) == 2) {
+      T part[OPS][2][8];
+      int own = 0;  // the power of this sample's dz of the pair
+      if constexpr (SCALED) {
+        float m = largest_of(z);
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        own = power_of(m);
+        const int by = own < power ? own - power : 0;
+        power += by;
+        if (p && __any(by))
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+          for (int t = 0; t < KT; t++) rescale(dx[t], by);
+        if (a.part) {
+          const int e = min_over_sixteen(own);
+          if (lane == 0) lowest[(p & 1) * WAVES + wave] = e;
+        }
+      }
+      if constexpr (sizeof(T) == 2) dz_operands(z, pow2(own), part);
+      if (a.part) {
+        if (SCALED || (p && p % NB == 0)) __syncthreads();  // the pairs before have been read; the waves' powers are there
+        int by = 0;
+        if constexpr (SCALED) {
+          int e = lowest[(p & 1) * WAVES];
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            T e[OPS];
-            dz_operands(z[m][i], e);
+          for (int w = 1; w < WAVES; w++) e = lowest[(p & 1) * WAVES + w] < e ? lowest[(p & 1) * WAVES + w] : e;
+          e = __builtin_amdgcn_readfirstlane(e);
+          if (e == kNoPower) e = tile_power[p];
+          if (e > lowest_power + 64) e = lowest_power + 64;
+          if (e < lowest_power) lowest_power = e;
+          if (e != tile_power[p]) {
 #pragma unroll
-            for (int q = 0; q < OPS; q++) part[q][m][i] = e[q];
+            for (int t = 0; t < KT_WAVE; t++) rescale(dw[p][t], e - tile_power[p]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) db[i] = j == p ? __builtin_amdgcn_ldexpf(db[i], e - tile_power[p]) : db[i];
+            tile_power[p] = e;
           }
+          by = own == kNoPower ? 0 : e - own;
+        }
+        char* zr = zs + (wave * 16 + j) * ZROW + p % NB * ZTILE + 8 * kg * sizeof(T);
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int q = 0; q < OPS; q++)
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+              u32x4 v = __builtin_bit_cast(u32x4, part[q][m]);
+              if (SCALED && __any(by)) v = times_pow2(v, by);
+              *reinterpret_cast<u32x4*>(zr + 128 * q + 64 * m) = v;
+            }
+        } else {
+#pragma unroll
+          for (int m = 0; m < 2; m++) __builtin_memcpy(__builtin_assume_aligned(zr + 128 * m, 16), z[m], sizeof(z[m]));
+        }
       }
       if (a.dx || a.dx_sum) {  // dx[k] += sum over these 32 features
+        if constexpr (SCALED)
+          if (__any(own != power && own != kNoPower))
+#pragma unroll
+            for (int q = 0; q < OPS; q++)
+#pragma unroll
+              for (int m = 0; m < 2; m++) {
+                const u32x4 v = times_pow2(__builtin_bit_cast(u32x4, part[q][m]), own == kNoPower ? 0 : power - own);
+                __builtin_memcpy(part[q][m], &v, 16);
+              }
         if constexpr (sizeof(T) == 2) {
           // features 8 kg .. + 3 are image rows 4 kg .. + 3 of tile 0, the next four those of tile 1
           const char* r = lds + (32 * p + 4 * kg + (j >> 2)) * ROW + 8 * (j & 3);
@@ -466,22 +543,9 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
             }
         }
       }
-      if (a.part) {
-        if (p && p % NB == 0) __syncthreads();  // the pairs before have been read
-        char* zr = zs + (wave * 16 + j) * ZROW + p % NB * ZTILE + 8 * kg * sizeof(T);
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-          for (int q = 0; q < OPS; q++)
-#pragma unroll
-            for (int m = 0; m < 2; m++) __builtin_memcpy(__builtin_assume_aligned(zr + 128 * q + 64 * m, 16), part[q][m], 16);
-        } else {
-#pragma unroll
-          for (int m = 0; m < 2; m++) __builtin_memcpy(__builtin_assume_aligned(zr + 128 * m, 16), z[m], sizeof(z[m]));
-        }
-        if (p % NB == NB - 1) {
-          __syncthreads();
-          product(p - NB + 1);
-        }
+      if (a.part && p % NB == NB - 1) {
+        __syncthreads();
+        product(p - NB + 1);
       }
     }
     loads_done();
@@ -491,7 +555,7 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         const int col = 16 * t + 4 * kg;
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = dx[t][i] * back;
+        for (int i = 0; i < 4; i++) v[i] = SCALED ? __builtin_amdgcn_ldexpf(dx[t][i], -power) : dx[t][i];
         if (col < k) {
           if (!a.dx_first) {
 #pragma unroll
@@ -510,7 +574,6 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
     }
   }
   if (a.part) {
-    const float back = pow2(-run_e);
     const int kp = a.kp;
     float* o = a.part + (int64_t)blockIdx.x * (64 * NP * kp);
 #pragma unroll
@@ -520,11 +583,13 @@ __global__ __launch_bounds__(64 * bwd_waves(KS), KS < 3 ? 2 : 1) void gated_bwd_
         const int col = 16 * (kt0 + t) + j;
         if (col < k)
 #pragma unroll
-          for (int r = 0; r < 4; r++) o[(64 * p + 16 * ft + 4 * kg + r) * kp + col] = dw[p][t][r] * back;
+          for (int r = 0; r < 4; r++) o[(64 * p + 16 * ft + 4 * kg + r) * kp + col] = SCALED ? __builtin_amdgcn_ldexpf(dw[p][t][r], -tile_power[p]) : dw[p][t][r];
       }
-    if (sums && j < NP)
 #pragma unroll
-      for (int r = 0; r < 4; r++) o[(64 * j + 16 * ft + 4 * kg + r) * kp + k] = db[r] * back;
+    for (int p = 0; p < NP; p++)
+      if (sums && j == p)
+#pragma unroll
+        for (int r = 0; r < 4; r++) o[(64 * p + 16 * ft + 4 * kg + r) * kp + k] = SCALED ? __builtin_amdgcn_ldexpf(db[r], -tile_power[p]) : db[r];
   }
 }
 

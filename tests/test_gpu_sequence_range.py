@@ -7,11 +7,9 @@ import pytest
 from helpers import ROOT  # noqa: F401  (puts oracle/ on the path)
 
 import sequence as oseq
+from test_gpu_sequence import KINDS, close, dt, gated_inputs
 
 pytestmark = pytest.mark.gpu
-
-KINDS = ["f32", "bf16", "f16"]
-
 
 @pytest.fixture(scope="module")
 def T():
@@ -29,10 +27,6 @@ def ops(T):
     from gfnerf_amd import ops as _ops
 
     return _ops
-
-
-def dt(T, kind):
-    return {"f32": T.float32, "bf16": T.bfloat16, "f16": T.float16}[kind]
 
 
 def held(T, kind, v):
@@ -68,3 +62,118 @@ def test_gated_gradients_of_exact_terms_are_exact(T, ops, kind, n, k, h):
         rounded = T.from_numpy(want[name]).to(got.dtype)
         differ = got.cpu() != rounded
         assert not bool(differ.any()), (name, int(differ.sum()), differ.numel())
+
+
+NAMES = ("dx", "dwg", "dwu", "dbg", "dbu")
+
+
+def on_device_of(like, v):
+    import torch
+
+    return torch.from_numpy(v).to(like.device)
+
+
+def backward_is_exact(ops, kind, act, x, wg, wu, bg, bu, dh):
+    """Every gradient within the oracle's bound, infinite where its value is past the type's largest number (f16: 65504 and half a step, 16); x, .. are
+    (tensor, its 64-bit values)."""
+    want = oseq.gated_bwd(x[1], wg[1], wu[1], dh[1], bg[1], bu[1], act, kind)
+    got = dict(zip(NAMES, ops.gated_bwd(x[0], wg[0], wu[0], dh[0], bg[0], bu[0], act)))
+    for name, (value, bound) in want.items():
+        v = got[name].double().cpu().numpy()
+        over = (np.abs(value) + bound >= 65520) & np.isinf(v) & (np.sign(v) == np.sign(value)) if kind == "f16" else np.zeros(v.shape, bool)
+        rest = got[name].masked_fill(on_device_of(got[name], over), 0.0)
+        close(rest, (np.where(over, 0.0, value), bound), name)
+    return got, want
+
+
+def scaled(T, kind, v, by):
+    t = (v[0].double() * T.from_numpy(np.ascontiguousarray(np.broadcast_to(by, v[1].shape))).cuda()).to(dt(T, kind))
+    return t, t.double().cpu().numpy()
+
+
+@pytest.mark.parametrize("k,h", [(64, 64), (128, 128), (20, 160)])
+@pytest.mark.parametrize("top", [0, 10])
+@pytest.mark.parametrize("low", [8, 12, 14, 16])
+def test_gated_f16_rows_of_small_gradient_beside_large_ones(T, ops, k, h, top, low):
+    """One row of every 64 has gradients 2^low times those of the others.  dx's rows and dW, each within what the operands and one rounding may do to
+    them: a row's own gradient decides what is cut off of it, and of dW's terms only what is far below the tile's largest."""
+    n = 300
+    x, wg, wu, bg, bu, dh = gated_inputs(T, "f16", n, k, h, True, "silu", seed=low)
+    by = np.full((n, 1), 2.0 ** (top - low))
+    by[7::64] = 2.0 ** top
+    dh = scaled(T, "f16", dh, by)
+    backward_is_exact(ops, "f16", "silu", x, wg, wu, bg, bu, dh)
+    # the large rows alone decide dW's entries; those of features that only small rows reach are seen where the large ones are taken out of x and dh
+    alone = dh[0].clone()
+    alone[7::64] = 0
+    got = ops.gated_bwd(x[0], wg[0], wu[0], alone, bg[0], bu[0])[0]
+    both = ops.gated_bwd(x[0], wg[0], wu[0], dh[0], bg[0], bu[0])[0]
+    keep = T.arange(n, device="cuda") % 64 != 7
+    assert T.equal(got[keep], both[keep])  # a sample's gradient does not depend on its neighbours
+
+
+@pytest.mark.parametrize("act", ["silu", "sigmoid", "gelu"])
+@pytest.mark.parametrize("size", [1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_gated_gradients_of_small_activations(T, ops, kind, act, size):
+    """Inputs of the size of freshly initialised hash features, without biases: u and act(g) are small, and dz far below dh."""
+    x, wg, wu, _, _, dh = gated_inputs(T, kind, 400, 32, 64, False, act, seed=1)
+    backward_is_exact(ops, kind, act, scaled(T, kind, x, size), wg, wu, (None, None), (None, None), dh)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -18, 1.0, 2.0 ** 10])
+def test_gated_f16_gradients_above_the_types_range(T, ops, scale):
+    """act(g) = 1e5 and u = 0.1: h = 1e4 is finite and so are its gradients where dh and the weights leave them finite, although dz passes f16's largest
+    number.  Ordinary rows beside them keep theirs."""
+    rng = np.random.default_rng(4)
+    n, k, h = 130, 16, 32
+    x, wg, wu = rng.standard_normal((n, k)), rng.standard_normal((h, k)), rng.standard_normal((h, k)) * 0.1
+    x[[3, 70]], wg[:, 0] = 0, 500.0
+    x[[3, 70], 0] = 200.0
+    wu[:, 0] = 0.1 / 200
+    dh = rng.standard_normal((n, h)) * min(scale, 1.0)
+    dh[[3, 70]] = 0
+    dh[3, 5], dh[70, 9] = 0.99 * min(scale, 1.0), -0.5 * min(scale, 1.0)
+    made = lambda v: (lambda t: (t.cuda(), t.double().numpy()))(T.from_numpy(v).to(T.float16))  # noqa: E731
+    got, want = backward_is_exact(ops, "f16", "relu", made(x), made(wg), made(wu), (None, None), (None, None), made(dh * max(scale, 1.0)))
+    if scale == 1.0:
+        assert np.abs(want["dx"][0][3]).max() < 65504 and bool(T.isfinite(got["dx"][3]).all())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_gated_gradients_that_are_not_finite_stay_in_their_rows(T, ops, kind, bad):
+    """An infinite or undefined dh of one sample reaches that sample's dx only, and of dW the rows of its features."""
+    x, wg, wu, bg, bu, dh = gated_inputs(T, kind, 200, 24, 48, True, "silu", seed=3)
+    clean = ops.gated_bwd(x[0], wg[0], wu[0], dh[0], bg[0], bu[0])
+    d = dh[0].clone()
+    d[70, 11] = bad
+    got = ops.gated_bwd(x[0], wg[0], wu[0], d, bg[0], bu[0])
+    keep = T.arange(200, device="cuda") != 70
+    assert T.equal(got[0][keep], clean[0][keep]) and not bool(T.isfinite(got[0][70]).any())
+    rows = T.arange(48, device="cuda") != 11
+    want = oseq.gated_bwd(x[1], wg[1], wu[1], np.where(np.arange(200)[:, None] == 70, np.where(np.arange(48) == 11, 0.0, dh[1]), dh[1]), bg[1], bu[1], "silu", kind)
+    for name, g in zip(NAMES[1:], got[1:]):
+        assert not bool(T.isfinite(g[11]).any())
+        value, bound = want[name]
+        off = (g.double().cpu().numpy() - value)[rows.cpu().numpy()]
+        assert (np.abs(off) <= bound[rows.cpu().numpy()]).all(), name
+    if bad == float("inf"):  # an infinity stays one
+        assert bool(T.isinf(got[3][11])) and bool(T.isinf(got[4][11]))
+
+
+@pytest.mark.parametrize("k,h", [(20, 128), (64, 128), (90, 100), (128, 128), (33, 200)])
+@pytest.mark.parametrize("first", [0, -20, 20])
+def test_gated_f16_features_and_rows_of_very_different_gradients(T, ops, k, h, first):
+    """Features of one block of 32 far below or above those of the next, blocks of 16 rows without any gradient, one block of features without any:
+    every power is met and changed, up and down, from tile to tile."""
+    n = 500
+    x, wg, wu, bg, bu, dh = gated_inputs(T, "f16", n, k, h, True, "gelu", seed=2)
+    by = np.ones((n, h))
+    by[:, :32] *= 2.0 ** min(first, 0)
+    by[:, 32:64] *= 2.0 ** -max(first, 0)
+    by[:, 64:96] = 0
+    by[100:170] *= 2.0 ** -3
+    by[250:400] *= 2.0 ** 9
+    by[16:32], by[48:64], by[448:] = 0, 0, 0
+    backward_is_exact(ops, "f16", "gelu", x, wg, wu, bg, bu, scaled(T, "f16", dh, by))
