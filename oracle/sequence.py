@@ -59,8 +59,10 @@ def gated_fwd(x, wg, wu, bg, bu, kind, dtype):
 
 
 def gated_bwd(x, wg, wu, dh, bg, bu, kind, dtype):
-    """dg = dh u act'(g), du = dh act(g), each rounded to dtype once (16 bits: the kernel feeds them to the matrix units); the sums over
-    2 h (dx) and n (dW) products in f32: (count + 2) u of their magnitudes; the result rounded once."""
+    """dg = dh u act'(g), du = dh act(g) in f32, which the matrix units of the 16-bit types take as several operands: bf16 three of 8 bits, which are
+    dz itself down to 2^-126; f16 two, each within 2^-11 of what it stands for, under powers of two that leave the sample's largest |dz| (for dx) and
+    the tile's (for dW; 64 or 128 rows: the bound takes 128) at 2^7 or above.  Half a step of f16's grid is 2^-25; a pair of operands meets it when it
+    is formed, and twice when it is brought to a lower power: below 2^-30 of that largest in all.  Sums over 2 h (dx) and n (dW) products of each operand in f32: (count + 2) u of their magnitudes; the result rounded once."""
     g, eg = _project(x, wg, bg)
     u, eu = _project(x, wu, bu)
     a, da, dda = act(g, kind)
@@ -68,21 +70,25 @@ def gated_bwd(x, wg, wu, dh, bg, bu, kind, dtype):
     dg, du = dh * u * da, dh * a
     edg = np.abs(dh) * (eu * np.abs(da) + (np.abs(u) + eu) * (dda * eg + 3 * ea)) + 4 * U * np.abs(dg)
     edu = np.abs(dh) * (1.13 * eg + ea) + 2 * U * np.abs(du)
-    # f16: formed under a power of two that puts the tile's largest |dh| at 2^-5 or above, so half a step below f16's normal range is
-    # 2^-25 2^5 of that largest
-    floor = np.abs(dh).max(initial=0.0) * 2.0 ** -20 if dtype == "f16" else 0.0
-    edg, edu = edg + (np.abs(dg) + edg) * HALF[dtype] + floor, edu + (np.abs(du) + edu) * HALF[dtype] + floor
     n, h = dg.shape
+    ops = {"f32": 1, "bf16": 3, "f16": 2}[dtype]
+
+    def fed(v, e, floor):  # what the operands add
+        return e + (np.abs(v) + e) * 2.0 ** -22 + floor if dtype == "f16" else e + (2.0 ** -126 if dtype == "bf16" else 0.0)
+
+    row = np.maximum(np.abs(dg), np.abs(du)).max(1, initial=0.0)[:, None]
+    tile = np.concatenate([np.full((len(r), 1), r.max()) for r in np.split(row, range(128, n, 128))]) if n else row
 
     def total(parts, count):
         v = sum(p @ q for p, e, q in parts)
-        err = sum(e @ np.abs(q) + (count + 2) * U * ((np.abs(p) + e) @ np.abs(q)) for p, e, q in parts)
+        err = sum(e @ np.abs(q) + (ops * count + 2) * U * ((np.abs(p) + e) @ np.abs(q)) for p, e, q in parts)
         return v, rounded(v, err, dtype)
 
+    xdg, xdu, wdg, wdu = (fed(v, e, f) for f in (row * 2.0 ** -30, tile * 2.0 ** -30) for v, e in ((dg, edg), (du, edu)))
     ones = np.ones((n, 1))
-    out = {"dx": total([(dg, edg, wg), (du, edu, wu)], 2 * h), "dwg": total([(dg.T, edg.T, x)], n), "dwu": total([(du.T, edu.T, x)], n)}
+    out = {"dx": total([(dg, xdg, wg), (du, xdu, wu)], 2 * h), "dwg": total([(dg.T, wdg.T, x)], n), "dwu": total([(du.T, wdu.T, x)], n)}
     if bg is not None:
-        out["dbg"], out["dbu"] = ((v[:, 0], e[:, 0]) for v, e in (total([(dg.T, edg.T, ones)], n), total([(du.T, edu.T, ones)], n)))
+        out["dbg"], out["dbu"] = ((v[:, 0], e[:, 0]) for v, e in (total([(dg.T, wdg.T, ones)], n), total([(du.T, wdu.T, ones)], n)))
     return out
 
 
