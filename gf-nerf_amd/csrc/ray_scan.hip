@@ -13,8 +13,9 @@
 // A lane owns VEC channels and walks rows: of one ray where there are rays enough to fill the chip, else of one RUN of rows (several to a
 // ray, or several rays to one).  Rows are taken in aligned blocks of 8, the next block requested before this one is worked on, so the
 // recurrence's chain of multiply-adds runs on data that has arrived.  A run's walk starts from a state that the rows in front of it
-// decide: a first reading (AGG) reduces every run to one step state -> A state + S, with A = 0 as soon as a ray begins in it,
-// run_prefix_kernel composes the steps in order, and the second reading writes the results.  Every sum has a fixed order: the same bits
+// decide: a first reading (AGG) reduces every run to one step state -> A state + S (state -> S where a ray begins in it), run_prefix_kernel
+// composes the steps in order, and the second reading writes the results.  A product of many gates leaves f32's range long before a state
+// does, so A has an exponent of its own: it is zero only where a gate is, and what a walk row by row keeps -- a state, a NaN -- a step keeps.  Every sum has a fixed order: the same bits
 // every run.  State and adjoint are f32.
 #include "gfn_common.h"
 
@@ -76,14 +77,43 @@ struct ScanArgs {
   int lanes, slot, parts;
   float* partial;
   int64_t run_rows, runs;  // 0: a walk is a ray; else rows of a run (a multiple of kBlock) and their number
-  float2* agg;             // [d][runs]: AGG writes (A, S); then .y is the state in front of the run
+  struct Step* agg;        // [d][runs]: AGG writes the steps; then .s is the state in front of the run
 };
 
-// a state that meets a ray's beginning (a = 0) stays out of it, infinite or not
-__device__ __forceinline__ float compose(float a, float b, float s) { return a == 0.f || s == 0.f ? b : __builtin_fmaf(a, s, b); }
-
-// the A of a step a1 and then a2: zero (a ray's beginning) stays zero
-__device__ __forceinline__ float carry(float a1, float a2) { return a1 == 0.f ? 0.f : a1 * a2; }
+// What a run does to the state in front of it: A state + s, A = m 2^e with m = 0 or 1/2 <= |m| < 1 (or not finite); begins: s alone.
+struct alignas(16) Step {
+  float m;
+  int e;
+  float s;
+  int begins;
+};
+struct Gain {  // A on its way through a run
+  float m = 1.f;
+  int e = 0;
+  __device__ __forceinline__ void times(float a) {  // up to 8 times between normalize()
+    m *= __builtin_amdgcn_frexp_mantf(a);
+    e += __builtin_amdgcn_frexp_expf(a);
+  }
+  __device__ __forceinline__ void normalize() {  // (e stays far inside an int however long the run)
+    e += __builtin_amdgcn_frexp_expf(m);
+    m = __builtin_amdgcn_frexp_mantf(m);
+    e = e < -(1 << 28) ? -(1 << 28) : e > 1 << 28 ? 1 << 28 : e;
+  }
+};
+// the state behind a step from the state in front of it.  (A state of zero leaves s: gates that are not finite have met it already.)
+__device__ __forceinline__ float after(const Step& q, float s) {
+  if (q.begins || s == 0.f) return q.s;
+  if (q.e > -100 && q.e < 100) return __builtin_fmaf(__builtin_amdgcn_ldexpf(q.m, q.e), s, q.s);
+  return (q.e > 0 ? __builtin_amdgcn_ldexpf(s, q.e - 1) * (q.m + q.m) : __builtin_amdgcn_ldexpf(q.m * s, q.e)) + q.s;
+}
+// q1 and then q2, as one step
+__device__ __forceinline__ Step both(const Step& q1, const Step& q2) {
+  Gain g;
+  g.m = q1.m * q2.m;
+  g.e = q1.e + q2.e;
+  g.normalize();
+  return {g.m, g.e, after(q2, q1.s), q1.begins | q2.begins};
+}
 
 struct Place {
   int64_t walk;  // the ray or run
@@ -275,22 +305,20 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
   Gates<T, GATE, VEC, SHARED> gates{dealt ? pool + (threadIdx.x & ~(a.slot - 1)) : nullptr, deal};
   const T *f = static_cast<const T*>(a.f) + at.gate, *c = static_cast<const T*>(a.c) + at.ch;
   T* h = static_cast<T*>(a.h) + at.ch;
-  float s[VEC], A[VEC];
+  float s[VEC];
+  Gain A[VEC];
+  int begun = 0;
 #pragma unroll
-  for (int v = 0; v < VEC; v++) {
-    s[v] = !AGG && a.run_rows ? a.agg[(at.ch + v) * a.runs + at.walk].y : 0.f;
-    A[v] = 1.f;
-  }
+  for (int v = 0; v < VEC; v++) s[v] = !AGG && a.run_rows ? a.agg[(at.ch + v) * a.runs + at.walk].s : 0.f;
   Pieces pieces(a, at.walk, asc);
   int64_t ray, lo, hi;
   bool begins, ends;
   while (pieces.next(ray, lo, hi, begins, ends)) {
-    if (begins)
+    if (begins) {
+      begun = 1;
 #pragma unroll
-      for (int v = 0; v < VEC; v++) {
-        s[v] = a.h0 ? a.h0[ray * a.d + at.ch + v] : 0.f;
-        A[v] = 0.f;
-      }
+      for (int v = 0; v < VEC; v++) s[v] = a.h0 ? a.h0[ray * a.d + at.ch + v] : 0.f;
+    }
     const int64_t b0 = lo / kBlock, blocks = hi > lo ? (hi - 1) / kBlock - b0 + 1 : 0;
     Rows<T, VEC, SHARED, false, AGG> now, next;
     auto base_of = [&](int64_t i) { return (asc ? b0 + i : b0 + blocks - 1 - i) * kBlock; };
@@ -317,7 +345,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
         for (int v = 0; v < VEC; v++) {
           const float n = __builtin_fmaf(x[v], s[v], y[v] * now.in(r, v));
           s[v] = in ? n : s[v];
-          if (AGG) A[v] = in ? carry(A[v], x[v]) : A[v];
+          if (AGG) A[v].times(in ? x[v] : 1.f);
           o.v[v] = (T)s[v];
         }
         if (!AGG) {
@@ -325,6 +353,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
           else if (in && at.active) *reinterpret_cast<V*>(out + r * step) = o;
         }
       }
+      if (AGG)
+#pragma unroll
+        for (int v = 0; v < VEC; v++) A[v].normalize();
       if (INNER || i + 1 < blocks) now = next;
     };
     for (int64_t i = 0; i < blocks; i++) {
@@ -338,7 +369,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanArgs a) {
   }
   if (AGG && at.active)
 #pragma unroll
-    for (int v = 0; v < VEC; v++) a.agg[(at.ch + v) * a.runs + at.walk] = make_float2(A[v], s[v]);
+    for (int v = 0; v < VEC; v++) a.agg[(at.ch + v) * a.runs + at.walk] = {A[v].m, A[v].e, s[v], begun};
 }
 
 template <typename T, int GATE, int VEC, bool SHARED, bool AGG>
@@ -357,22 +388,20 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
   Gates<T, GATE, VEC, SHARED> gates{dealt ? pool + (threadIdx.x & ~(a.slot - 1)) : nullptr, deal};
   const T *f = static_cast<const T*>(a.f) + at.gate, *c = static_cast<const T*>(a.c) + at.ch, *dh = static_cast<const T*>(a.dh) + at.ch;
   T *df = static_cast<T*>(a.df) + at.gate, *dc = static_cast<T*>(a.dc) + at.ch;
-  float l[VEC], A[VEC];
+  float l[VEC];
+  Gain A[VEC];
+  int begun = 0;
 #pragma unroll
-  for (int v = 0; v < VEC; v++) {
-    l[v] = !AGG && a.run_rows ? a.agg[(at.ch + v) * a.runs + at.walk].y : 0.f;
-    A[v] = 1.f;
-  }
+  for (int v = 0; v < VEC; v++) l[v] = !AGG && a.run_rows ? a.agg[(at.ch + v) * a.runs + at.walk].s : 0.f;
   Pieces pieces(a, at.walk, asc);
   int64_t ray, lo, hi;
   bool begins, ends;
   while (pieces.next(ray, lo, hi, begins, ends)) {
-    if (begins)
+    if (begins) {
+      begun = 1;
 #pragma unroll
-      for (int v = 0; v < VEC; v++) {
-        l[v] = a.d_state ? a.d_state[ray * a.d + at.ch + v] : 0.f;
-        A[v] = 0.f;
-      }
+      for (int v = 0; v < VEC; v++) l[v] = a.d_state ? a.d_state[ray * a.d + at.ch + v] : 0.f;
+    }
     const int64_t b0 = lo / kBlock, blocks = hi > lo ? (hi - 1) / kBlock - b0 + 1 : 0;
     Rows<T, VEC, SHARED, true, AGG> now, next;
     auto base_of = [&](int64_t i) { return (asc ? b0 + i : b0 + blocks - 1 - i) * kBlock; };
@@ -442,7 +471,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
             else of.v[v] = (T)d;
           }
           l[v] = in ? xv * lt : l[v];
-          if (AGG) A[v] = in ? carry(A[v], xv) : A[v];
+          if (AGG) A[v].times(in ? xv : 1.f);
         }
         if (!AGG) {
           if (whole) {
@@ -483,6 +512,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
             }
           }
       }
+      if (AGG)
+#pragma unroll
+        for (int v = 0; v < VEC; v++) A[v].normalize();
       if (INNER || i + 1 < blocks) now = next;
     };
     for (int64_t i = 0; i < blocks; i++) {
@@ -495,7 +527,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
   }
   if (AGG && at.active)
 #pragma unroll
-    for (int v = 0; v < VEC; v++) a.agg[(at.ch + v) * a.runs + at.walk] = make_float2(A[v], l[v]);
+    for (int v = 0; v < VEC; v++) a.agg[(at.ch + v) * a.runs + at.walk] = {A[v].m, A[v].e, l[v], begun};
 }
 
 // AGG's steps -> the state in front of every run (in the walk's order).  A workgroup: one channel, 1,024 stretches of neighbouring runs, each
@@ -503,50 +535,42 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
 // waves' steps one after the other.  Latency bound: 5 us for 4,096 runs of 64 channels; with the steps as [runs][channels], four
 // channels a workgroup, 18 us -- every load then takes 32 bytes of a line, on a quarter of the CUs.
 constexpr int kHeld = 4, kPrefixWaves = 16;
-__global__ __launch_bounds__(64 * kPrefixWaves) void run_prefix_kernel(float2* __restrict__ steps, int64_t runs) {
-  __shared__ float2 last[kPrefixWaves];
-  float2* __restrict__ agg = steps + (int64_t)blockIdx.x * runs;
+__device__ __forceinline__ Step step_up(const Step& q, int by) {
+  return {__shfl_up(q.m, by, 64), __shfl_up(q.e, by, 64), __shfl_up(q.s, by, 64), __shfl_up(q.begins, by, 64)};
+}
+__global__ __launch_bounds__(64 * kPrefixWaves) void run_prefix_kernel(Step* __restrict__ steps, int64_t runs) {
+  __shared__ Step last[kPrefixWaves];
+  Step* __restrict__ agg = steps + (int64_t)blockIdx.x * runs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t per = (runs + 64 * kPrefixWaves - 1) / (64 * kPrefixWaves), lo = threadIdx.x * per, hi = lo + per < runs ? lo + per : runs;
-  float2 held[kHeld];
-  float a = 1.f, s = 0.f;
+  Step held[kHeld], q = {0.5f, 1, 0.f, 0};
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) held[i] = lo + i < hi ? agg[lo + i] : make_float2(1.f, 0.f);
+  for (int i = 0; i < kHeld; i++) held[i] = lo + i < hi ? agg[lo + i] : Step{0.5f, 1, 0.f, 0};
 #pragma unroll
   for (int i = 0; i < kHeld; i++)
-    if (lo + i < hi) {
-      s = compose(held[i].x, held[i].y, s);
-      a = carry(a, held[i].x);
-    }
-  for (int64_t i = lo + kHeld; i < hi; i++) {
-    const float2 q = agg[i];
-    s = compose(q.x, q.y, s);
-    a = carry(a, q.x);
-  }
+    if (lo + i < hi) q = both(q, held[i]);
+  for (int64_t i = lo + kHeld; i < hi; i++) q = both(q, agg[i]);
 #pragma unroll
-  for (int off = 1; off < 64; off *= 2) {  // then (a, s) is the step of the wave's stretches up to this one
-    const float a1 = __shfl_up(a, off, 64), s1 = __shfl_up(s, off, 64);
-    if (lane >= off) {
-      s = compose(a, s, s1);
-      a = carry(a1, a);
-    }
+  for (int off = 1; off < 64; off *= 2) {  // then q is the step of the wave's stretches up to this one
+    const Step q1 = step_up(q, off);
+    if (lane >= off) q = both(q1, q);
   }
-  if (lane == 63) last[wave] = make_float2(a, s);
+  if (lane == 63) last[wave] = q;
   __syncthreads();
   float front = 0.f;  // the state in front of the wave's first stretch, then of this one
-  for (int w = 0; w < wave; w++) front = compose(last[w].x, last[w].y, front);
-  const float a1 = __shfl_up(a, 1, 64), s1 = __shfl_up(s, 1, 64);
-  s = lane ? compose(a1, s1, front) : front;
+  for (int w = 0; w < wave; w++) front = after(last[w], front);
+  const Step q1 = step_up(q, 1);
+  float s = lane ? after(q1, front) : front;
 #pragma unroll
   for (int i = 0; i < kHeld; i++)
     if (lo + i < hi) {
-      agg[lo + i].y = s;
-      s = compose(held[i].x, held[i].y, s);
+      agg[lo + i].s = s;
+      s = after(held[i], s);
     }
   for (int64_t i = lo + kHeld; i < hi; i++) {
-    const float2 q = agg[i];
-    agg[i].y = s;
-    s = compose(q.x, q.y, s);
+    const Step r = agg[i];
+    agg[i].s = s;
+    s = after(r, s);
   }
 }
 
@@ -641,7 +665,7 @@ int64_t scan_workspace(int64_t rays, int64_t n_max, int d, int g) {
       if (p.runs > runs) runs = p.runs;
       if (p.parts > parts) parts = p.parts;
     }
-  return runs * d * 8 + (parts > 1 ? parts * n_max * g * 4 : 0);
+  return runs * d * (int64_t)sizeof(Step) + (parts > 1 ? parts * n_max * g * 4 : 0);
 }
 
 template <typename T, int GATE, int VEC, bool SHARED>
@@ -652,8 +676,8 @@ int launch_scan(ScanArgs a, bool bwd, char* ws, hipStream_t st) {
   a.lanes = p.lanes;
   a.run_rows = p.run_rows;
   a.runs = p.runs;
-  a.agg = reinterpret_cast<float2*>(ws);
-  a.partial = reinterpret_cast<float*>(ws + p.runs * a.d * 8);
+  a.agg = reinterpret_cast<Step*>(ws);
+  a.partial = reinterpret_cast<float*>(ws + p.runs * a.d * sizeof(Step));
   const int64_t threads = (p.run_rows ? p.runs : a.rays) * p.lanes, blocks = (threads + kScanThreads - 1) / kScanThreads;
   GFN_CHECK_ARG(blocks < (1ll << 31), "gfn_ray_scan: %lld rays of %d channels are too many for one launch", (long long)a.rays, a.d);
   const unsigned grid = (unsigned)(blocks < 1 ? 1 : blocks);

@@ -177,3 +177,105 @@ def test_gated_f16_features_and_rows_of_very_different_gradients(T, ops, k, h, f
     by[250:400] *= 2.0 ** 9
     by[16:32], by[48:64], by[448:] = 0, 0, 0
     backward_is_exact(ops, "f16", "gelu", x, wg, wu, bg, bu, scaled(T, "f16", dh, by))
+
+
+# ---- recurrence, walked in runs of rows -------------------------------------------------------------------------------------------------------
+LONG = [4096, 3000, 5000]  # few and long: every ray is many runs of 32 rows
+
+
+def gates(T, kind, gate, n, g, seed):
+    rng = np.random.default_rng(seed)
+    v = rng.standard_normal((n, g))
+    return T.from_numpy(np.exp(v * 1.5 - 2) if gate == "decay" else 1 / (1 + np.exp(-v - 1)) if gate == "linear" else v + 1).to(dt(T, kind)).cuda()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("gate", ["linear", "sigmoid", "decay"])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("bad", ["nan", "large"])
+def test_gates_of_one_ray_do_not_reach_the_next_in_runs(T, ops, kind, gate, reverse, bad):
+    """Undefined gates in the middle of a ray, and gates whose product passes f32's range: the other rays' states, outputs and gradients are those of a
+    call without them, bit for bit."""
+    off = T.tensor(np.concatenate([[0], np.cumsum(LONG)]), dtype=T.int32, device="cuda")
+    n, d = sum(LONG), 8
+    rng = np.random.default_rng(1)
+    made = lambda *s: T.from_numpy(rng.standard_normal(s))  # noqa: E731
+    f, c, dh = gates(T, kind, gate, n, d, 0), made(n, d).to(dt(T, kind)).cuda(), made(n, d).to(dt(T, kind)).cuda()
+    h0, ds = made(3, d).float().cuda(), made(3, d).float().cuda()
+
+    def call(f):
+        r = ops.ray_scan_fwd(off, f, c, gate, reverse, h0, save=True)
+        b = ops.ray_scan_bwd(off, f, c, dh, r["saved"], gate, reverse, h0, ds)
+        return [r["h"], b["df"], b["dc"]], [r["state"], b["dh0"]]
+
+    clean_rows, clean_rays = call(f)
+    for ray in range(3):
+        s, e = sum(LONG[:ray]), sum(LONG[:ray + 1])
+        g = f.clone()
+        if bad == "nan":
+            g[s + 700:s + 703] = float("nan")
+        else:
+            g[s + 100:e - 100] = {"linear": 20.0, "sigmoid": 80.0, "decay": -3.0}[gate]
+        rows, rays = call(g)
+        keep = T.ones(n, dtype=T.bool, device="cuda")
+        keep[s:e] = False
+        for a, b in zip(rows, clean_rows):
+            assert T.equal(a[keep], b[keep]), ray
+        others = [r for r in range(3) if r != ray]
+        for a, b in zip(rays, clean_rays):
+            assert T.equal(a[others], b[others]), ray
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_what_is_not_finite_stays_to_the_end_of_its_ray_in_runs(T, ops, kind, reverse, value):
+    """An input that is undefined or infinite early in a ray whose gates multiply to nothing within a run (exp(-10) a row): the definition keeps it to the
+    ray's end, in its channel."""
+    off = T.tensor(np.concatenate([[0], np.cumsum(LONG)]), dtype=T.int32, device="cuda")
+    n, d = sum(LONG), 8
+    f = T.full((n, d), 10.0, dtype=dt(T, kind), device="cuda")
+    c = T.ones(n, d, dtype=dt(T, kind), device="cuda")
+    at = 4096 + (2900 if reverse else 100)
+    c[at, 3] = value
+    r = ops.ray_scan_fwd(off, f, c, "decay", reverse, save=True)
+    want = T.zeros(n, d, dtype=T.bool, device="cuda")
+    if reverse:
+        want[4096:at + 1, 3] = True
+    else:
+        want[at:7096, 3] = True
+    same = T.isnan if value != value else T.isinf
+    assert T.equal(same(r["h"]), want) and T.equal(T.isfinite(r["h"]), ~want)
+    assert T.equal(same(r["state"]), T.tensor([[False] * 8, [False] * 3 + [True] + [False] * 4, [False] * 8], device="cuda"))
+    dh = T.ones(n, d, dtype=dt(T, kind), device="cuda")
+    dh[at, 3] = value
+    ok = ops.ray_scan_fwd(off, f, T.ones_like(c), "decay", reverse, save=True)
+    b = ops.ray_scan_bwd(off, f, T.ones_like(c), dh, ok["saved"], "decay", reverse)
+    want = T.zeros(n, d, dtype=T.bool, device="cuda")
+    if reverse:
+        want[at:7096, 3] = True
+    else:
+        want[4096:at + 1, 3] = True
+    assert T.equal(~T.isfinite(b["dc"]), want)
+    assert T.equal(~T.isfinite(b["dh0"]), T.tensor([[False] * 8, [False] * 3 + [True] + [False] * 4, [False] * 8], device="cuda"))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("first,start", [(2.0 ** -5, 2.0 ** 100), (2.0 ** 5, 2.0 ** -100)])
+def test_a_state_in_f32s_range_survives_gates_whose_product_leaves_it(T, ops, kind, reverse, first, start):
+    """32 rows of 2^-5 (2^5) and 32 of its reciprocal, over and over in the recurrence's order, from 2^100 (2^-100): every state is a power of two between
+    2^-60 and 2^100 (2^-100 and 2^60), although the product of a run's gates is 2^-160 (2^160).  The adjoint meets the reciprocals first and starts from
+    the reciprocal."""
+    off = T.tensor([0, 4096, 6144], dtype=T.int32, device="cuda")
+    n, d = 6144, 8
+    f = np.where((np.arange(n) % 64 < 32) != reverse, first, 1 / first)[:, None] * np.ones((1, d))
+    zero = np.zeros((n, d))
+    h0, ds = np.full((2, d), start), np.full((2, d), 1 / start)
+    want = oseq.ray_scan(off.cpu().numpy(), f, zero, "linear", reverse, "f32", h0, zero, ds)
+    assert all(2.0 ** -100 <= v.min() and v.max() <= 2.0 ** 100 for v in (want["h"][0], want["dc"][0]))
+    t = lambda v, k=kind: T.from_numpy(v).to(dt(T, k)).cuda()  # noqa: E731
+    r = ops.ray_scan_fwd(off, t(f), t(zero), "linear", reverse, t(h0, "f32"), save=True)
+    assert np.array_equal(r["h"].double().cpu().numpy(), want["h"][0]) and np.array_equal(r["state"].double().cpu().numpy(), want["state"][0]), lens
+    b = ops.ray_scan_bwd(off, t(f), t(zero), t(zero), r["saved"], "linear", reverse, t(h0, "f32"), t(ds, "f32"))
+    assert np.array_equal(b["dc"].double().cpu().numpy(), want["dc"][0]) and np.array_equal(b["dh0"].double().cpu().numpy(), want["dh0"][0])
