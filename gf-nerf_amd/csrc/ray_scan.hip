@@ -168,12 +168,10 @@ struct Pieces {
   }
   // rows [s, e) of the next piece and whether its ray begins / ends (in the walk's order) there; false: no more
   __device__ bool next(int64_t& of, int64_t& s, int64_t& e, bool& begins, bool& ends) {
-    for (;;) {
+    for (bool passed = false;; passed = true) {
       if (ray < 0 || ray >= a.rays) return false;
       const int64_t rs = clamp_row(a.offsets[ray], 0, a.n_max), re = clamp_row(a.offsets[ray + 1], rs, a.n_max);
-      if (a.run_rows && (asc ? rs >= hi : re <= lo)) {
-        if (rs < re || (asc ? rs > hi : re < lo)) return false;  // an empty ray on the border says nothing about the next one
-      }
+      if (a.run_rows && (asc ? rs >= hi : re <= lo)) return false;
       of = ray;
       s = rs > lo ? rs : lo;
       e = re < hi ? re : hi;
@@ -183,8 +181,18 @@ struct Pieces {
         ray = a.rays;
         return true;
       }
-      ray += asc ? 1 : -1;
-      if (s < e) return true;
+      if (s < e || !passed) {
+        ray += asc ? 1 : -1;
+        if (s < e) return true;
+      } else {  // a second ray without rows: there may be many
+        int64_t x = asc ? ray + 1 : 0, y = asc ? a.rays : ray;
+        while (x < y) {
+          const int64_t m = (x + y) >> 1;
+          if (asc ? a.offsets[m + 1] > rs : a.offsets[m] >= re) y = m;
+          else x = m + 1;
+        }
+        ray = asc ? x : x - 1;
+      }
     }
   }
 };

@@ -279,3 +279,48 @@ def test_a_state_in_f32s_range_survives_gates_whose_product_leaves_it(T, ops, ki
     assert np.array_equal(r["h"].double().cpu().numpy(), want["h"][0]) and np.array_equal(r["state"].double().cpu().numpy(), want["state"][0]), lens
     b = ops.ray_scan_bwd(off, t(f), t(zero), t(zero), r["saved"], "linear", reverse, t(h0, "f32"), t(ds, "f32"))
     assert np.array_equal(b["dc"].double().cpu().numpy(), want["dc"][0]) and np.array_equal(b["dh0"].double().cpu().numpy(), want["dh0"][0])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_runs_pass_over_long_stretches_of_rays_without_rows(T, ops, kind, reverse):
+    """Stretches of rays that miss the scene, in front of, between and behind the rays with rows, in the middle of a run and on its border: values, and
+    a time that is not theirs.  (Taken one after the other they cost a walk a microsecond or two each, seven hundred several times the whole call.)"""
+    lens = np.zeros(1500, np.int64)
+    lens[[70, 700, 701, 750, 1450]] = (32 * 6000, 7, 32 * 1000 - 7, 96000, 90005)
+    rays, n, d = len(lens), int(lens.sum()), 8
+    assert n // rays >= 96 and rays < 6 * (n // rays)  # few enough and long enough on average to be walked in runs
+    rng = np.random.default_rng(2)
+    made = lambda *s: (lambda t: (t.cuda(), t.double().numpy()))(T.from_numpy(rng.standard_normal(s)).to(dt(T, kind)))  # noqa: E731
+    f, c, dh = made(n, d), made(n, d), made(n, d)
+    h0 = T.from_numpy(rng.standard_normal((rays, d))).float().cuda()
+    full = np.flatnonzero(lens)
+    offsets = lambda l: T.tensor(np.concatenate([[0], np.cumsum(l)]), dtype=T.int32, device="cuda")  # noqa: E731
+
+    def call(off, h0):
+        r = ops.ray_scan_fwd(off, f[0], c[0], "sigmoid", reverse, h0, save=True)
+        return r, ops.ray_scan_bwd(off, f[0], c[0], dh[0], r["saved"], "sigmoid", reverse, h0, h0)
+
+    off, few = offsets(lens), offsets(lens[full])
+    at = T.from_numpy(full).cuda()
+    r, b = call(off, h0)
+    rf, bf = call(few, h0[at].contiguous())
+    for got, want in ((r["h"], rf["h"]), (b["df"], bf["df"]), (b["dc"], bf["dc"]), (r["state"][at], rf["state"]), (b["dh0"][at], bf["dh0"])):
+        assert T.equal(got, want)
+    none = T.from_numpy(lens == 0).cuda()
+    assert T.equal(r["state"][none], h0[none]) and T.equal(b["dh0"][none], h0[none])
+
+    def best(*args):
+        t = []
+        for _ in range(5):
+            a, z = T.cuda.Event(enable_timing=True), T.cuda.Event(enable_timing=True)
+            a.record()
+            call(*args)
+            z.record()
+            z.synchronize()
+            t.append(a.elapsed_time(z))
+        return min(t)
+
+    few_h0 = h0[at].contiguous()
+    best(few, few_h0)
+    assert best(off, h0) <= 4 * best(few, few_h0)
