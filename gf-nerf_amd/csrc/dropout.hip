@@ -90,6 +90,10 @@ int gfn_dropout(const void* x, int64_t ldx, int64_t rows, int cols, int dtype, f
   if (rows == 0 || cols == 0) return GFN_OK;
   GFN_CHECK_ARG(x && y && call, "gfn_dropout: null pointer");
   GFN_CHECK_ARG(ldx >= cols && ldy >= cols, "gfn_dropout: a row stride is below the row's width");
+  const int size = dtype == GFN_F32 ? 4 : 2;
+  const gfn_rows rx{"x", x, rows, cols, ldx, size}, ry{"y", y, rows, cols, ldy, size};
+  GFN_CHECK_ARG(gfn_same_rows(rx, ry) || !gfn_overlap(rx, ry), "gfn_dropout: y overlaps x, and is not x");
+  GFN_CHECK_ARG(!gfn_overlap(ry, gfn_flat("call", call, 1, 8)), "gfn_dropout: y overlaps call");
   const uint32_t below = (uint32_t)((double)p * 65536.0 + 0.5);
   const float scale = below < 65536u ? (float)(65536.0 / (65536u - below)) : 0.f;
   hipStream_t st = gfn_stream(stream);
@@ -100,6 +104,7 @@ int gfn_dropout(const void* x, int64_t ldx, int64_t rows, int cols, int dtype, f
 
 int gfn_dropout_call(uint64_t* counter, uint64_t* call, void* stream) {
   GFN_CHECK_ARG(counter && call, "gfn_dropout_call: null pointer");
+  GFN_CHECK_ARG(!gfn_overlap(gfn_flat("counter", counter, 1, 8), gfn_flat("call", call, 1, 8)), "gfn_dropout_call: call overlaps counter");
   dropout_call_kernel<<<1, 1, 0, gfn_stream(stream)>>>(reinterpret_cast<unsigned long long*>(counter), reinterpret_cast<unsigned long long*>(call));
   GFN_CHECK_LAUNCH();
   return GFN_OK;

@@ -775,6 +775,12 @@ int gfn_gated_fwd(const void* x, int64_t ldx, const void* wg, const void* wu, co
   GFN_CHECK_ARG(x && wg && wu && out, "gfn_gated_fwd: null pointer");
   GFN_CHECK_ARG(!bg == !bu, "gfn_gated_fwd: one bias without the other");
   GFN_CHECK_ARG(ldx >= in_dim && ldo >= hidden, "gfn_gated_fwd: row strides %lld / %lld below %d / %d", (long long)ldx, (long long)ldo, in_dim, hidden);
+  const int size = dtype == GFN_F32 ? 4 : 2;
+  const int64_t weights = (int64_t)hidden * in_dim;
+  if (int rc = gfn_check_apart("gfn_gated_fwd", {{"out", out, n_max, hidden, ldo, size}},
+                               {{"x", x, n_max, in_dim, ldx, size}, gfn_flat("wg", wg, weights, size), gfn_flat("wu", wu, weights, size), gfn_flat("bg", bg, hidden, size),
+                                gfn_flat("bu", bu, hidden, size), gfn_flat("n_dev", n_dev, 1, 4)}))
+    return rc;
   const GatedFwd a{x, wg, wu, bg, bu, ldx, ldo, n_max, n_dev, in_dim, hidden, act, out};
   hipStream_t st = gfn_stream(stream);
   if (dtype == GFN_F32) return dispatch_fwd<float>(a, st);
@@ -803,6 +809,14 @@ int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, co
   const int64_t need = gfn_gated_bwd_workspace(n_max, in_dim, hidden, dtype, bg != nullptr, dx != nullptr, dwg != nullptr);
   GFN_CHECK_ARG(workspace_bytes >= need && (need == 0 || workspace), "gfn_gated_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   if (n_max == 0 && !dwg) return GFN_OK;
+  const int size = dtype == GFN_F32 ? 4 : 2;
+  const int64_t weights = (int64_t)hidden * in_dim;
+  if (int rc = gfn_check_apart("gfn_gated_bwd",
+                               {{"dx", dx, n_max, in_dim, lddx, size}, gfn_flat("dwg", dwg, weights, size), gfn_flat("dwu", dwu, weights, size), gfn_flat("dbg", dbg, hidden, size),
+                                gfn_flat("dbu", dbu, hidden, size), gfn_flat("the workspace", workspace, need, 1)},
+                               {{"x", x, n_max, in_dim, ldx, size}, {"dh", dh, n_max, hidden, lddh, size}, gfn_flat("wg", wg, weights, size), gfn_flat("wu", wu, weights, size),
+                                gfn_flat("bg", bg, hidden, size), gfn_flat("bu", bu, hidden, size), gfn_flat("n_dev", n_dev, 1, 4)}))
+    return rc;
   const BwdPlan p = plan_bwd(n_max, in_dim, hidden, dtype, bg != nullptr);
   GatedBwd a{};
   a.n_max = n_max; a.n_dev = n_dev;

@@ -44,6 +44,36 @@ static inline hipStream_t gfn_stream(void* s) { return reinterpret_cast<hipStrea
 // library does may end up inside a caller's capture (a training step, a forward, a render tile), so none of them is a memset.
 hipError_t gfn_zero_async(void* p, size_t bytes, hipStream_t stream);
 
+// Rows of a tensor in memory, for the checks of what a call writes against what it reads: `rows` of `width` elements of `size` bytes, `ld` apart.
+struct gfn_rows {
+  const char* name;
+  const void* p;
+  int64_t rows, width, ld;
+  int size;
+};
+inline gfn_rows gfn_flat(const char* name, const void* p, int64_t n, int size) { return {name, p, 1, n, n, size}; }
+// Whether two share a byte.  Rows of one stride may lie beside each other in a buffer (columns of a wider tensor); otherwise their extents
+// must not meet.
+inline bool gfn_overlap(const gfn_rows& a, const gfn_rows& b) {
+  if (!a.p || !b.p || a.rows < 1 || b.rows < 1 || a.width < 1 || b.width < 1) return false;
+  const int64_t pa = (int64_t)reinterpret_cast<intptr_t>(a.p), pb = (int64_t)reinterpret_cast<intptr_t>(b.p);
+  const int64_t wa = a.width * a.size, wb = b.width * b.size, sa = a.ld * a.size, sb = b.ld * b.size;
+  if (pa + (a.rows - 1) * sa + wa <= pb || pb + (b.rows - 1) * sb + wb <= pa) return false;
+  if ((a.rows > 1 && b.rows > 1 && sa != sb) || (a.rows == 1 && b.rows == 1)) return true;
+  const int64_t s = a.rows > 1 ? sa : sb, off = ((pb - pa) % s + s) % s;  // b's columns in a's rows
+  return off < wa || off + wb > s;
+}
+inline bool gfn_same_rows(const gfn_rows& a, const gfn_rows& b) { return a.p == b.p && a.size == b.size && (a.ld == b.ld || (a.rows == 1 && b.rows == 1)); }
+// Refuses outputs that overlap an input or each other: their rows are written while other workgroups still read.
+template <int O, int I>
+inline int gfn_check_apart(const char* who, const gfn_rows (&out)[O], const gfn_rows (&in)[I]) {
+  for (int o = 0; o < O; o++) {
+    for (int i = 0; i < I; i++) GFN_CHECK_ARG(!gfn_overlap(out[o], in[i]), "%s: %s overlaps %s", who, out[o].name, in[i].name);
+    for (int i = 0; i < o; i++) GFN_CHECK_ARG(!gfn_overlap(out[o], out[i]), "%s: %s overlaps %s", who, out[o].name, out[i].name);
+  }
+  return GFN_OK;
+}
+
 // One-time set-up per (call site, device), e.g. hipFuncSetAttribute for a kernel's dynamic LDS size: true the first time it is
 // reached with the current device selected (`seen`: a function-local static, one bit per device ordinal).
 static inline bool gfn_first_call_on_device(unsigned long long& seen) {

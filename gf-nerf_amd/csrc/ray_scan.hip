@@ -725,6 +725,14 @@ int dispatch_scan(const char* who, const ScanArgs& a, int dtype, int gate, bool 
   const int64_t need = scan_workspace(a.rays, a.n_max, a.d, a.g);
   GFN_CHECK_ARG(bytes >= need && (need == 0 || workspace), "%s: workspace of %lld bytes, %lld needed", who, (long long)bytes, (long long)need);
   if (a.rays == 0 && !(a.clear && a.n_max > 0)) return GFN_OK;
+  const int size = dtype == GFN_F32 ? 4 : 2;
+  const int64_t n = a.n_max, states = a.rays * a.d, blocks = (n + kBlock - 1) / kBlock * a.d;
+  if (int rc = gfn_check_apart(who,
+                               {{"h", a.h, n, a.d, a.ldh, size}, {"df", a.df, n, a.g, a.lddf, size}, {"dc", a.dc, n, a.d, a.lddc, size}, gfn_flat("state", a.state, states, 4),
+                                gfn_flat("saved", a.saved, blocks, 4), gfn_flat("dh0", a.dh0, states, 4), gfn_flat("the workspace", workspace, need, 1)},
+                               {gfn_flat("pts_offsets", a.offsets, a.rays + 1, 4), {"f", a.f, n, a.g, a.ldf, size}, {"c", a.c, n, a.d, a.ldc, size}, {"dh", a.dh, n, a.d, a.lddh, size},
+                                gfn_flat("h0", a.h0, states, 4), gfn_flat("d_state", a.d_state, states, 4), gfn_flat("saved", a.saved_in, blocks, 4)}))
+    return rc;
   char* ws = static_cast<char*>(workspace);
   if (dtype == GFN_F32) return dispatch_gate<float>(a, gate, bwd, ws, st);
   if (dtype == GFN_BF16) return dispatch_gate<__bf16>(a, gate, bwd, ws, st);
@@ -781,6 +789,12 @@ int gfn_ray_scan_step(const void* f, int64_t ldf, const void* c, int64_t ldc, in
   ScanArgs a{};
   a.rays = n_rays; a.f = f; a.ldf = ldf; a.c = c; a.ldc = ldc; a.h = h; a.ldh = ldh; a.state = state;
   a.d = channels; a.g = gates; a.per_gate = channels / gates;
+  // a thread reads its row's gate and its channel of c and of the state and writes state and h: what lies in the same places may be the same
+  const int size = dtype == GFN_F32 ? 4 : 2;
+  const gfn_rows rf{"f", f, n_rays, gates, ldf, size}, rc{"c", c, n_rays, channels, ldc, size}, rh{"h", h, n_rays, channels, ldh, size}, rs{"state", state, n_rays, channels, channels, 4};
+  if (int e = gfn_check_apart("gfn_ray_scan_step", {rh, rs}, {gates == channels && gfn_same_rows(rs, rf) ? gfn_rows{} : rf})) return e;
+  GFN_CHECK_ARG(gfn_same_rows(rh, rc) || !gfn_overlap(rh, rc), "gfn_ray_scan_step: h overlaps c");
+  GFN_CHECK_ARG(gfn_same_rows(rs, rc) || !gfn_overlap(rs, rc), "gfn_ray_scan_step: state overlaps c");
   const int64_t blocks = (n_rays * channels + 255) / 256;
   const unsigned grid = (unsigned)(blocks < 8192 ? blocks : 8192);
   hipStream_t st = gfn_stream(stream);

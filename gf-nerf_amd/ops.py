@@ -1435,13 +1435,6 @@ def _flat(t, dtype, name, shape):
     raise _lib.GfnError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _apart(out, *inputs):
-    """The output is not one of the inputs (rows are read by other workgroups while it is written): their addresses -> out's."""
-    if out and out in inputs:
-        raise _lib.GfnError("out is one of the inputs")
-    return out
-
-
 def _gated_args(x, Wg, Wu, bg, bu, act, n_dev, what):
     n, k, ldx = _rows(x, "x")
     if act not in GATED_ACT:
@@ -1460,14 +1453,14 @@ def _gated_args(x, Wg, Wu, bg, bu, act, n_dev, what):
 def gated_fwd(x, Wg, Wu, bg=None, bu=None, act="silu", out=None, n_dev=None):
     """h = act(x Wg^T + bg) * (x Wu^T + bu): both projections, the activation and the product in one launch.  x [n, in] (rows at any
     stride), Wg / Wu [hidden, in], bg / bu [hidden] or both None; f32, bf16 or f16 throughout, sums in f32; act "silu", "gelu" (erf),
-    "relu" or "sigmoid"; in 1..128, hidden 1..1024.  n_dev i32 [1]: live rows (those behind are left alone)."""
+    "relu" or "sigmoid"; in 1..128, hidden 1..1024.  n_dev i32 [1]: live rows (those behind are left alone).  out may be columns of the buffer
+    that x is columns of, but shares no element with an input."""
     n, k, h, ldx, dtype = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_fwd")
     if out is None:
         out = x.new_empty((n, h))
     ldo = _rows(out, "out", dtype, h, n)[2]
     stream = _place(x, Wg, Wu, bg, bu, n_dev, out)
-    at = [_at(t) for t in (x, Wg, Wu, bg, bu)]
-    rc = _lib.lib().gfn_gated_fwd(at[0], ldx, at[1], at[2], at[3], at[4], n, _at(n_dev), k, h, DTYPES[dtype], GATED_ACT[act], _apart(out.data_ptr(), *at), ldo, stream)
+    rc = _lib.lib().gfn_gated_fwd(_at(x), ldx, _at(Wg), _at(Wu), _at(bg), _at(bu), n, _at(n_dev), k, h, DTYPES[dtype], GATED_ACT[act], _at(out), ldo, stream)
     _lib.check(rc, "gfn_gated_fwd")
     return out
 
@@ -1521,7 +1514,8 @@ def ray_scan_fwd(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, out=
       gate "linear": a = f, b = c;  "sigmoid": a = sigmoid(f), b = (1 - a) c;  "decay": a = exp(-f), b = (1 - a) c -- with f = sigma dt and
       reverse, the first sample's h is the composite of `channels` feature channels.
     h0 f32 [rays, channels] or None (0).  -> dict(h [n, channels], state f32 [rays, channels] (every ray's last state), saved (save=True:
-    what ray_scan_bwd needs)).  Rows behind the last ray's: 0 in an h allocated here, left alone in `out`."""
+    what ray_scan_bwd needs)).  Rows behind the last ray's: 0 in an h allocated here, left alone in `out`, which shares no element with an
+    input."""
     R = _scan_rays(pts_offsets, "ray_scan_fwd")
     n, d, g, ldf, ldc, dtype = _scan_args(f, c, gate, "ray_scan_fwd")
     _flat(h0, torch.float32, "h0", (R, d))
@@ -1531,8 +1525,7 @@ def ray_scan_fwd(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, out=
     state = c.new_empty((R, d), dtype=torch.float32)
     ws, size = _scan_workspace(R, n, d, g, c)
     saved = c.new_empty(((n + SCAN_BLOCK - 1) // SCAN_BLOCK, d), dtype=torch.float32) if save else None
-    at = _at(f), _at(c), _at(h0)
-    rc = _lib.lib().gfn_ray_scan_fwd(_at(pts_offsets), R, at[0], ldf, at[1], ldc, n, d, g, DTYPES[dtype], SCAN_GATE[gate], int(reverse), at[2], _apart(h.data_ptr(), *at), ldh,
+    rc = _lib.lib().gfn_ray_scan_fwd(_at(pts_offsets), R, _at(f), ldf, _at(c), ldc, n, d, g, DTYPES[dtype], SCAN_GATE[gate], int(reverse), _at(h0), _at(h), ldh,
                                      _at(state), _at(saved), out is None, _at(ws), size, stream)
     _lib.check(rc, "gfn_ray_scan_fwd")
     return dict(h=h, state=state, saved=saved)
@@ -1560,7 +1553,7 @@ def ray_scan_bwd(pts_offsets, f, c, dh, saved, gate="sigmoid", reverse=False, h0
 
 def ray_scan_step(f, c, state, gate="sigmoid", out=None):
     """One more sample of every ray: state [rays, channels] f32 <- a state + b, in place; -> h [rays, channels] in c's dtype.  f [rays, gates],
-    c [rays, channels] as in ray_scan_fwd."""
+    c [rays, channels] as in ray_scan_fwd; out may be c."""
     n, d, g, ldf, ldc, dtype = _scan_args(f, c, gate, "ray_scan_step")
     if state is None:
         raise _lib.GfnError("ray_scan_step: state is missing")
@@ -1568,8 +1561,7 @@ def ray_scan_step(f, c, state, gate="sigmoid", out=None):
     h = c.new_empty((n, d)) if out is None else out
     ldh = _rows(h, "out", dtype, d, n)[2]
     stream = _place(f, c, state, h)
-    at = _at(f), _at(state)
-    rc = _lib.lib().gfn_ray_scan_step(at[0], ldf, _at(c), ldc, n, d, g, DTYPES[dtype], SCAN_GATE[gate], at[1], _apart(h.data_ptr(), *at), ldh, stream)
+    rc = _lib.lib().gfn_ray_scan_step(_at(f), ldf, _at(c), ldc, n, d, g, DTYPES[dtype], SCAN_GATE[gate], _at(state), _at(h), ldh, stream)
     _lib.check(rc, "gfn_ray_scan_step")
     return h
 
@@ -1589,7 +1581,8 @@ def dropout_call(counter):
 def dropout(x, p, seed, call, out=None):
     """y = x where the element is kept, times 65536 / (65536 - t), t = round(65536 p); 0 where it is dropped.  Which elements are kept is a
     function of (seed, call, row, column) -- Philox4x32-10, 16 bits an element -- and never stored: the gradient is the same call on dy.
-    x [n, columns] (f32, bf16 or f16, rows at any stride), call i64 [1] (dropout_call); out may be x."""
+    x [n, columns] (f32, bf16 or f16, rows at any stride), call i64 [1] (dropout_call); out may be x, but not
+    overlap it otherwise."""
     n, d, ldx = _rows(x, "x")
     if call is None:
         raise _lib.GfnError("dropout: call is missing")

@@ -752,6 +752,8 @@ int gfn_octree_fit_weight_host(const float* w2xz, const float* pts, int64_t n_pt
  * Sequence-head operators: a gated feed-forward layer on every sample, dropout, and a
  * gated linear recurrence along each ray's packed samples.  No reference
  * counterpart: they stand beside gfn_linear_*, gfn_step_draws and gfn_composite_*.
+ * What a call writes must not overlap what it reads or what else it writes, unless said otherwise (refused); columns of one wider
+ * buffer that lie beside each other do not.
  * Element types of their tensors: */
 typedef enum { GFN_F32 = 0, GFN_BF16 = 1, GFN_F16 = 2 } gfn_dtype;
 
@@ -797,7 +799,7 @@ int gfn_ray_scan_bwd(const int32_t* pts_offsets, int64_t n_rays, const void* f, 
                      const void* dh, int64_t lddh, int64_t n_max, int channels, int gates, int dtype, int gate, int reverse,
                      const float* h0, const float* d_state, const float* saved, void* df, int64_t lddf, void* dc, int64_t lddc,
                      float* dh0, int clear_tail, void* workspace, int64_t workspace_bytes, void* stream);
-/* One more sample of every ray: state[r] = a state[r] + b in place, h [n_rays, channels] = state rounded to dtype. */
+/* One more sample of every ray: state[r] = a state[r] + b in place, h [n_rays, channels] = state rounded to dtype; h may be c. */
 int gfn_ray_scan_step(const void* f, int64_t ldf, const void* c, int64_t ldc, int64_t n_rays, int channels, int gates,
                       int dtype, int gate, float* state, void* h, int64_t ldh, void* stream);
 

@@ -324,3 +324,36 @@ def test_runs_pass_over_long_stretches_of_rays_without_rows(T, ops, kind, revers
     few_h0 = h0[at].contiguous()
     best(few, few_h0)
     assert best(off, h0) <= 4 * best(few, few_h0)
+
+
+# ---- outputs beside and over inputs ---------------------------------------------------------------------------------------------------------------
+def test_outputs_beside_inputs_in_one_buffer(T, ops):
+    """Columns of one buffer, input and output beside each other, are taken; one column in common is refused, and nothing is written."""
+    from gfnerf_amd import _lib
+
+    x, wg, wu, bg, bu, _ = gated_inputs(T, "f32", 500, 31, 40, True, "silu")
+    want = ops.gated_fwd(x[0], wg[0], wu[0], bg[0], bu[0])
+    buf = T.zeros(500, 80, device="cuda")
+    for first, out in ((0, 31), (45, 0), (45, 5)):
+        buf[:, first:first + 31] = x[0]
+        ops.gated_fwd(buf[:, first:first + 31], wg[0], wu[0], bg[0], bu[0], out=buf[:, out:out + 40])
+        assert T.equal(buf[:, out:out + 40], want)
+    before = buf.clone()
+    off = T.tensor([0, 250, 500], dtype=T.int32, device="cuda")
+    f = T.zeros(500, 8, device="cuda")
+    state = T.zeros(500, 8, device="cuda")
+    call = T.zeros(1, dtype=T.int64, device="cuda")
+    for bad in (lambda: ops.gated_fwd(buf[:, 0:31], wg[0], wu[0], bg[0], bu[0], out=buf[:, 30:70]), lambda: ops.gated_fwd(buf[:, 45:76], wg[0], wu[0], bg[0], bu[0], out=buf[:, 6:46]),
+                lambda: ops.gated_fwd(buf[:400, 0:31], wg[0], wu[0], bg[0], bu[0], out=buf.view(-1)[7:7 + 400 * 60].view(400, 60)[:, :40]),
+                lambda: ops.ray_scan_fwd(off, f, buf[:, 0:8], out=buf[:, 7:15]), lambda: ops.ray_scan_step(f, buf[:, 0:8], state, out=buf[:, 1:9]),
+                lambda: ops.dropout(buf[:, 0:8], 0.5, 1, call, out=buf[:, 7:15]), lambda: ops.dropout(buf[1:, :8], 0.5, 1, call, out=buf[:-1, :8])):
+        with pytest.raises(_lib.GfnError, match="overlaps"):
+            bad()
+    T.cuda.synchronize()
+    assert T.equal(buf, before) and not bool(state.any())
+    h = ops.ray_scan_fwd(off, f, buf[:, 0:8], out=buf[:, 8:16])["h"]
+    assert T.equal(h, ops.ray_scan_fwd(off, f, before[:, 0:8])["h"])
+    c = before[:, 0:8].contiguous()
+    s = state.clone()
+    want = ops.ray_scan_step(f, c, s)
+    assert T.equal(ops.ray_scan_step(f, c, state, out=c), want) and T.equal(state, s)  # h may be c

@@ -1,4 +1,7 @@
-"""The sequence-head operators without a GPU, where their numbers end: what the oracle's bounds let through."""
+"""The sequence-head operators without a GPU, where their numbers end: what the oracle's bounds let through, and calls whose outputs
+overlap their inputs."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -36,3 +39,75 @@ def test_the_f16_bound_sees_what_a_power_from_dh_loses(low, seen):
     from_dh = -4 * ((int(np.frexp(np.abs(dh).max())[1])) // 4) - 4
     own = (15 - np.frexp(np.abs(dz).max((0, 2)))[1]) // 8 * 8
     assert (outside(from_dh) > 0) == seen and outside(own[:, None]) == 0
+
+
+# ---- outputs that overlap inputs: refused before anything is launched ------------------------------------------------------------------------
+def at(byte):
+    return C.c_void_p((1 << 40) + byte)
+
+
+FAR = {name: at((i + 1) << 30) for i, name in enumerate(("x", "wg", "wu", "bg", "bu", "dh", "f", "c", "h0", "off", "saved", "out"))}
+
+
+def refused(name, *args, match):
+    import gfnerf_amd  # noqa: F401
+    from gfnerf_amd import _lib
+
+    assert getattr(_lib.lib(), name)(*args) == -1
+    assert match in _lib.lib().gfn_last_error().decode(), _lib.lib().gfn_last_error().decode()
+
+
+@pytest.mark.parametrize("x,ldx,out,ldo,match", [
+    (at(0), 63, at(100 * 63 * 4 - 4), 128, "out overlaps x"),         # its last element
+    (at(128 * 99 * 4 + 127 * 4), 63, at(0), 128, "out overlaps x"),    # out's last element is x's first
+    (at(0), 200, at(62 * 4), 200, "out overlaps x"),                  # columns 0 .. 62 and 62 .. 189 of one buffer
+    (at(0), 200, at(100 * 4), 200, "out overlaps x"),                 # columns 100 .. 227: the next row's first
+    (at(0), 200, at(63 * 4 + 200 * 4 * 50), 201, "out overlaps x"),   # another stride inside the same extent
+    (FAR["x"], 63, at((2 << 30) + 8), 128, "out overlaps wg"), (FAR["x"], 63, at((3 << 30) - 128 * 4 * 100 + 4), 128, "out overlaps wu"),
+    (FAR["x"], 63, at((4 << 30) + 127 * 4), 128, "out overlaps bg"), (FAR["x"], 63, at(5 << 30), 128, "out overlaps bu")])
+def test_gated_fwd_refuses_overlap(x, ldx, out, ldo, match):
+    refused("gfn_gated_fwd", x, ldx, FAR["wg"], FAR["wu"], FAR["bg"], FAR["bu"], 100, None, 63, 128, 0, 0, out, ldo, None, match=match)
+
+
+@pytest.mark.parametrize("change,match", [(dict(dx=FAR["x"]), "dx overlaps x"), (dict(dx=at((6 << 30) + 4)), "dx overlaps dh"), (dict(dwg=FAR["wg"]), "dwg overlaps wg"),
+                                          (dict(dwu=at((20 << 30) + 4)), "dwu overlaps dwg"), (dict(dbu=at(22 << 30)), "dbu overlaps dbg"),
+                                          (dict(ws=at(6 << 30)), "the workspace overlaps dh")])
+def test_gated_bwd_refuses_overlap(change, match):
+    a = dict(dx=FAR["out"], dwg=at(20 << 30), dwu=at(21 << 30), dbg=at(22 << 30), dbu=at(23 << 30), ws=at(24 << 30))
+    a.update(change)
+    refused("gfn_gated_bwd", FAR["x"], 63, FAR["wg"], FAR["wu"], FAR["bg"], FAR["bu"], FAR["dh"], 128, 100, None, 63, 128, 0, 0, a["dx"], 63, a["dwg"], a["dwu"], a["dbg"],
+            a["dbu"], a["ws"], 1 << 29, None, match=match)
+
+
+@pytest.mark.parametrize("change,match", [(dict(h=at((8 << 30) + 4)), "h overlaps c"), (dict(h=FAR["f"]), "h overlaps f"), (dict(state=FAR["h0"]), "state overlaps h0"),
+                                          (dict(saved=at((9 << 30) + 12)), "saved overlaps h0"), (dict(state=FAR["off"]), "state overlaps pts_offsets"),
+                                          (dict(saved=at((30 << 30) + 8)), "saved overlaps state")])
+def test_ray_scan_fwd_refuses_overlap(change, match):
+    a = dict(h=FAR["out"], state=at(30 << 30), saved=at(31 << 30))
+    a.update(change)
+    refused("gfn_ray_scan_fwd", FAR["off"], 10, FAR["f"], 8, FAR["c"], 32, 100, 32, 8, 0, 1, 0, FAR["h0"], a["h"], 32, a["state"], a["saved"], 0, None, 0, None, match=match)
+
+
+@pytest.mark.parametrize("change,match", [(dict(df=FAR["f"]), "df overlaps f"), (dict(dc=FAR["dh"]), "dc overlaps dh"), (dict(dc=at((8 << 30) + 64)), "dc overlaps c"),
+                                          (dict(dh0=FAR["h0"]), "dh0 overlaps h0"), (dict(dc=FAR["saved"]), "dc overlaps saved"), (dict(dc=at((30 << 30) + 4)), "dc overlaps df")])
+def test_ray_scan_bwd_refuses_overlap(change, match):
+    a = dict(df=at(30 << 30), dc=at(31 << 30), dh0=at(32 << 30))
+    a.update(change)
+    refused("gfn_ray_scan_bwd", FAR["off"], 10, FAR["f"], 8, FAR["c"], 32, FAR["dh"], 32, 100, 32, 8, 0, 1, 0, FAR["h0"], None, FAR["saved"], a["df"], 8, a["dc"], 32, a["dh0"], 0,
+            None, 0, None, match=match)
+
+
+def test_ray_scan_step_and_dropout_refuse_overlap():
+    step = lambda f, c, state, h, ldh=32: ("gfn_ray_scan_step", f, 8, c, 32, 10, 32, 8, 0, 1, state, h, ldh, None)  # noqa: E731
+    refused(*step(FAR["f"], FAR["c"], FAR["h0"], at((8 << 30) + 4)), match="h overlaps c")
+    refused(*step(FAR["f"], FAR["c"], FAR["h0"], FAR["c"], 33), match="h overlaps c")
+    refused(*step(FAR["f"], FAR["c"], FAR["h0"], FAR["f"]), match="h overlaps f")
+    refused(*step(FAR["f"], FAR["c"], FAR["h0"], FAR["h0"]), match="state overlaps h")
+    refused(*step(FAR["f"], FAR["c"], at((8 << 30) + 128), FAR["out"]), match="state overlaps c")
+    refused(*step(FAR["f"], FAR["c"], FAR["f"], FAR["out"]), match="state overlaps f")
+    drop = lambda x, ldx, y, ldy, call=FAR["off"]: ("gfn_dropout", x, ldx, 100, 64, 0, 0.5, 1, call, y, ldy, None)  # noqa: E731
+    refused(*drop(FAR["x"], 64, at((1 << 30) + 4), 64), match="y overlaps x")
+    refused(*drop(FAR["x"], 64, FAR["x"], 65), match="y overlaps x")
+    refused(*drop(FAR["x"], 100, at((1 << 30) + 40 * 4), 100), match="y overlaps x")
+    refused(*drop(FAR["x"], 64, FAR["out"], 64, at((12 << 30) + 8)), match="y overlaps call")
+    refused("gfn_dropout_call", FAR["x"], FAR["x"], None, match="call overlaps counter")
