@@ -82,7 +82,7 @@ def build_extension(force=False, verbose=False):
 
 def _build_locked(force, verbose):
     os.makedirs(OBJ, exist_ok=True)
-    headers = [os.path.join(CSRC, h) for h in ("gfn_common.h", "x3_device.h", "hash_device.h", "gated_device.h")]
+    headers = [os.path.join(CSRC, h) for h in ("gfn_common.h", "gfn_once.h", "x3_device.h", "hash_device.h", "gated_device.h")]
     headers += [os.path.join(INCLUDE, "gfnerf_amd.h")]
     hipcc = _hipcc()
     jobs, objs, keys = [], [], []

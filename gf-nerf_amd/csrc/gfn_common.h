@@ -5,6 +5,7 @@
 #include <stdio.h>
 
 #include "../../include/gfnerf_amd.h"
+#include "gfn_once.h"
 
 static_assert(sizeof(gfn_tree_node) == GFN_TREE_NODE_BYTES, "TreeNode ABI (PersSampler.h:39-48)");
 static_assert(sizeof(gfn_trans_info) == GFN_TRANS_INFO_BYTES, "TransInfo ABI (PersSampler.h:31-37)");
@@ -74,15 +75,12 @@ inline int gfn_check_apart(const char* who, const gfn_rows (&out)[O], const gfn_
   return GFN_OK;
 }
 
-// One-time set-up per (call site, device), e.g. hipFuncSetAttribute for a kernel's dynamic LDS size: true the first time it is
-// reached with the current device selected (`seen`: a function-local static, one bit per device ordinal).
+// One-time set-up per (call site, device), e.g. hipFuncSetAttribute for a kernel's dynamic LDS size: true where the calling thread has to
+// run it for the current device (`seen`: a function-local static, one bit per device ordinal).
 static inline bool gfn_first_call_on_device(unsigned long long& seen) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return true;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (seen & bit) return false;
-  seen |= bit;
-  return true;
+  return gfn_first_call(seen, dev);
 }
 
 // live element count: device value if given, else the host capacity.

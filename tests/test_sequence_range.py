@@ -1,6 +1,8 @@
 """The sequence-head operators without a GPU, where their numbers end: what the oracle's bounds let through, and calls whose outputs
-overlap their inputs."""
+overlap their inputs, and the first call of two threads at once."""
 import ctypes as C
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -111,3 +113,34 @@ def test_ray_scan_step_and_dropout_refuse_overlap():
     refused(*drop(FAR["x"], 100, at((1 << 30) + 40 * 4), 100), match="y overlaps x")
     refused(*drop(FAR["x"], 64, FAR["out"], 64, at((12 << 30) + 8)), match="y overlaps call")
     refused("gfn_dropout_call", FAR["x"], FAR["x"], None, match="call overlaps counter")
+
+
+ONCE = r"""
+#include <atomic>
+#include <cstdio>
+#include <thread>
+#include "gfn_once.h"
+static unsigned long long seen = 0, other = 0;
+int main() {
+  std::atomic<int> step{0};
+  bool a1, a2, b1, b2, c1;
+  std::thread a([&] { a1 = gfn_first_call(seen, 3); step = 1; while (step != 2) std::this_thread::yield(); a2 = gfn_first_call(seen, 3); });
+  std::thread b([&] { while (step != 1) std::this_thread::yield(); b1 = gfn_first_call(seen, 3); step = 2; });  // while a's set-up is under way
+  a.join(); b.join();
+  std::thread c([&] { c1 = gfn_first_call(seen, 3); b2 = gfn_first_call(seen, 4); });
+  c.join();
+  bool d = true;  // a thread that meets more call sites than it remembers runs their set-up again rather than go without
+  static unsigned long long sites[1000];
+  for (auto& s : sites) d = d && gfn_first_call(s, 0);
+  for (int i = 900; i < 1000; i++) d = d && gfn_first_call(sites[i], 0);
+  std::printf("%d %d %d %d %d %d %d", a1, a2, b1, c1, b2, gfn_first_call(other, 0), d);
+}
+"""
+
+
+def test_two_threads_in_a_first_call_both_run_its_set_up(tmp_path):
+    """The set-up in front of a launch (a kernel's LDS limit) is complete for every thread that gets past it, not only for the one that came first."""
+    (tmp_path / "once.cpp").write_text(ONCE)
+    exe = str(tmp_path / "once")
+    subprocess.check_call(["g++", "-O2", "-std=c++17", "-pthread", "-I", os.path.join(ROOT, "gf-nerf_amd", "csrc"), str(tmp_path / "once.cpp"), "-o", exe])
+    assert subprocess.check_output([exe], text=True, timeout=60) == "1 0 1 0 1 1 1"
