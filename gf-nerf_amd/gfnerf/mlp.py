@@ -15,7 +15,8 @@ from .. import _lib, ops
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, W, b, act):
+    def forward(ctx, x, W, b, act, alive=None):
+        ctx.alive = alive
         x = x.contiguous()
         y = ops.linear_fwd(x, W.contiguous(), b.contiguous(), act)
         ctx.save_for_backward(x, W, y)
@@ -26,7 +27,7 @@ class _LinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, W, y = ctx.saved_tensors
         dx, dW, db = ops.linear_bwd(x, W.contiguous(), y, dy.contiguous(), ctx.act, need_dx=ctx.needs_input_grad[0])
-        return dx, dW, db, None
+        return dx, dW, db, None, None
 
 
 class MLPNetwork(nn.Module):
@@ -66,7 +67,8 @@ def one_graph_at_a_time(*tensors):
     """What a forward of these tensors holds on to while its autograd graph lives (None: nothing is recorded).  Refuses to
     record a forward into a hipGraph while an eager autograd graph of the same leaves lives.  The leaf's gradient accumulator
     belongs to that graph and to its stream; a captured backward would wait for a stream outside the capture, and ending the capture then ends
-    the process.  Drop the eager outputs (or detach them) before capturing."""
+    the process.  Drop the eager outputs (or detach them) before capturing.  Of leaves that a caller's own operations stand in front of nothing is
+    known here."""
     leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf] if torch.is_grad_enabled() else []
     if not leaves:
         return None
@@ -168,11 +170,11 @@ class GatedMLPNetwork(nn.Module):
         self.dropout = nn.ModuleList(Dropout(p, seed + i) for i in range(self.n_hidden_layers)) if p else None
 
     def forward(self, x):
-        shape = x.shape[:-1]
+        out, shape = self.layers[-1], x.shape[:-1]
+        alive = one_graph_at_a_time(x, out.weight, out.bias)  # the hidden layers see to their own
         x = x.reshape(-1, x.shape[-1]).float()
         for i in range(self.n_hidden_layers):
             x = self.layers[i](x)
             if self.dropout is not None:
                 x = self.dropout[i](x)
-        out = self.layers[-1]
-        return _LinearFn.apply(x, out.weight, out.bias, "sigmoid" if self.sigmoid_out else "none").reshape(*shape, -1)
+        return _LinearFn.apply(x, out.weight, out.bias, "sigmoid" if self.sigmoid_out else "none", alive).reshape(*shape, -1)

@@ -28,7 +28,7 @@ class _RayScanFn(torch.autograd.Function):
 
 
 def ray_scan(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, leaves=()):
-    """ops.ray_scan_fwd with gradients for f, c and h0 -> (h [n, channels], state f32 [rays, channels]).  leaves: the parameters that f and c were
+    """ops.ray_scan_fwd with gradients for f, c and h0 -> (h [n, channels], state f32 [rays, channels]).  leaves: the tensors that f and c were
     made from, where nothing else keeps a capture of this forward apart from an eager graph of theirs (one_graph_at_a_time)."""
     alive = one_graph_at_a_time(f, c, h0, *leaves)
     save = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (f, c, h0))
@@ -41,7 +41,7 @@ def render_features(pts_offsets, sigma, dt, features):
     h = exp(-sigma dt) h + alpha c taken back to front: no weights array, any number of channels.  sigma dt is formed in f32 and rounded once
     to the features' dtype (the recurrence takes its gates and inputs in one type): with 16-bit features a weight is off by half a step of it."""
     thickness = (sigma.reshape(-1) * dt.reshape(-1)).to(features.dtype)
-    return ray_scan(pts_offsets, thickness[:, None], features, "decay", reverse=True)[1]
+    return ray_scan(pts_offsets, thickness[:, None], features, "decay", reverse=True, leaves=(sigma, dt))[1]
 
 
 class RayRecurrence(nn.Module):
@@ -60,7 +60,7 @@ class RayRecurrence(nn.Module):
     def forward(self, x, pts_offsets, state=None):
         """x [n, n_input_dims] packed -> (h [n, dim], state [rays, dim]); state: the rays' states in front of x (default 0)."""
         f, c = self._project(x)
-        return ray_scan(pts_offsets, f, c, "sigmoid", self.reverse, state, tuple(self.parameters()))
+        return ray_scan(pts_offsets, f, c, "sigmoid", self.reverse, state, (x, *self.parameters()))
 
     @torch.no_grad()
     def step(self, x, state):
