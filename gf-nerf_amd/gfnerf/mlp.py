@@ -121,7 +121,8 @@ class _DropoutFn(torch.autograd.Function):
 
 class Dropout(nn.Module):
     """Dropout over the last dimension with a mask that is never stored (ops.dropout): a function of the module's seed, the number of its
-    forward passes in training mode (`counter`, on the device: replayed graphs draw fresh masks), the row and the column."""
+    forward passes in training mode (`counter`, on the device: replayed graphs draw fresh masks), the row and the column.  Every forward pass
+    draws a mask of its own, so one that is run again inside a backward pass is refused."""
 
     def __init__(self, p: float = 0.5, seed: int = 0):
         super().__init__()
@@ -133,6 +134,9 @@ class Dropout(nn.Module):
     def forward(self, x):
         if not self.training or self.p == 0.0:
             return x
+        if torch._C._current_graph_task_id() != -1:
+            raise _lib.GfnError("a dropout is recomputed inside a backward pass (torch.utils.checkpoint): it would draw another mask than its first forward; "
+                                "leave it outside of the recomputed part (it keeps nothing of its input)")
         alive = one_graph_at_a_time(x)
         return _DropoutFn.apply(x.reshape(-1, x.shape[-1]).contiguous(), self.p, self.seed, ops.dropout_call(self.counter), alive).reshape(x.shape)
 

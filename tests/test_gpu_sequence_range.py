@@ -402,3 +402,27 @@ def test_a_capture_beside_a_live_eager_graph_of_any_leaf_is_refused(T, i):
     with T.cuda.graph(T.cuda.CUDAGraph()):  # without it the capture is taken
         out = forward()
     T.cuda.synchronize()
+
+
+# ---- dropout modules ------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_recomputed_dropout_is_refused(T, reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    from gfnerf_amd import _lib
+    from gfnerf_amd.gfnerf.mlp import Dropout, gated_linear
+
+    drop = Dropout(0.5, seed=1).cuda()
+    x, w = T.randn(64, 16, device="cuda", requires_grad=True), T.randn(32, 16, device="cuda", requires_grad=True)
+    y = checkpoint(lambda v: gated_linear(drop(v), w, w), x, use_reentrant=reentrant)
+    with pytest.raises(_lib.GfnError, match="recomputed inside a backward pass"):
+        y.sum().backward()
+    # outside of the recomputed part it has one mask: the gradients are those without recomputation
+    def grads(layer):
+        x.grad = w.grad = None
+        drop.counter.fill_(5)
+        drop(layer(x)).square().sum().backward()
+        return x.grad.clone(), w.grad.clone()
+
+    got = grads(lambda v: checkpoint(gated_linear, v, w, w, use_reentrant=reentrant))
+    assert all(T.equal(a, b) for a, b in zip(got, grads(lambda v: gated_linear(v, w, w)))) and int(drop.counter) == 6

@@ -1,5 +1,5 @@
 """The sequence-head operators without a GPU, where their numbers end: what the oracle's bounds let through, and calls whose outputs
-overlap their inputs, and the first call of two threads at once."""
+overlap their inputs, the first call of two threads at once, and the dropout module's masks."""
 import ctypes as C
 import os
 import subprocess
@@ -144,3 +144,28 @@ def test_two_threads_in_a_first_call_both_run_its_set_up(tmp_path):
     exe = str(tmp_path / "once")
     subprocess.check_call(["g++", "-O2", "-std=c++17", "-pthread", "-I", os.path.join(ROOT, "gf-nerf_amd", "csrc"), str(tmp_path / "once.cpp"), "-o", exe])
     assert subprocess.check_output([exe], text=True, timeout=60) == "1 0 1 0 1 1 1"
+
+
+# ---- dropout's masks ----------------------------------------------------------------------------------------------------------------------------
+def test_a_dropout_inside_a_backward_pass_is_refused():
+    """Recomputation (torch.utils.checkpoint) runs a forward again inside the backward pass.  In eval mode and with p = 0 there is no mask to differ."""
+    import torch
+
+    from gfnerf_amd import _lib
+    from gfnerf_amd.gfnerf.mlp import Dropout
+
+    class Again(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, module):
+            ctx.module = module
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            return ctx.module(g), None
+
+    x = torch.ones(4, 8, requires_grad=True)
+    with pytest.raises(_lib.GfnError, match="recomputed inside a backward pass"):
+        Again.apply(x, Dropout(0.5)).sum().backward()
+    Again.apply(x, Dropout(0.5).eval()).sum().backward()
+    Again.apply(x, Dropout(0.0)).sum().backward()
