@@ -10,7 +10,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 from torch.utils.weak import WeakIdKeyDictionary
 
-from .. import _lib, ops
+from .. import _lib, dist, ops
 
 
 class _LinearFn(torch.autograd.Function):
@@ -122,14 +122,20 @@ class _DropoutFn(torch.autograd.Function):
 class Dropout(nn.Module):
     """Dropout over the last dimension with a mask that is never stored (ops.dropout): a function of the module's seed, the number of its
     forward passes in training mode (`counter`, on the device: replayed graphs draw fresh masks), the row and the column.  Every forward pass
-    draws a mask of its own, so one that is run again inside a backward pass is refused."""
+    draws a mask of its own, so one that is run again inside a backward pass is refused.  seed: default, a number from torch's generator
+    (torch.manual_seed), so that modules differ; a copy of a module draws the module's masks.  The ranks of a distributed run differ whatever
+    the seed."""
 
-    def __init__(self, p: float = 0.5, seed: int = 0):
+    def __init__(self, p: float = 0.5, seed=None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p = {p} is not in [0, 1]")
-        self.p, self.seed = float(p), int(seed)
+        self.p, self.seed = float(p), int(torch.randint(1 << 62, (), device="cpu")) if seed is None else int(seed)
         self.register_buffer("counter", torch.zeros(1, dtype=torch.int64))
+
+    def key(self):
+        """The masks' key on this rank (rank 0, and without a process group: the seed)."""
+        return (self.seed + dist.rank() * 0x9E3779B97F4A7C15) & 0xFFFFFFFFFFFFFFFF
 
     def forward(self, x):
         if not self.training or self.p == 0.0:
@@ -138,7 +144,7 @@ class Dropout(nn.Module):
             raise _lib.GfnError("a dropout is recomputed inside a backward pass (torch.utils.checkpoint): it would draw another mask than its first forward; "
                                 "leave it outside of the recomputed part (it keeps nothing of its input)")
         alive = one_graph_at_a_time(x)
-        return _DropoutFn.apply(x.reshape(-1, x.shape[-1]).contiguous(), self.p, self.seed, ops.dropout_call(self.counter), alive).reshape(x.shape)
+        return _DropoutFn.apply(x.reshape(-1, x.shape[-1]).contiguous(), self.p, self.key(), ops.dropout_call(self.counter), alive).reshape(x.shape)
 
 
 class GatedLayer(nn.Module):
@@ -154,12 +160,12 @@ class GatedLayer(nn.Module):
 
 class GatedMLPNetwork(nn.Module):
     """MLPNetwork's arguments and call with gated hidden layers: network_config["activation"] is "SwiGLU", "GEGLU", "ReGLU" or "GLU";
-    network_config["dropout"] (default 0) is applied behind every hidden layer in training mode.  Computes in f32 like MLPNetwork;
+    network_config["dropout"] (default 0) is applied behind every hidden layer in training mode, with seeds seed, seed + 1, .. (default: Dropout's).  Computes in f32 like MLPNetwork;
     at most 128 inputs and 128 neurons (the layers' kernels)."""
 
     ACTIVATIONS = {"SwiGLU": "silu", "GEGLU": "gelu", "ReGLU": "relu", "GLU": "sigmoid"}
 
-    def __init__(self, n_input_dims, n_output_dims, network_config, seed=1337):
+    def __init__(self, n_input_dims, n_output_dims, network_config, seed=None):
         super().__init__()
         if network_config["activation"] not in self.ACTIVATIONS:
             raise ValueError(f"activation {network_config['activation']!r} is none of {sorted(self.ACTIVATIONS)}")
@@ -171,7 +177,7 @@ class GatedMLPNetwork(nn.Module):
         self.layers = nn.ModuleList(GatedLayer(a, b, act) for a, b in zip(widths, widths[1:]))
         self.layers.append(nn.Linear(widths[-1], n_output_dims))
         p = float(network_config.get("dropout", 0.0))
-        self.dropout = nn.ModuleList(Dropout(p, seed + i) for i in range(self.n_hidden_layers)) if p else None
+        self.dropout = nn.ModuleList(Dropout(p, None if seed is None else seed + i) for i in range(self.n_hidden_layers)) if p else None
 
     def forward(self, x):
         out, shape = self.layers[-1], x.shape[:-1]

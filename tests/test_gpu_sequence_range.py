@@ -426,3 +426,14 @@ def test_a_recomputed_dropout_is_refused(T, reentrant):
 
     got = grads(lambda v: checkpoint(gated_linear, v, w, w, use_reentrant=reentrant))
     assert all(T.equal(a, b) for a, b in zip(got, grads(lambda v: gated_linear(v, w, w)))) and int(drop.counter) == 6
+
+
+def test_default_dropout_modules_draw_masks_of_their_own(T):
+    """Two layers of one width, each in its first call: 64,000 pairs of fair coins agree in half, within five standard deviations."""
+    from gfnerf_amd.gfnerf.mlp import Dropout
+
+    x = T.ones(1000, 64, device="cuda")
+    a, b = Dropout(0.5).cuda(), Dropout(0.5).cuda()
+    masks = [m(x) != 0 for m in (a, b, a)]
+    for p, q in ((0, 1), (0, 2), (1, 2)):
+        assert abs(float((masks[p] == masks[q]).double().mean()) - 0.5) < 5 * 0.5 / 64000 ** 0.5

@@ -169,3 +169,28 @@ def test_a_dropout_inside_a_backward_pass_is_refused():
         Again.apply(x, Dropout(0.5)).sum().backward()
     Again.apply(x, Dropout(0.5).eval()).sum().backward()
     Again.apply(x, Dropout(0.0)).sum().backward()
+
+
+def test_dropout_modules_and_ranks_have_masks_of_their_own(monkeypatch):
+    import torch
+
+    from gfnerf_amd import dist
+    from gfnerf_amd.gfnerf.mlp import Dropout, GatedMLPNetwork
+
+    spec = {"activation": "SwiGLU", "output_activation": "None", "n_neurons": 16, "n_hidden_layers": 3, "dropout": 0.1}
+    seeds = [m.seed for net in (GatedMLPNetwork(8, 4, spec), GatedMLPNetwork(8, 4, spec)) for m in net.dropout] + [Dropout().seed, Dropout().seed]
+    assert len(set(seeds)) == 8
+    torch.manual_seed(3)
+    first = [Dropout().seed, Dropout().seed]
+    torch.manual_seed(3)
+    assert [Dropout().seed, Dropout().seed] == first
+    assert Dropout(0.5, 7).seed == 7 and [m.seed for m in GatedMLPNetwork(8, 4, spec, seed=1337).dropout] == [1337, 1338, 1339]
+    module, keys = Dropout(0.5, 7), []
+    assert module.key() == 7  # without a process group
+    for rank in range(8):
+        monkeypatch.setattr(dist, "rank", lambda group=None: rank)
+        keys += [module.key(), Dropout(0.5, 8).key()]
+    assert len(set(keys)) == 16 and all(0 <= k < 1 << 64 for k in keys) and keys[0] == 7
+    kept = [oseq.dropout_mask(200, 64, 0.5, k, 0)[0] for k in keys[::2]]
+    for i in range(1, 8):  # 12,800 pairs of fair coins: half of them agree, within five standard deviations
+        assert abs((kept[0] == kept[i]).mean() - 0.5) < 5 * 0.5 / np.sqrt(12800)
