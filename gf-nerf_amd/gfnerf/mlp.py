@@ -86,7 +86,7 @@ def one_graph_at_a_time(*tensors):
 class _GatedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, Wg, Wu, bg, bu, act, alive):
-        Wg, Wu = Wg.contiguous(), Wu.contiguous()
+        Wg, Wu, bg, bu = (t if t is None else t.contiguous() for t in (Wg, Wu, bg, bu))
         h = ops.gated_fwd(x, Wg, Wu, bg, bu, act)
         ctx.save_for_backward(x, Wg, Wu, bg, bu)
         ctx.act, ctx.alive = act, alive

@@ -437,3 +437,19 @@ def test_default_dropout_modules_draw_masks_of_their_own(T):
     masks = [m(x) != 0 for m in (a, b, a)]
     for p, q in ((0, 1), (0, 2), (1, 2)):
         assert abs(float((masks[p] == masks[q]).double().mean()) - 0.5) < 5 * 0.5 / 64000 ** 0.5
+
+
+# ---- arguments of the autograd functions ------------------------------------------------------------------------------------------------------
+def test_gated_linear_takes_parameters_of_any_strides(T):
+    from gfnerf_amd.gfnerf.mlp import gated_linear
+
+    x = T.randn(70, 24, device="cuda", requires_grad=True)
+    wide = T.randn(24, 40, 2, device="cuda", requires_grad=True)
+    flat = T.randn(40, 4, device="cuda", requires_grad=True)
+    params = lambda: [wide[:, :, 0].t(), wide[:, :, 1].t(), flat[:, 1], flat[:, 3]]  # noqa: E731
+    got = gated_linear(x, *params())
+    want = gated_linear(x, *(p.contiguous() for p in params()))
+    assert T.equal(got, want)
+    g = T.randn(70, 40, device="cuda")
+    for a, b in zip(T.autograd.grad(got, (x, wide, flat), g), T.autograd.grad(want, (x, wide, flat), g)):
+        assert T.equal(a, b)
