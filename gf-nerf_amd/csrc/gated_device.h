@@ -178,7 +178,7 @@ __device__ __forceinline__ void gated8(F g, U u, float (&v)[8]) {
       for (int i = 0; i < 8; i++) v[i] = sigmoid<EXACT>(g(i)) * u(i);
   }
 }
-// dg[i] = d[i] u[i] act'(g[i]), du[i] = d[i] act(g[i])
+// dg[i] = d[i] u[i] act'(g[i]), du[i] = d[i] act(g[i]).  A NaN stays one.
 template <int ACT, bool EXACT, typename F, typename U>
 __device__ __forceinline__ void gated8_grad(F g, U u, const float (&d)[8], float (&dg)[8], float (&du)[8]) {
   switch (ACT) {
@@ -202,7 +202,7 @@ __device__ __forceinline__ void gated8_grad(F g, U u, const float (&d)[8], float
     case GATED_RELU:
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        dg[i] = (g(i) > 0.f ? d[i] * u(i) : 0.f);
+        dg[i] = g(i) > 0.f ? d[i] * u(i) : (g(i) <= 0.f ? 0.f : g(i));
         du[i] = (d[i] * (g(i) < 0.f ? 0.f : g(i)));
       }
       break;

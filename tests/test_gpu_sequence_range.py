@@ -453,3 +453,19 @@ def test_gated_linear_takes_parameters_of_any_strides(T):
     g = T.randn(70, 40, device="cuda")
     for a, b in zip(T.autograd.grad(got, (x, wide, flat), g), T.autograd.grad(want, (x, wide, flat), g)):
         assert T.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
+def test_an_undefined_gate_makes_its_features_gradients_undefined(T, ops, kind, act):
+    """g of one feature is NaN: h, the gradients of that feature's weights and biases, and dx (a sum over all features) are; the other features' are not."""
+    x, wg, wu, bg, bu, dh = gated_inputs(T, kind, 90, 20, 40, True, act)
+    bad = bg[0].clone()
+    bad[7] = float("nan")
+    want = ops.gated_bwd(x[0], wg[0], wu[0], dh[0], bg[0], bu[0], act)
+    dx, dwg, dwu, dbg, dbu = ops.gated_bwd(x[0], wg[0], wu[0], dh[0], bad, bu[0], act)
+    h = ops.gated_fwd(x[0], wg[0], wu[0], bad, bu[0], act)
+    rest = T.arange(40, device="cuda") != 7
+    assert bool(T.isnan(h[:, 7]).all()) and bool(T.isfinite(h[:, rest]).all()) and bool(T.isnan(dx).all())
+    for got, clean in zip((dwg, dwu, dbg, dbu), want[1:]):
+        assert bool(T.isnan(got[7]).all()) and T.equal(got[rest], clean[rest])
