@@ -38,10 +38,11 @@ def ray_scan(pts_offsets, f, c, gate="sigmoid", reverse=False, h0=None, leaves=(
 def render_features(pts_offsets, sigma, dt, features):
     """Composite `features` [n, channels] along each ray with the weights T_i alpha_i, alpha = 1 - exp(-sigma dt) (RaySamples.get_weights_f2nerf,
     nerfstudio/cameras/rays.py:178-200) -> f32 [rays, channels]; gradients for sigma, dt and features.  The sum over a ray is the recurrence
-    h = exp(-sigma dt) h + alpha c taken back to front: no weights array, any number of channels.  sigma dt is formed in f32 and rounded once
-    to the features' dtype (the recurrence takes its gates and inputs in one type): with 16-bit features a weight is off by half a step of it."""
-    thickness = (sigma.reshape(-1) * dt.reshape(-1)).to(features.dtype)
-    return ray_scan(pts_offsets, thickness[:, None], features, "decay", reverse=True, leaves=(sigma, dt))[1]
+    h = exp(-sigma dt) h + alpha c taken back to front: no weights array, any number of channels.  All of it is in f32 whatever the features'
+    dtype (the recurrence takes its gates and inputs in one type, and a sigma dt of 16 bits would be off by 2^-9 of itself in every factor of the
+    transmittance): features of 16 bits are cast."""
+    thickness = sigma.reshape(-1).float() * dt.reshape(-1).float()
+    return ray_scan(pts_offsets, thickness[:, None], features.float(), "decay", reverse=True, leaves=(sigma, dt, features))[1]
 
 
 class RayRecurrence(nn.Module):

@@ -469,3 +469,29 @@ def test_an_undefined_gate_makes_its_features_gradients_undefined(T, ops, kind, 
     assert bool(T.isnan(h[:, 7]).all()) and bool(T.isfinite(h[:, rest]).all()) and bool(T.isnan(dx).all())
     for got, clean in zip((dwg, dwu, dbg, dbu), want[1:]):
         assert bool(T.isnan(got[7]).all()) and T.equal(got[rest], clean[rest])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_render_features_weighs_in_f32_whatever_the_features_type(T, kind):
+    """The composite of 16-bit features is that of their f32 values: within the oracle's f32 bound of the 64-bit one, gradients of sigma and dt too."""
+    from gfnerf_amd.gfnerf.ray_scan import render_features
+
+    rng = np.random.default_rng(6)
+    lens = rng.integers(0, 120, 40)
+    off = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    n = int(off[-1])
+    leaf = lambda v, k="f32": T.from_numpy(v).to(dt(T, k)).cuda().requires_grad_(True)  # noqa: E731
+    sigma, delta, feats = leaf(rng.exponential(0.5, n)), leaf(rng.uniform(0.01, 0.2, n)), leaf(rng.standard_normal((n, 12)), kind)
+    out = render_features(T.from_numpy(off).cuda(), sigma, delta, feats)
+    g = T.from_numpy(rng.standard_normal((40, 12))).float().cuda()
+    ds, dd, df = T.autograd.grad(out, (sigma, delta, feats), g)
+    thick = sigma.detach() * delta.detach()  # the same f32 product
+    wide = lambda t: t.detach().double().cpu().numpy()  # noqa: E731
+    want = oseq.ray_scan(off, wide(thick)[:, None], wide(feats), "decay", True, "f32", None, np.zeros((n, 12)), wide(g))
+    close(out.detach(), want["state"], "state")
+    dthick, bound = (v[:, 0] for v in want["df"])
+    for got, other, what in ((ds, delta, "sigma"), (dd, sigma, "dt")):
+        o = wide(other)
+        close(got, (dthick * o, bound * o + np.abs(dthick * o) * oseq.U), what)
+    assert df.dtype == feats.dtype
+    close(df, (want["dc"][0], oseq.rounded(want["dc"][0], want["dc"][1], kind)), "features")
