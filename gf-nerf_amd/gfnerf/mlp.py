@@ -138,7 +138,7 @@ class Dropout(nn.Module):
         return (self.seed + dist.rank() * 0x9E3779B97F4A7C15) & 0xFFFFFFFFFFFFFFFF
 
     def forward(self, x):
-        if not self.training or self.p == 0.0:
+        if not self.training or self.p == 0.0 or 0 in x.shape[-1:]:
             return x
         if torch._C._current_graph_task_id() != -1:
             raise _lib.GfnError("a dropout is recomputed inside a backward pass (torch.utils.checkpoint): it would draw another mask than its first forward; "

@@ -194,3 +194,13 @@ def test_dropout_modules_and_ranks_have_masks_of_their_own(monkeypatch):
     kept = [oseq.dropout_mask(200, 64, 0.5, k, 0)[0] for k in keys[::2]]
     for i in range(1, 8):  # 12,800 pairs of fair coins: half of them agree, within five standard deviations
         assert abs((kept[0] == kept[i]).mean() - 0.5) < 5 * 0.5 / np.sqrt(12800)
+
+
+def test_dropout_of_rows_without_columns_is_the_rows():
+    import torch
+
+    from gfnerf_amd.gfnerf.mlp import Dropout
+
+    for shape in ((4, 0), (2, 3, 0), (0, 0)):
+        x = torch.zeros(shape)
+        assert Dropout(0.5)(x) is x
