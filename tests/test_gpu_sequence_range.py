@@ -193,14 +193,15 @@ def gates(T, kind, gate, n, g, seed):
 @pytest.mark.parametrize("gate", ["linear", "sigmoid", "decay"])
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("bad", ["nan", "large"])
-def test_gates_of_one_ray_do_not_reach_the_next_in_runs(T, ops, kind, gate, reverse, bad):
+@pytest.mark.parametrize("g", [8, 1])
+def test_gates_of_one_ray_do_not_reach_the_next_in_runs(T, ops, kind, gate, reverse, bad, g):
     """Undefined gates in the middle of a ray, and gates whose product passes f32's range: the other rays' states, outputs and gradients are those of a
     call without them, bit for bit."""
     off = T.tensor(np.concatenate([[0], np.cumsum(LONG)]), dtype=T.int32, device="cuda")
     n, d = sum(LONG), 8
     rng = np.random.default_rng(1)
     made = lambda *s: T.from_numpy(rng.standard_normal(s))  # noqa: E731
-    f, c, dh = gates(T, kind, gate, n, d, 0), made(n, d).to(dt(T, kind)).cuda(), made(n, d).to(dt(T, kind)).cuda()
+    f, c, dh = gates(T, kind, gate, n, g, 0), made(n, d).to(dt(T, kind)).cuda(), made(n, d).to(dt(T, kind)).cuda()
     h0, ds = made(3, d).float().cuda(), made(3, d).float().cuda()
 
     def call(f):
@@ -211,12 +212,12 @@ def test_gates_of_one_ray_do_not_reach_the_next_in_runs(T, ops, kind, gate, reve
     clean_rows, clean_rays = call(f)
     for ray in range(3):
         s, e = sum(LONG[:ray]), sum(LONG[:ray + 1])
-        g = f.clone()
+        other = f.clone()
         if bad == "nan":
-            g[s + 700:s + 703] = float("nan")
+            other[s + 700:s + 703] = float("nan")
         else:
-            g[s + 100:e - 100] = {"linear": 20.0, "sigmoid": 80.0, "decay": -3.0}[gate]
-        rows, rays = call(g)
+            other[s + 100:e - 100] = {"linear": 20.0, "sigmoid": 80.0, "decay": -3.0}[gate]
+        rows, rays = call(other)
         keep = T.ones(n, dtype=T.bool, device="cuda")
         keep[s:e] = False
         for a, b in zip(rows, clean_rows):
@@ -495,3 +496,27 @@ def test_render_features_weighs_in_f32_whatever_the_features_type(T, kind):
         close(got, (dthick * o, bound * o + np.abs(dthick * o) * oseq.U), what)
     assert df.dtype == feats.dtype
     close(df, (want["dc"][0], oseq.rounded(want["dc"][0], want["dc"][1], kind)), "features")
+
+
+def test_gated_f16_tiles_of_very_different_size_in_one_workgroups_run(T, ops):
+    """dz of 2^35 in some tiles, whose dW passes f16 in column 0 and is nothing elsewhere, and of 2^-16 in the tiles that the same workgroups take before
+    and behind them (more tiles than workgroups): the other columns are sums of the small tiles alone, and keep f16's precision."""
+    n, k, h = 66000, 8, 32
+    rng = np.random.default_rng(8)
+    big = np.isin(np.arange(n) // 64, np.r_[0:256, 768:1032])
+    x = np.where(big[:, None], np.eye(1, k) * 6e4, rng.standard_normal((n, k)) * 1e-2)
+    x[~big, 0] = 0
+    wg, wu, dh = rng.standard_normal((h, k)), rng.standard_normal((h, k)), rng.standard_normal((n, h)) * np.where(big, 1024.0, 2.0 ** -10)[:, None]
+    wg[:, 0], wu[:, 0] = 600, 600
+    x, wg, wu, dh = ((lambda t: (t.cuda(), t.double().numpy()))(T.from_numpy(v).to(T.float16)) for v in (x, wg, wu, dh))
+    want = oseq.gated_bwd(x[1], wg[1], wu[1], dh[1], None, None, "relu", "f16")
+    got = dict(zip(NAMES, ops.gated_bwd(x[0], wg[0], wu[0], dh[0], act="relu")))
+    small = T.from_numpy(~big).cuda()
+    close(got["dx"][small], tuple(v[~big] for v in want["dx"]), "dx")
+    for name in ("dwg", "dwu"):
+        value, bound = want[name]
+        assert bool((~T.isfinite(got[name][:, 0])).any())
+        v = got[name][:, 1:].double().cpu().numpy()
+        # (the oracle's bound on dW holds the large tiles' share of the grid against the small ones' sums only where x is not zero)
+        assert (np.abs(v - value[:, 1:]) <= bound[:, 1:]).all(), name
+        assert np.linalg.norm(v - value[:, 1:]) <= 2.0 ** -11 * np.linalg.norm(value[:, 1:]) + 2.0 ** -25 * np.sqrt(v.size), name
