@@ -17,16 +17,18 @@
 // and travel as column k of the partials.
 // 16-bit: dz goes into both products as several operands of the type (dz_operands), not rounded to one.  bf16: three, which are dz itself;
 // of 33 million values of dx in the case below 5,300 then differ from their rounded 64-bit values (f32 torch: 7,600; two operands, 17 bits:
-// 80,000, and one: two in five), for 176 us instead of 141 and 115 a call.  f16: two, 22 bits, under powers of two taken from
-// the |dz| themselves (power_of); 28,400 of 12.8 million values of dx at 100k x 128 -> 128 differ (f32 torch: 28,200), for 89 instead of 83 us.
+// 80,000, and one: two in five), for 180 us instead of 141 and 115 a call.  f16: two, 22 bits, under powers of two taken from
+// the |dz| themselves (power_of); 28,400 of 12.8 million values of dx at 100k x 128 -> 128 differ (f32 torch: 28,200; a power
+// from |dh| alone: 79,000), for 91 instead of 84 us.
 //
-// What bounds them.  Forward, 786k x 63 -> 128 bf16 silu: 92 us for 300 MB (a copy of that size: 55); four waves a SIMD, requests a tile
-// ahead; relu takes as long, rows of 64 instead of 63 16 % less (odd rows start at any 2 bytes).  262k x 32 -> 128 f32 gelu: 66 us, of
-// which the matrix pipe is busy 27 (f32 products run at 1/8 of bf16's rate) and vector instructions issue for 30; the two hardly overlap.
-// Backward, 524k x 63 -> 128 bf16: 176 us with the reduction's 7, 266 MB (a copy: 49).  Two waves a SIMD (W's image, x, dz and dW's
-// accumulators fill LDS and registers); a tile's vector instructions, LDS reads and products, a third of its time each, add up rather
-// than overlap.  100k x 128 -> 128 f16: 89 with the reduction's 13; 50k x 32 -> 64 f32: 29 + 5, 64 % of it the
-// matrix pipe.
+// What bounds them (times without a profiler, shares of the kernel's cycles from counters: matrix pipe, vector issue, LDS).
+// Forward, 786k x 63 -> 128 bf16 silu: 92 us for 300 MB (a copy of that size: 55); four waves a SIMD, requests a tile ahead.  No unit is full
+// (11, 43, 10 %); rows that start at any 2 bytes cost 16 % (64 columns), and what holds the rest is not known.  262k x 32 -> 128 f32 gelu:
+// 65 us; products (f32's run at 1/8 of bf16's rate) take 41 % and vector instructions 44 %, one after the other for the most part.
+// Backward, two waves a SIMD (W's image, x, dz and dW's accumulators fill LDS and registers), whose vector instructions, LDS reads and
+// products add up rather than overlap.  524k x 63 -> 128 bf16: 180 us a call, the reduction's 7 included, for 266 MB (a copy: 49); 31, 46 and
+// 48 %.  100k x 128 -> 128 f16: 91 with the reduction's 13, four rounds of tiles for 3.05 of samples; 17, 35 and 27 %.  50k x 32 -> 64 f32: 29
+// + 5, two rounds for 1.5; 23, 16 and 10 %.
 #include "gated_device.h"
 
 namespace {
@@ -224,8 +226,8 @@ __device__ __forceinline__ u32x2 tr4(const char* a) {
 }
 
 // waves a workgroup of the backward: eight where the weights' images leave a CU one workgroup, four where two fit and wait for their
-// barriers apart from each other (us for both launches, ten calls in a row, eight / four: 262k x 63 -> 64 bf16 64 / 50, 524k x 20 -> 128
-// bf16 120 / 105, 262k x 96 -> 128 bf16 113 / 149, 100k x 128 -> 128 f16 89 / 98)
+// barriers apart from each other (us a call, eight / four: 524k x 63 -> 128 bf16 200 / 183, f16 208 / 182; 524k x 20 -> 128 bf16 126 / 115, f16
+// 157 / 137; 262k x 96 -> 128 bf16 121 / 165, f16 122 / 169; 100k x 128 -> 128 bf16 88 / 102)
 constexpr int bwd_waves(int ks) { return ks == 3 || ks == 4 ? 8 : 4; }
 
 // dz as the operands of its products.  bf16: three, each the upper eight of the bits that the one before left -- 24 in all, so their sum is dz
@@ -268,8 +270,8 @@ constexpr int bwd_lds(int dtype, int ks, int np, int buffers) {
   return 64 * np * (ks * 64 + 16 + 4) + 16 * bwd_waves(ks) * (ks * 64 + 16 + buffers * bwd_ztile(dtype) + bwd_pad(dtype)) + 64;
 }
 // Pairs of feature tiles whose dz are kept at once, all, two or one, as many as fit without costing the CU its second workgroup: dW's product
-// reads x once for them, between two barriers.  (As many / one at a time: 262k x 96 -> 128 bf16 113 / 121 us, 262k x 63 -> 64 bf16 50 / 55,
-// 100k x 48 -> 128 f32 132 / 145.)
+// reads x once for them, between two barriers.  (As many / one at a time: 262k x 96 -> 128 f32 862 / 969 us, f16 122 / 126;
+// 100k x 48 -> 128 f32 127 / 140.  bf16, whose dz are three operands, has room for one where rows are long.)
 constexpr int bwd_buffers(int dtype, int ks, int np) {
   const int room = bwd_lds(dtype, ks, np, 1) <= 80 * 1024 ? 80 * 1024 : 160 * 1024;
   return bwd_lds(dtype, ks, np, np) <= room ? np : np > 2 && bwd_lds(dtype, ks, np, 2) <= room ? 2 : 1;

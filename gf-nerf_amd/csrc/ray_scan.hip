@@ -283,7 +283,7 @@ struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 // Whether this block and the next are whole rows of the piece in every lane, with one more behind them.  Such blocks are worked on without
 // a branch, so that a wait for the next block's rows is not one for the stores behind their requests (loads and stores are counted together,
-// in order): backward of 4096 rays x 192 rows x 128 channels in bf16 255 -> 237 us, a first reading 21 -> 19 and 20 -> 18 us.
+// in order): backward of 4096 rays x 192 rows x 128 channels in bf16 255 -> 237 us, a first reading of 2 x 131072 x 64 f16 21 -> 19 us (then without the exponents).
 template <typename F>
 __device__ __forceinline__ bool inner(int64_t i, int64_t blocks, int64_t lo, int64_t hi, F base_of, bool active) {
   if (!__all(active && i + 2 < blocks)) return false;
@@ -540,8 +540,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
 
 // AGG's steps -> the state in front of every run (in the walk's order).  A workgroup: one channel, 1,024 stretches of neighbouring runs, each
 // composed in registers (up to kHeld runs of a stretch; more are read twice), the stretches joined by doubling within a wave and the
-// waves' steps one after the other.  Latency bound: 5 us for 4,096 runs of 64 channels; with the steps as [runs][channels], four
-// channels a workgroup, 18 us -- every load then takes 32 bytes of a line, on a quarter of the CUs.
+// waves' steps one after the other.  Latency bound: 9 us for 4,096 runs of 64 channels.  (Steps without an exponent: 5,
+// and laid out as [runs][channels], four channels a workgroup, 18 -- every load then takes a part of a line, on a quarter of the CUs.)
 constexpr int kHeld = 4, kPrefixWaves = 16;
 __device__ __forceinline__ Step step_up(const Step& q, int by) {
   return {__shfl_up(q.m, by, 64), __shfl_up(q.e, by, 64), __shfl_up(q.s, by, 64), __shfl_up(q.begins, by, 64)};
@@ -630,9 +630,17 @@ bool two_channels(const ScanArgs& a, bool shared, bool bwd) {
   return strides % 2 == 0 && at % 4 == 0;
 }
 
-// Rays or runs.  A walk along a ray waits 0.27 us a row where rays do not fill the chip; runs read everything twice and stop at every ray's
-// beginning.  us, bf16 forward, runs / rays: 16 rays x 2048 rows x 32 channels 19 / 453, 512 x 512 x 128 87 / 139, 1024 x 192 x 64 58 / 55,
-// 512 x 128 x 64 33 / 37, 1024 x 100 x 8 42 / 31, 2048 x 128 x 32 65 / 40, 4096 x 192 x 128 245 / 154.
+// Rays or runs.  A walk along a ray waits 0.13 to 0.3 us a row where rays do not fill the chip; runs read everything twice and stop at every
+// ray's beginning.  One rule for every type, gate and direction, by the rays' mean length; us of a call, rays of EQUAL lengths (of spread lengths
+// the longest decides a walk along rays: 512 x 512 x 128 bf16 139 instead of 82), runs / rays:
+//                                     bf16 forward   bf16 backward   f32 forward   f32 backward   one gate, bf16 backward
+//   16 rays x 2048 rows x 32 channels   22 / 261        24 / 284       24 / 366      26 / 380        30 / 593
+//   512 x 512 x 128                     82 / 82         97 / 99       160 / 128     193 / 167        87 / 169
+//   512 x 128 x 64                      27 / 22         31 / 25        33 / 30       36 / 31         37 / 46
+//   1024 x 192 x 64                     43 / 35         48 / 34        60 / 44       67 / 46         48 / 65
+//   1024 x 100 x 8                      36 / 18         44 / 22        42 / 23       49 / 27         58 / 38
+//   512 x 1024 x 256                   299 / 219       368 / 259      551 / 314     676 / 452       293 / 344
+//   4096 x 192 x 128                   232 / 130       276 / 178      443 / 247     532 / 332       227 / 156
 bool use_runs(int64_t rays, int64_t n_max, int d) {
   const int64_t mean = rays > 0 ? n_max / rays : 0;
   return mean >= 96 && rays < 6 * mean && rays * d < 128 * 1024;
