@@ -1467,8 +1467,9 @@ def gated_fwd(x, Wg, Wu, bg=None, bu=None, act="silu", out=None, n_dev=None):
 
 def gated_bwd(x, Wg, Wu, dh, bg=None, bu=None, act="silu", need_dx=True, need_dw=True, n_dev=None):
     """Gradients of gated_fwd for dh -> (dx, dWg, dWu, dbg, dbu); None for what is not wanted or not there.  The projections are formed
-    again from x (the forward saves nothing); the weights' gradients are sums in a fixed order, rounded once to x's dtype.  n_dev as in the
-    forward: dx's rows behind the live ones are not written."""
+    again from x (the forward saves nothing); the weights' gradients are sums in a fixed order, rounded once to x's dtype.  Their terms are not
+    rounded to 16 bits first: bf16's are f32's, f16's have 22 bits down to 2^-30 of the largest of their sample (dx) or of their tile of up to 128
+    samples (dW).  n_dev as in the forward: dx's rows behind the live ones are not written."""
     n, k, h, ldx, dtype = _gated_args(x, Wg, Wu, bg, bu, act, n_dev, "gated_bwd")
     lddh = _rows(dh, "dh", dtype, h, n)[2]
     stream = _place(x, Wg, Wu, bg, bu, n_dev, dh)
@@ -1579,7 +1580,7 @@ def dropout_call(counter):
 
 
 def dropout(x, p, seed, call, out=None):
-    """y = x where the element is kept, times 65536 / (65536 - t), t = round(65536 p); 0 where it is dropped.  Which elements are kept is a
+    """y = x where the element is kept, times 65536 / (65536 - t), t = round(65536 p) of p in f32; 0 where it is dropped.  Which elements are kept is a
     function of (seed, call, row, column) -- Philox4x32-10, 16 bits an element -- and never stored: the gradient is the same call on dy.
     x [n, columns] (f32, bf16 or f16, rows at any stride), call i64 [1] (dropout_call); out may be x, but not
     overlap it otherwise."""

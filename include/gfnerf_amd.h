@@ -768,7 +768,8 @@ int gfn_gated_fwd(const void* x, int64_t ldx, const void* wg, const void* wu, co
  * given exactly when the biases and dwg are.  All gradients are WRITTEN (not added to) in type dtype, each rounded once from an f32
  * sum taken in a fixed order: a call repeats its bits.  The intermediate gradients of the two projections enter the products of
  * bf16 as three numbers of bf16 each, which are their f32 values, and those of f16 as two (22 bits, under powers of two that follow
- * their size: each sample's own for dx, one for a tile of up to 128 samples and 32 features for dwg, dwu and the biases).  workspace: gfn_gated_bwd_workspace bytes of device memory, 16-byte aligned, owned by the call until its work is done
+ * their size: each sample's own for dx, one for a tile of up to 128 samples and 32 features for dwg, dwu and the biases, so
+ * that of a term 2^-30 of its sample's or tile's largest is cut off).  workspace: gfn_gated_bwd_workspace bytes of device memory, 16-byte aligned, owned by the call until its work is done
  * (two calls in flight need two). */
 int64_t gfn_gated_bwd_workspace(int64_t n_max, int in_dim, int hidden, int dtype, int bias, int need_dx, int need_dw);
 int gfn_gated_bwd(const void* x, int64_t ldx, const void* wg, const void* wu, const void* bg, const void* bu,
